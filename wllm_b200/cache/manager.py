@@ -11,6 +11,11 @@ tokens of a sequence, which such a group may keep readable behind the window, st
 either every request of the step gets its pages or nothing changes and
 `OutOfPages` is raised, which is how the scheduler learns that it has to preempt.
 
+A request may be *forked*: the new one holds the full pages of the tokens that both have, together with the old one
+(`PagePool` counts the holders), and a copy of the page that is partly written, so that nobody writes to a page that
+somebody else reads.  Its per-request state is copied.  The whole cache may be given another number of pages
+(`resize`): the live pages are moved to the front of new pools.
+
 Beside the pages, every live request owns one *slot*: a row index into the state
 tensors (per-request state of fixed size that a mixer may declare, for instance a
 recurrent state) and, for the engine, a stable small integer for the request.
@@ -32,6 +37,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from ..kernels import ops
 from .pages import OutOfPages, PagePool
 
 
@@ -75,6 +81,7 @@ class RequestCache:
     closed: bool = False
     released_upto: list = field(default_factory=list)   # per group: pages below this index were given back
     version: int = 0           # bumped whenever a table changes (lets a reader cache a copy)
+    forked: int = 0            # tokens that were in front of it when it was forked, or of a request forked from it: it may share pages below that
 
 
 class CacheGroup:
@@ -82,14 +89,19 @@ class CacheGroup:
         self.spec = spec
         self.pool = PagePool(num_pages)
         self.page_size = page_size
-        self.pages = None               # keys and values of one size: one pool with a k|v axis
-        self.key_pages = self.value_pages = None      # value heads of their own size: two pools
         self.poison = poison
+        self.dtype, self.device = dtype, device
         self.v_head_dim = spec.v_head_dim or spec.head_dim
         self._item = torch.empty((), dtype=dtype).element_size() if dtype is not None else 4
+        self._allocate(num_pages)
+
+    def _allocate(self, num_pages: int) -> None:
+        spec, page_size, dtype, device = self.spec, self.page_size, self.dtype, self.device
+        self.pages = None               # keys and values of one size: one pool with a k|v axis
+        self.key_pages = self.value_pages = None      # value heads of their own size: two pools
         if device is not None:
             def pool(*shape):
-                return torch.full(shape, float("nan"), dtype=dtype, device=device) if poison else \
+                return torch.full(shape, float("nan"), dtype=dtype, device=device) if self.poison else \
                     torch.zeros(shape, dtype=dtype, device=device)
             if spec.values_in_keys:
                 self.key_pages = self.value_pages = pool(spec.layers, num_pages, spec.kv_heads, page_size, spec.head_dim)
@@ -102,15 +114,35 @@ class CacheGroup:
         self._views = [(self.pages[i, 0], self.pages[i, 1]) if self.pages is not None else (self.key_pages[i], self.value_pages[i])
                        for i in range(spec.layers)] if device is not None else []
 
+    def tensors(self) -> list:
+        """The pools, [layers, (k | v,) pages, kv heads, slots, head]."""
+        return [t for t in (self.pages, self.key_pages, None if self.spec.values_in_keys else self.value_pages) if t is not None]
+
     def give(self, pages: list) -> None:
-        """Pages go back to the pool; with `poison` their contents become NaN first (in stream order, so a step
-        still running has read them before)."""
-        if self.poison and pages:
-            for pool, axis in ((self.pages, 2), (self.key_pages, 1), (None if self.spec.values_in_keys else self.value_pages, 1)):
-                if pool is not None:
-                    pool.index_fill_(axis, torch.tensor(pages, dtype=torch.long, device=pool.device), float("nan"))
-        for page in pages:
-            self.pool.give(page)
+        """Pages go back to the pool, or lose a holder; with `poison` the contents of those that are free now become NaN (in
+        stream order, so a step still running has read them before)."""
+        freed = [page for page in pages if self.pool.give(page)]
+        if self.poison and freed:
+            for pool in self.tensors():
+                pool.index_fill_(pool.dim() - 4, torch.tensor(freed, dtype=torch.long, device=pool.device), float("nan"))
+
+    def resize(self, num_pages: int) -> dict:
+        """New pools of that many pages; the held pages move to their front.  {page before: page now}"""
+        try:
+            pool, moved = self.pool.renumbered(num_pages)
+        except OutOfPages as e:
+            raise OutOfPages(self.spec.name, e.needed, e.free) from None
+        old = self.tensors()
+        before = (self.pages, self.key_pages, self.value_pages, self._views)
+        try:
+            self._allocate(num_pages)
+            if moved and old:
+                ops.copy_pages([(a, b, list(moved), list(moved.values()), None) for a, b in zip(old, self.tensors())])
+        except BaseException:
+            self.pages, self.key_pages, self.value_pages, self._views = before
+            raise
+        self.pool = pool
+        return moved
 
     def keys(self, layer: int) -> torch.Tensor:
         return self._views[layer][0]
@@ -127,7 +159,7 @@ class StateSlots:
     """Rows of fixed-size per-request state: tensor `name` has shape [num_slots, *shape]."""
 
     def __init__(self, num_slots: int, specs: list, device):
-        self.num_slots = num_slots
+        self.num_slots, self.specs = num_slots, list(specs)
         self._free = list(range(num_slots - 1, -1, -1))
         self._held = [False] * num_slots
         self.tensors = {}
@@ -139,14 +171,18 @@ class StateSlots:
     def num_free(self) -> int:
         return len(self._free)
 
-    def take(self) -> int:
+    def take(self, zero: bool = True) -> int:
         if not self._free:
             raise OutOfPages("request slots", 1, 0)
         slot = self._free.pop()
         self._held[slot] = True
-        for t in self.tensors.values():   # a new request starts from zero state
+        for t in self.tensors.values() if zero else ():   # a new request starts from zero state
             t[slot].zero_()
         return slot
+
+    def rows(self) -> list:
+        """The state tensors as pools of pages of one slot."""
+        return [t.view(self.num_slots, 1, 1, -1) for t in self.tensors.values() if t.numel()]
 
     def give(self, slot: int) -> None:
         if not self._held[slot]:
@@ -178,6 +214,73 @@ class CacheManager:
                           released_upto=[0] * len(self.groups))
         self.live[request_id] = rc
         return rc
+
+    def fork(self, rc: RequestCache, request_id, num_tokens: int | None = None) -> RequestCache:
+        """A new request that begins with the first `num_tokens` committed tokens of `rc` (None: all of them): it holds their full
+        pages together with it, and gets a copy of the page that the last of them lie in and of the per-request state.  One page
+        of every group where num_tokens is no whole number of pages, and a slot; `OutOfPages` leaves everything as it was.  Per-request
+        state is that of all tokens, so a cache that has some forks at all of them; and a window must not have passed what the
+        token behind the first `num_tokens` reads."""
+        n = rc.num_tokens if num_tokens is None else num_tokens
+        if rc.closed or rc.reserved:
+            raise RuntimeError(f"request {rc.request_id!r} is " + ("closed" if rc.closed else "in a step"))
+        if not 0 <= n <= rc.num_tokens:
+            raise ValueError(f"request {rc.request_id!r} has {rc.num_tokens} tokens; it cannot be forked at {n}")
+        if n != rc.num_tokens and self.slots.specs:
+            raise ValueError(f"request {rc.request_id!r} has state of all its {rc.num_tokens} tokens; it cannot be forked at {n}")
+        if request_id in self.live:
+            raise KeyError(f"request {request_id!r} is already open")
+        ps = self.page_size
+        full, tail = n // ps, n % ps
+        for g, table in zip(self.groups, rc.tables):
+            seen = list(range(min(g.spec.first_needed(n), n) // ps, -(-n // ps)))
+            if g.spec.window is not None:
+                seen += range(min(-(-g.spec.keep_first // ps), -(-n // ps)))
+            if any(table[i] < 0 for i in seen):
+                raise ValueError(f"request {rc.request_id!r}: the window of group '{g.spec.name}' has passed tokens that are read behind the first {n}")
+            if tail and g.pool.num_free < 1:
+                raise OutOfPages(g.spec.name, 1, 0)
+        new = RequestCache(request_id, self.slots.take(zero=False), [], num_tokens=n, released_upto=[min(u, full) for u in rc.released_upto])
+        moves = []
+        for g, table in zip(self.groups, rc.tables):
+            mine = list(table[:full])
+            for page in mine:
+                if page >= 0:
+                    g.pool.share(page)
+            if tail:
+                mine.append(g.pool.take())
+                moves += [(t, t, [table[full]], [mine[-1]], [tail]) for t in g.tensors()]
+            new.tables.append(mine)
+        moves += [(t, t, [rc.slot], [new.slot], None) for t in self.slots.rows()]
+        try:
+            for i in range(0, len(moves), ops.MAX_COPY_POOLS):
+                ops.copy_pages(moves[i:i + ops.MAX_COPY_POOLS])
+        except BaseException:
+            for g, mine in zip(self.groups, new.tables):
+                g.give([page for page in mine if page >= 0])
+            self.slots.give(new.slot)
+            raise
+        rc.forked, new.forked = max(rc.forked, n), n
+        self.live[request_id] = new
+        self._note_high_water()
+        return new
+
+    def resize(self, num_pages: int) -> None:
+        """Another number of pages in every group, with the live pages at the front of the new pools (every table follows; whoever holds views
+        of the old pools asks for them again).  `OutOfPages` if some group holds more than that, and everything is as it was."""
+        if num_pages < 1:
+            raise ValueError("a pool needs at least one page")
+        for rc in self.live.values():
+            if rc.reserved:
+                raise RuntimeError(f"request {rc.request_id!r} is in a step")
+        for g in self.groups:
+            if g.pool.num_pages - g.pool.num_free > num_pages:
+                raise OutOfPages(g.spec.name, g.pool.num_pages - g.pool.num_free, num_pages)
+        for gi, g in enumerate(self.groups):
+            moved = g.resize(num_pages)
+            for rc in self.live.values():
+                rc.tables[gi] = [page if page < 0 else moved[page] for page in rc.tables[gi]]
+                rc.version += 1
 
     def close(self, rc: RequestCache) -> None:
         """Give back everything the request holds.  Closing twice is an error."""
@@ -222,6 +325,9 @@ class CacheManager:
                     table.append(g.pool.take())
                     rc.version += 1
             rc.reserved += n
+        self._note_high_water()
+
+    def _note_high_water(self) -> None:
         for gi, g in enumerate(self.groups):
             used = g.pool.num_pages - g.pool.num_free
             self.pages_high_water[gi] = max(self.pages_high_water[gi], used)
@@ -273,17 +379,22 @@ class CacheManager:
         return sum(g.bytes_per_token() for g in self.groups)
 
     def check(self) -> None:
-        """Every page is either free or in exactly one live table; used by the tests."""
+        """Every page is either free or in as many live tables as it has holders, at the same place and behind the same pages in all of them,
+        and no slot behind the tokens that its holders have in common is written by more than one of them; used by the tests."""
         for gi, g in enumerate(self.groups):
             seen = {}
             for rc in self.live.values():
-                for page in rc.tables[gi]:
+                for i, page in enumerate(rc.tables[gi]):
                     if page < 0:
                         continue
-                    if page in seen:
-                        raise AssertionError(f"group {g.spec.name}: page {page} held by {seen[page]!r} and {rc.request_id!r}")
                     if not g.pool.is_held(page):
                         raise AssertionError(f"group {g.spec.name}: page {page} is in a table but free")
-                    seen[page] = rc.request_id
+                    seen.setdefault(page, []).append((i, rc))
+            for page, held in seen.items():
+                who = [rc.request_id for _, rc in held]
+                if len(held) != g.pool.holders(page):
+                    raise AssertionError(f"group {g.spec.name}: page {page} held by {who!r}, counted {g.pool.holders(page)} times")
+                if len(held) > 1 and (len({i for i, _ in held}) > 1 or any((i + 1) * self.page_size > min(rc.num_tokens, rc.forked) for i, rc in held)):
+                    raise AssertionError(f"group {g.spec.name}: page {page} held by {who!r} at places where they do not agree")
             if len(seen) + g.pool.num_free != g.pool.num_pages:
                 raise AssertionError(f"group {g.spec.name}: {g.pool.num_pages - g.pool.num_free - len(seen)} pages lost")

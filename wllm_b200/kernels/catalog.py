@@ -11,6 +11,7 @@ FAMILIES = {
     "embedding": [{}],
     "norm": [{}],
     "rope_cache": [{}],
+    "cache_pages": [{}],
     "attention_simt": [{}],
     "activation": [{}],
     "linear_attention": [{}],

@@ -17,6 +17,7 @@ import functools
 import ctypes
 from ctypes import c_float, c_void_p
 
+import numpy as np
 import torch
 
 from .build import KernelBuildError, entry_address, load_family, load_host_calls
@@ -36,7 +37,8 @@ def sm_count() -> int:
             if torch.cuda.is_available() else 148
     return _sms
 _STATUS = {1: "element type not supported", 2: "size not supported", 3: "pointer or stride not aligned",
-           4: "size beyond the entry point's fixed scratch", 5: "device set-up failed"}
+           4: "size beyond the entry point's fixed scratch", 5: "device set-up failed", 7: "a page or a number of slots outside its pool",
+           8: "a page is a destination twice, or both destination and source", 9: "pools of one call overlap"}
 
 
 class KernelError(RuntimeError):
@@ -55,6 +57,15 @@ def _need_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise KernelError("the engine's kernels run on a CUDA device only; got a tensor on " + str(t.device))
+
+
+def _one_device(*tensors) -> None:
+    """Tensors of one call lie on the current device: launches go to its current stream."""
+    _need_cuda(*tensors)
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"a tensor on {t.device} in a call on cuda:{here}; make its device the current one (torch.cuda.device)")
 
 
 def _ptr(t) -> c_void_p:
@@ -755,6 +766,75 @@ def attention_mma_prefill(q, out, k_pages, v_pages, req_q_start, req_q_len, req_
         _check(status, f"attention_mma_prefill(head_dim={hd}, heads={nq}/{nkv})")
     global launches
     launches += 1
+
+
+class _PoolMoves(ctypes.Structure):
+    _fields_ = [("src", c_void_p), ("dst", c_void_p)] + [(name, ctypes.c_longlong) for name in ("outer", "src_pages", "dst_pages", "heads", "slots", "row_bytes", "moves")] + \
+        [(name, c_void_p) for name in ("src_list", "dst_list", "slot_list")]
+
+
+def _whole_numbers(values, name: str, count: int | None = None) -> np.ndarray:
+    """A list of page numbers, slots or lengths known on the host as an int32 array."""
+    if isinstance(values, torch.Tensor):
+        if values.is_cuda:
+            raise KernelError(f"{name} is known on the host: a list, an array or a tensor of the CPU")
+        values = values.numpy()
+    a = np.asarray(values)
+    if a.size == 0:
+        a = a.astype(np.int32)
+    if a.ndim != 1 or a.dtype.kind not in "iu" or (count is not None and a.shape[0] != count):
+        raise KernelError(f"{name} must be a list of whole numbers" + (f", {count} of them" if count is not None else ""))
+    if a.size and not (-(1 << 31) <= int(a.min()) and int(a.max()) < 1 << 31):
+        raise KernelError(f"{name}: {_STATUS[7]}")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+MAX_COPY_POOLS = 16
+
+
+def copy_pages(moves) -> None:
+    """Copies pages of the cache, all layers of them, in one launch (csrc/cache_pages.cu).  `moves`: for every pool (src, dst, src_pages, dst_pages, slots):
+    `src` and `dst` [..., pages, heads, slots of a page, row], contiguous, alike but for their numbers of pages (`dst` may be `src`); the lists of pages are known
+    on the host (lists, arrays); `slots`: how many slots of each page hold tokens (of every head's run the first that many rows are copied, the others stay as they
+    are), or None: all.  All of it happens at once: no page is a destination twice, none is destination and source, and no destination pool overlaps another pool."""
+    moves = list(moves)
+    if len(moves) > MAX_COPY_POOLS:
+        raise KernelError(f"copy_pages: {len(moves)} pools in one call, at most {MAX_COPY_POOLS}")
+    args, kept = (_PoolMoves * max(1, len(moves)))(), []
+    device = None
+    for a, (src, dst, src_pages, dst_pages, slots) in zip(args, moves):
+        if src.dim() < 4 or src.dim() != dst.dim() or src.dtype != dst.dtype or src.shape[:-4] != dst.shape[:-4] or src.shape[-3:] != dst.shape[-3:]:
+            raise KernelError(f"copy_pages: pools {tuple(src.shape)} {src.dtype} and {tuple(dst.shape)} {dst.dtype} are alike in everything but their numbers of pages")
+        if not (src.is_contiguous() and dst.is_contiguous()):
+            raise KernelError("copy_pages: pools are contiguous")
+        if src.device != dst.device or (device is not None and src.device != device):
+            raise KernelError("copy_pages: the pools of a call lie on one device")
+        device = src.device
+        from_list = _whole_numbers(src_pages, "src_pages")
+        n = from_list.shape[0]
+        lists = [from_list, _whole_numbers(dst_pages, "dst_pages", n), None if slots is None else _whole_numbers(slots, "slots", n)]
+        kept.append(lists)
+        outer = 1
+        for d in src.shape[:-4]:
+            outer *= d
+        if src.numel() == 0 or dst.numel() == 0:
+            if n:
+                raise KernelError(f"copy_pages: {_STATUS[7]}")
+            outer = 1
+        a.src, a.dst = src.data_ptr(), dst.data_ptr()
+        a.outer, a.src_pages, a.dst_pages, a.heads, a.slots = outer, src.shape[-4], dst.shape[-4], max(1, src.shape[-3]), max(1, src.shape[-2])
+        a.row_bytes, a.moves = max(1, src.shape[-1] * src.element_size()), n
+        a.src_list, a.dst_list = lists[0].ctypes.data, lists[1].ctypes.data
+        a.slot_list = None if slots is None else lists[2].ctypes.data
+    if not any(lists[0].shape[0] for lists in kept):
+        return
+    _one_device(*[t for src, dst, *_ in moves for t in (src, dst)])
+    done = ctypes.c_int(0)
+    status = load_family("cache_pages").wllm_copy_pages(args, len(moves), sm_count(), ctypes.byref(done), _stream())
+    global launches
+    launches += done.value
+    if status:
+        _check(status, "copy_pages")
 
 
 ACTIVATIONS = {"gelu_tanh": 0, "silu": 1, "relu": 2, "capped_swish": 3}

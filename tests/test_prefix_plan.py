@@ -1,0 +1,129 @@
+"""The plan of attention over shared prefixes, on the host: every (token, key) that is to be seen stands in exactly one item, results are listed in the order of their keys."""
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from prefix_refs import Batch
+from wllm_b200.kernels import ops
+
+HEADER = 16
+
+
+def parts(plan):
+    h = plan.host.numpy()
+    items = h[h[2]:h[2] + 8 * h[0]].reshape(-1, 8)
+    tokens = h[h[3]:].copy()
+    starts = h[h[4]:h[4] + h[1] + 1]
+    listed = h[h[5]:h[5] + starts[-1]]
+    positions = h[h[6]:h[6] + h[1]]
+    return items, tokens, starts, listed, positions
+
+
+def check(plan, tables, q_lens, ctx_lens, ps, rep, tile_rows, align):
+    items, tokens, starts, listed, positions = parts(plan)
+    n = sum(q_lens)
+    owner = [r for r, q in enumerate(q_lens) for _ in range(q)]
+    pos = [c - q + t for q, c in zip(q_lens, ctx_lens) for t in range(q)]
+    assert positions.tolist() == pos
+    seen = [np.zeros(p + 1, dtype=np.int32) for p in pos]
+    rows = {}
+    for first, count, lo, hi, request, own, row, _ in items.tolist():
+        assert 0 < count * rep <= tile_rows and lo < hi and lo % align == 0 and (own or hi % align == 0)
+        for i in range(count):
+            token, at = tokens[2 * (first + i)], tokens[2 * (first + i) + 1]
+            assert at == pos[token] and (own or hi <= at - 0) and (not own or owner[token] == request)
+            top = min(hi, at + 1)
+            if top > lo:
+                seen[token][lo:top] += 1
+            pages = range(lo // ps, -(-hi // ps))
+            assert all(tables[request][p] == tables[owner[token]][p] for p in pages)     # the item's keys are the token's own
+            key = row + i * rep
+            assert key not in rows and key + rep <= plan.rows
+            rows[key] = (token, lo)
+    assert all((s == 1).all() for s in seen)
+    assert len(rows) == len(listed) and starts[0] == 0
+    for t in range(n):
+        mine = [rows[int(k)] for k in listed[starts[t]:starts[t + 1]]]
+        assert mine and all(m[0] == t for m in mine) and [m[1] for m in mine] == sorted(m[1] for m in mine)
+    taken = sorted(rows)
+    assert all(b - a >= rep for a, b in zip(taken, taken[1:]))
+    lengths = [-(-int(i[3] - i[2]) // (128 if tile_rows == 128 else 64)) for i in items]
+    assert lengths == sorted(lengths, reverse=True)
+
+
+TREES = [
+    (0, [(5, 1)]),                                                        # one request, nothing shared
+    (0, [(0, 1), (0, 1)]),                                                # first tokens
+    (512, [(3, 1), (0, 1), (40, 1)]),                                     # a prefix, one right behind it
+    (256, [(512, [(1, 1), (17, 3), (0, 9)]), (1024, [(5, 1)] * 30), (70, 1)]),      # two levels, a branch that ends early
+    (1024, [(0, 40), (33, 1)] * 9),                                       # portions beside decoded tokens
+    (64, [(200, 1)] * 3),                                                 # too short to share
+    (0, [(512, [(0, 1)] * 5), (512, [(7, 2)] * 5), (99, 1)]),             # several prompts
+    (128, [(128, [(128, [(128, [(3, 1), (2, 1)]), (2, 1)]), (1, 1)]), (0, 1)]),     # a chain of forks
+    (16384, [(100, 1)] * 20),
+]
+
+
+@pytest.mark.parametrize("tree", TREES)
+@pytest.mark.parametrize("nq,nkv,dtype", [(8, 1, torch.bfloat16), (7, 1, torch.bfloat16), (4, 4, torch.bfloat16), (6, 2, torch.float32), (32, 1, torch.float32), (128, 1, torch.bfloat16)])
+@pytest.mark.parametrize("ps", [16, 64])
+def test_every_key_stands_in_one_item(tree, nq, nkv, dtype, ps):
+    if tree[0] > 4000 and nq > 8:
+        tree = (1024, tree[1])
+    b = Batch(tree, nq, nkv, 8, 8, ps)
+    plan = ops.prefix_plan(b.table, b.q_lens, b.ctx_lens, ps, nq, nkv, 8, 8, dtype)
+    assert plan.n_tokens == b.n
+    bf16 = dtype == torch.bfloat16
+    check(plan, b.table.tolist(), b.q_lens, b.ctx_lens, ps, nq // nkv, 128 if bf16 else 32, 1 if bf16 else 64)
+
+
+def test_shared_keys_are_counted_once_for_all():
+    b = Batch((1024, [(256, [(3, 1), (4, 1)]), (9, 1)]), 4, 1, 8, 8, 64)
+    plan = ops.prefix_plan(b.table, b.q_lens, b.ctx_lens, 64, 4, 1, 8)
+    assert plan.saved_keys == 2 * 1024 + 256
+    assert ops.prefix_plan(b.table, b.q_lens, b.ctx_lens, 64, 4, 1, 8, min_keys=300).saved_keys == 2 * 1024
+    assert ops.prefix_plan(b.table, b.q_lens, b.ctx_lens, 64, 4, 1, 8, min_keys=2000).saved_keys == 0
+    # a page that new tokens are written to is nobody else's, whatever the table says: only the keys in front of every new token are shared
+    table = np.array([[3, 4, 5], [3, 4, 5]], dtype=np.int32)
+    plan = ops.prefix_plan(table, [1, 70], [140, 190], 64, 4, 1, 8, min_keys=1)
+    assert plan.saved_keys == 64
+
+
+def test_requests_that_bring_nothing_and_empty_batches():
+    table = np.array([[3, 4], [-1, -1], [3, 9]], dtype=np.int32)
+    plan = ops.prefix_plan(table, [1, 0, 2], [70, 0, 71], 64, 4, 2, 8, min_keys=64)
+    check(plan, table.tolist(), [1, 0, 2], [70, 0, 71], 64, 2, 128, 1)
+    empty = ops.prefix_plan(np.zeros((2, 3), dtype=np.int32), [0, 0], [0, 5], 64, 4, 2, 8)
+    assert empty.n_tokens == empty.items == empty.rows == 0
+    none = ops.prefix_plan(np.zeros((0, 3), dtype=np.int32), [], [], 64, 4, 2, 8)
+    assert none.items == 0
+
+
+def test_refusals():
+    table = np.array([[3, 4], [3, 9]], dtype=np.int32)
+    good = dict(tables=table, q_lens=[1, 2], ctx_lens=[70, 71], page_size=64, nq=4, nkv=2, hd=8)
+    ops.prefix_plan(**good)
+    for wrong in (dict(q_lens=[1]), dict(q_lens=[-1, 2]), dict(q_lens=[71, 2]), dict(ctx_lens=[129, 71]), dict(tables=np.array([[3, -1], [3, 9]], dtype=np.int32)),
+                  dict(tables=table.astype(np.int64)), dict(tables=table[0]), dict(nq=5), dict(nq=512), dict(hd=12), dict(hd=264), dict(vd=0), dict(page_size=8), dict(page_size=48),
+                  dict(dtype=torch.float16), dict(dtype=torch.float32, nq=128), dict(ctx_lens=[0, 71]), dict(q_lens=[1.0, 2.0])):
+        with pytest.raises(ops.KernelError):
+            ops.prefix_plan(**{**good, **wrong})
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_random_trees(seed):
+    rng = random.Random(seed)
+    ps = rng.choice([16, 32, 128])
+
+    def node(depth):
+        if depth == 0 or rng.random() < 0.4:
+            return (rng.randint(0, 300), rng.choice([1, 1, 1, rng.randint(2, 90)]))
+        return (ps * rng.randint(0, 900 // ps), [node(depth - 1) for _ in range(rng.randint(1, 6))])
+    b = Batch((0, [node(3) for _ in range(4)]), 1, 1, 8, 8, ps, seed)
+    nkv, rep = rng.choice([1, 3]), rng.choice([1, 2, 5, 16])
+    for dtype in (torch.bfloat16, torch.float32):
+        plan = ops.prefix_plan(b.table, b.q_lens, b.ctx_lens, ps, nkv * rep, nkv, 8, 8, dtype, min_keys=rng.choice([1, 64, 128]))
+        bf16 = dtype == torch.bfloat16
+        check(plan, b.table.tolist(), b.q_lens, b.ctx_lens, ps, rep, 128 if bf16 else 32, 1 if bf16 else 64)

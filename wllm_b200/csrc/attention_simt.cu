@@ -47,6 +47,7 @@
 // Used for the 32-bit path at every size, and for bfloat16 at the sizes that the
 // tensor-core kernels refuse.
 #include "common.cuh"
+#include "prefix_plan.cuh"
 
 constexpr int WARPS = 4;
 constexpr int CHUNK = 64;
@@ -588,41 +589,14 @@ __device__ __forceinline__ int chunk_pair(const int* __restrict__ req_q_len, con
     return -1;
 }
 
-template <typename T, int NE>
-__global__ void __launch_bounds__(TL_WARPS * 32, 2)
-paged_attention_simt_chunk_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
-                                  const int* __restrict__ req_q_start, const int* __restrict__ req_q_len, const int* __restrict__ req_ctx_len,
-                                  const int* __restrict__ block_table, int max_pages, int requests, int nq, int nkv, int hd, int page_size, float scale, int vd,
-                                  float cap, const float* __restrict__ slopes, float* __restrict__ scratch, int max_chunks) {
+// A warp's four rows over chunk `c`, whose keys' rows in the pools are `row_of`, by all warps of a CTA together; keys from key_hi on are zeros that no row sees.
+// `queries` puts the rows' queries into `qs` while the first tile is on its way (there is a barrier behind it).
+template <typename T, int NE, typename Queries>
+__device__ __forceinline__ void chunk_of_rows(const float* qs, T* ks, T* vs, const size_t* row_of, const T* __restrict__ k_pages, const T* __restrict__ v_pages, int hd, int vd, int c,
+                                              int key_hi, float scale, float cap, const int (&pos_r)[TL_RPW], const float (&slope_r)[TL_RPW], Queries queries, float (&m_c)[TL_RPW],
+                                              float (&l_c)[TL_RPW], float (&o_c)[TL_RPW][NE]) {
     constexpr int VN = Vec<T>::N;
-    extern __shared__ __align__(16) unsigned char tl_smem[];
-    __shared__ size_t row_of[CHUNK];               // the chunk's keys in the pools
-    pdl_begin();
-    int tile_at, c;
-    const int g = blockIdx.y, rep = nq / nkv, r = chunk_pair(req_q_len, req_ctx_len, requests, rep, max_chunks, blockIdx.x, tile_at, c);
-    if (r < 0) return;
-    const int q_len = req_q_len[r], rows = q_len * rep, m0 = tile_at * TL_ROWS;
-    const int ctx = req_ctx_len[r], q_start = req_q_start[r], pos0 = ctx - q_len;
-    const int key_hi = pos0 + (min(rows, m0 + TL_ROWS) - 1) / rep + 1;         // one past the last row's position
-    if (c * CHUNK >= key_hi) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kld = hd + VN;
-    float* qs = reinterpret_cast<float*>(tl_smem);                          // [32 rows][hd] float
-    T* ks = reinterpret_cast<T*>(qs + TL_ROWS * hd);                        // [32 keys][kld]
-    T* vs = ks + 32 * kld;                                                  // [32 keys][vd]
-    if (threadIdx.x < CHUNK) {
-        const int key = min(c * CHUNK + (int)threadIdx.x, key_hi - 1);
-        row_of[threadIdx.x] = ((size_t)block_table[(size_t)r * max_pages + key / page_size] * nkv + g) * page_size + key % page_size;
-    }
-    int pos_r[TL_RPW];
-    float slope_r[TL_RPW];
-#pragma unroll
-    for (int i = 0; i < TL_RPW; ++i) {
-        const int m = m0 + warp * TL_RPW + i;
-        slope_r[i] = slopes ? slopes[g * rep + m % rep] : 0.f;
-        pos_r[i] = m < rows ? pos0 + m / rep : -1;                          // a row past the end takes no key
-    }
-    __syncthreads();
+    const int lane = threadIdx.x & 31, kld = hd + VN;
     // 32 rows of `pieces` 16-byte pieces; keys past the last row's are zeros
     auto load = [&](int t, T* to, const T* from, int ld, int width, int to_ld) {
         const int pieces = width / VN, rows_on = (int)blockDim.x / pieces, pieces_on = (int)blockDim.x % pieces;
@@ -638,11 +612,7 @@ paged_attention_simt_chunk_kernel(const T* __restrict__ q, int q_stride, const T
     const int t0 = 2 * c, t1 = min(t0 + 2, (key_hi + 31) >> 5);
     load(t0, ks, k_pages, hd, hd, kld);
     load(t0, vs, v_pages, vd, vd, vd);
-    for (int idx = threadIdx.x; idx < TL_ROWS * hd; idx += blockDim.x) {
-        const int m = m0 + idx / hd, d = idx % hd;
-        qs[idx] = m < rows ? to_f32(q[(size_t)(q_start + m / rep) * q_stride + (size_t)(g * rep + m % rep) * hd + d]) : 0.f;
-    }
-    float m_c[TL_RPW], l_c[TL_RPW], o_c[TL_RPW][NE];
+    queries();
 #pragma unroll
     for (int i = 0; i < TL_RPW; ++i) {
         m_c[i] = -INFINITY; l_c[i] = 0.f;
@@ -659,7 +629,7 @@ paged_attention_simt_chunk_kernel(const T* __restrict__ q, int q_stride, const T
         float p[TL_RPW] = {0.f, 0.f, 0.f, 0.f};
         if (any) {
             const T* kr = ks + (size_t)lane * kld;
-            const float* qw = qs + (size_t)(warp * TL_RPW) * hd;
+            const float* qw = qs + (size_t)((int)(threadIdx.x >> 5) * TL_RPW) * hd;
             float acc[TL_RPW][4];
 #pragma unroll
             for (int i = 0; i < TL_RPW; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
@@ -723,6 +693,50 @@ paged_attention_simt_chunk_kernel(const T* __restrict__ q, int q_stride, const T
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <typename T, int NE>
+__global__ void __launch_bounds__(TL_WARPS * 32, 2)
+paged_attention_simt_chunk_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
+                                  const int* __restrict__ req_q_start, const int* __restrict__ req_q_len, const int* __restrict__ req_ctx_len,
+                                  const int* __restrict__ block_table, int max_pages, int requests, int nq, int nkv, int hd, int page_size, float scale, int vd,
+                                  float cap, const float* __restrict__ slopes, float* __restrict__ scratch, int max_chunks) {
+    constexpr int VN = Vec<T>::N;
+    extern __shared__ __align__(16) unsigned char tl_smem[];
+    __shared__ size_t row_of[CHUNK];               // the chunk's keys in the pools
+    pdl_begin();
+    int tile_at, c;
+    const int g = blockIdx.y, rep = nq / nkv, r = chunk_pair(req_q_len, req_ctx_len, requests, rep, max_chunks, blockIdx.x, tile_at, c);
+    if (r < 0) return;
+    const int q_len = req_q_len[r], rows = q_len * rep, m0 = tile_at * TL_ROWS;
+    const int ctx = req_ctx_len[r], q_start = req_q_start[r], pos0 = ctx - q_len;
+    const int key_hi = pos0 + (min(rows, m0 + TL_ROWS) - 1) / rep + 1;         // one past the last row's position
+    if (c * CHUNK >= key_hi) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kld = hd + VN;
+    float* qs = reinterpret_cast<float*>(tl_smem);                          // [32 rows][hd] float
+    T* ks = reinterpret_cast<T*>(qs + TL_ROWS * hd);                        // [32 keys][kld]
+    T* vs = ks + 32 * kld;                                                  // [32 keys][vd]
+    if (threadIdx.x < CHUNK) {
+        const int key = min(c * CHUNK + (int)threadIdx.x, key_hi - 1);
+        row_of[threadIdx.x] = ((size_t)block_table[(size_t)r * max_pages + key / page_size] * nkv + g) * page_size + key % page_size;
+    }
+    int pos_r[TL_RPW];
+    float slope_r[TL_RPW];
+#pragma unroll
+    for (int i = 0; i < TL_RPW; ++i) {
+        const int m = m0 + warp * TL_RPW + i;
+        slope_r[i] = slopes ? slopes[g * rep + m % rep] : 0.f;
+        pos_r[i] = m < rows ? pos0 + m / rep : -1;                          // a row past the end takes no key
+    }
+    __syncthreads();
+    float m_c[TL_RPW], l_c[TL_RPW], o_c[TL_RPW][NE];
+    chunk_of_rows<T, NE>(qs, ks, vs, row_of, k_pages, v_pages, hd, vd, c, key_hi, scale, cap, pos_r, slope_r, [&]() {
+        for (int idx = threadIdx.x; idx < TL_ROWS * hd; idx += blockDim.x) {
+            const int m = m0 + idx / hd, d = idx % hd;
+            qs[idx] = m < rows ? to_f32(q[(size_t)(q_start + m / rep) * q_stride + (size_t)(g * rep + m % rep) * hd + d]) : 0.f;
+        }
+    }, m_c, l_c, o_c);
 #pragma unroll
     for (int i = 0; i < TL_RPW; ++i) {
         const int m = m0 + warp * TL_RPW + i;
@@ -733,6 +747,68 @@ paged_attention_simt_chunk_kernel(const T* __restrict__ q, int q_stride, const T
         for (int e = 0; e < NE; ++e) {
             const int d = e * 32 + lane;
             if (d < vd) dst[2 + d] = o_c[i][e];
+        }
+    }
+}
+
+// --------------------------------------------------------------------------------------
+// items of a plan (prefix_plan.cuh), for batches whose requests share pages: up to 32 rows of any requests against a range of whole chunks, each chunk's results left where those of the
+// kernel above are.  The rows of all requests that hold a stretch of pages meet its keys together; a row's arithmetic is the walk's, so its bits are too.
+// --------------------------------------------------------------------------------------
+template <int NE>
+__global__ void __launch_bounds__(TL_WARPS * 32, 2)
+paged_attention_simt_prefix_kernel(const float* __restrict__ q, int q_stride, const float* __restrict__ k_pages, const float* __restrict__ v_pages, int pool_pages,
+                                   const int* __restrict__ block_table, int max_pages, const int* __restrict__ plan, int nq, int nkv, int hd, int page_size, float scale, int vd,
+                                   float cap, const float* __restrict__ slopes, float* __restrict__ scratch, int max_chunks) {
+    extern __shared__ __align__(16) unsigned char tl_smem[];
+    __shared__ size_t row_of[CHUNK];
+    pdl_begin();
+    const int rep = nq / nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, total = plan[PLAN_ITEMS] * nkv;
+    float* qs = reinterpret_cast<float*>(tl_smem);                          // [32 rows][hd]
+    float* ks = qs + TL_ROWS * hd;                                          // [32 keys][hd + 4]
+    float* vs = ks + 32 * (hd + Vec<float>::N);                             // [32 keys][vd]
+    const int* tokens = plan + plan[PLAN_AT_TOKENS];
+    for (int it = blockIdx.x; it < total; it += gridDim.x) {
+        const int* item = plan + plan[PLAN_AT_ITEMS] + it / nkv * PLAN_ITEM;
+        const int g = it % nkv, rows = item[ITEM_TOKENS] * rep, key_hi = item[ITEM_KEY_HI];
+        const int* mine = tokens + 2 * item[ITEM_TOKEN];
+        const int* table = block_table + (size_t)item[ITEM_REQUEST] * max_pages;
+        int pos_r[TL_RPW];
+        float slope_r[TL_RPW];
+#pragma unroll
+        for (int i = 0; i < TL_RPW; ++i) {
+            const int m = warp * TL_RPW + i;
+            slope_r[i] = slopes && m < rows ? slopes[g * rep + m % rep] : 0.f;
+            pos_r[i] = m < rows ? mine[2 * (m / rep) + 1] : -1;             // a row past the end takes no key
+        }
+        for (int c = item[ITEM_KEY_LO] / CHUNK; c * CHUNK < key_hi; ++c) {
+            __syncthreads();                                                // everyone is done with the chunk (and the queries) before
+            if (threadIdx.x < CHUNK) {
+                const int key = min(c * CHUNK + (int)threadIdx.x, key_hi - 1), page = min(max(table[min(key / page_size, max_pages - 1)], 0), pool_pages - 1);
+                row_of[threadIdx.x] = ((size_t)page * nkv + g) * page_size + key % page_size;
+            }
+            __syncthreads();
+            const bool first = c == item[ITEM_KEY_LO] / CHUNK;
+            float m_c[TL_RPW], l_c[TL_RPW], o_c[TL_RPW][NE];
+            chunk_of_rows<float, NE>(qs, ks, vs, row_of, k_pages, v_pages, hd, vd, c, key_hi, scale, cap, pos_r, slope_r, [&]() {
+                if (first)
+                    for (int idx = threadIdx.x; idx < TL_ROWS * hd; idx += blockDim.x) {
+                        const int m = idx / hd, d = idx % hd;
+                        qs[idx] = m < rows ? q[(size_t)mine[2 * (m / rep)] * q_stride + (size_t)(g * rep + m % rep) * hd + d] : 0.f;
+                    }
+            }, m_c, l_c, o_c);
+#pragma unroll
+            for (int i = 0; i < TL_RPW; ++i) {
+                const int m = warp * TL_RPW + i;
+                if (pos_r[i] < c * CHUNK || c >= max_chunks) continue;
+                float* dst = scratch + (((size_t)mine[2 * (m / rep)] * nq + g * rep + m % rep) * max_chunks + c) * (vd + 2);
+                if (lane == 0) { dst[0] = m_c[i]; dst[1] = l_c[i]; }
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    const int d = e * 32 + lane;
+                    if (d < vd) dst[2 + d] = o_c[i][e];
+                }
+            }
         }
     }
 }
@@ -843,6 +919,40 @@ WLLM_API int wllm_paged_attention_simt_chunks(const void* q, int q_stride, void*
         const int st = wllm_launch(paged_attention_simt_chunk_kernel<float, NE>, grid, TL_WARPS * 32, smem, stream, (const float*)q, q_stride, \
                                    (const float*)k_pages, (const float*)v_pages, req_q_start, req_q_len, req_ctx_len, block_table, max_pages, requests, \
                                    nq, nkv, hd, page_size, scale, vd, cap, slopes, scratch, max_chunks); \
+        if (st != WLLM_OK) return st; \
+        return wllm_launch(paged_attention_simt_merge_kernel<float, NE>, blocks, WARPS * 32, 0, stream, (float*)out, out_stride, positions, n_tokens, nq, vd, 0, \
+                           (const float*)scratch, max_chunks, sinks, 0); \
+    } while (0)
+    if (vd <= 64) GO(2);
+    if (vd <= 128) GO(4);
+    GO(8);
+#undef GO
+}
+
+// A planned batch (prefix_plan.cuh; its items of at most 32 rows, its ranges of whole chunks): the walk's result, bit for bit.  n_tokens: rows of q and out; pool_pages: pages of the pools;
+// pairs: (item, kv head) pairs of the plan, or the most that there may be; ctas: CTAs that run at once; positions [n_tokens], on the device; scratch: n_tokens * nq * max_chunks * (vd + 2)
+// floats; max_chunks: chunks of 64 keys of the longest context.
+WLLM_API int wllm_paged_attention_simt_prefix(const void* q, int q_stride, void* out, int out_stride, const void* k_pages, const void* v_pages, int pool_pages, const int* block_table,
+                                              int max_pages, int n_tokens, int nq, int nkv, int hd, int vd, int page_size, float scale, float cap, const float* sinks, const float* slopes,
+                                              const int* plan, const int* positions, float* scratch, int max_chunks, long long pairs, int ctas, cudaStream_t stream) {
+    if (n_tokens <= 0 || pairs <= 0) return WLLM_OK;
+    if (hd <= 0 || hd > 256 || hd % 8 != 0 || vd <= 0 || vd > 256 || vd % 8 != 0 || nq <= 0 || nkv <= 0 || nq % nkv != 0 || nq / nkv > TL_ROWS || page_size <= 0 || max_pages <= 0 ||
+        pool_pages <= 0 || max_chunks < 1 || scratch == nullptr || !(cap >= 0.f) || ctas < 1)
+        return WLLM_BAD_SIZE;
+    if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) return WLLM_BAD_ALIGN;
+    constexpr int VN = Vec<float>::N, most = (TL_ROWS * 256 + 32 * (256 + VN) + 32 * 256) * (int)sizeof(float);
+    const size_t smem = ((size_t)TL_ROWS * hd + 32 * (hd + VN) + 32 * vd) * sizeof(float);
+    const int blocks = (int)(((long long)n_tokens * nq + WARPS - 1) / WARPS);
+#define GO(NE) do { \
+        static bool raised = false; \
+        if (!raised) { \
+            const cudaError_t e = cudaFuncSetAttribute(paged_attention_simt_prefix_kernel<NE>, cudaFuncAttributeMaxDynamicSharedMemorySize, most); \
+            if (e != cudaSuccess) return 1000 + (int)e; \
+            raised = true; \
+        } \
+        const int st = wllm_launch(paged_attention_simt_prefix_kernel<NE>, dim3((unsigned)(pairs < ctas ? pairs : ctas)), TL_WARPS * 32, smem, stream, (const float*)q, q_stride, \
+                                   (const float*)k_pages, (const float*)v_pages, pool_pages, block_table, max_pages, plan, nq, nkv, hd, page_size, scale, vd, cap, slopes, scratch, \
+                                   max_chunks); \
         if (st != WLLM_OK) return st; \
         return wllm_launch(paged_attention_simt_merge_kernel<float, NE>, blocks, WARPS * 32, 0, stream, (float*)out, out_stride, positions, n_tokens, nq, vd, 0, \
                            (const float*)scratch, max_chunks, sinks, 0); \

@@ -1,0 +1,217 @@
+// The plan of attention over shared prefixes, worked out on the host from the step's block tables: no kernels here.
+//
+// Requests that hold the same page at the same place of their tables have the same tokens up to its end.  So the tables are walked as a tree: the requests that agree on
+// the next page stay together, and every stretch of pages on which a set of two or more agrees is one *segment*, attended to by the rows of all of them; what is left of a
+// request's keys is its own segment.  Segments are cut into items, (tile of rows) x (range of keys), one CTA each and key/value head.  How long the ranges are decides
+// between SMs without work (long ranges) and results that have to be written and merged (short ones): of a few lengths the one with the earliest estimated end is
+// taken, an item costing its tiles of keys and a tile and a half beside them.  Items are listed longest first, those that read the same keys side by side (for the L2).
+#include "common.cuh"
+#include "prefix_plan.cuh"
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+namespace {
+
+enum { OUT_TOO_SMALL = 4, PAGES_OUT_OF_RANGE = 7 };
+
+struct Segment { int first, count, key_lo, key_hi; bool own; };       // first, count: its requests in `members`
+
+struct Planner {
+    const int* tables;
+    long long width;
+    int R, ps, align, min_keys;
+    std::vector<int> share, cover, members;
+    std::vector<Segment> segments;
+
+    int page(int r, int i) const { return tables[r * width + i]; }
+
+    // `set`: requests that agree on all pages in front of `from`; their keys in front of `key` belong to segments
+    void walk(const std::vector<int>& set, int from, int key) {
+        std::vector<int> next;
+        for (int r : set)
+            if (share[r] > from) next.push_back(r);
+        std::stable_sort(next.begin(), next.end(), [&](int a, int b) { return page(a, from) < page(b, from); });
+        for (size_t i = 0; i < next.size();) {
+            size_t j = i + 1;
+            while (j < next.size() && page(next[j], from) == page(next[i], from)) ++j;
+            if (j - i >= 2) {
+                std::vector<int> group(next.begin() + i, next.begin() + j);
+                std::sort(group.begin(), group.end());
+                int p = from + 1, most = share[group[0]];
+                for (int r : group) most = std::min(most, share[r]);
+                for (; p < most; ++p) {
+                    bool same = true;
+                    for (size_t m = 1; m < group.size() && same; ++m) same = page(group[m], p) == page(group[0], p);
+                    if (!same) break;
+                }
+                int hi = (int)((long long)p * ps / align * align);
+                if (hi - key >= min_keys) {
+                    segments.push_back({(int)members.size(), (int)group.size(), key, hi, false});
+                    members.insert(members.end(), group.begin(), group.end());
+                    for (int r : group) cover[r] = hi;
+                } else hi = key;
+                walk(group, p, hi);
+            }
+            i = j;
+        }
+    }
+};
+
+struct Tile { int token, tokens, key_lo, key_hi, request; bool own; };
+struct Item { int tile, key_lo, key_hi, row, order; };
+
+long long padded(long long n) { return (n + 3) & ~3ll; }
+
+}  // namespace
+
+// tables [R][width] (pages that hold no key of a request are not looked at), q_len, ctx_len [R] on the host.  rep: query heads a key/value head; tile_rows: rows of an item at
+// most; key_tile: keys of a tile, whole tiles make an item's range; align: segments end at multiples of it; min_keys: no shared segment is shorter; pool_pages: one past the largest
+// page number; ctas: CTAs that run at once; caps: {items, tokens, results, tokens of the batch} that the array is laid out for, zeros: what this plan needs (a captured
+// step's array lies at fixed places whatever the batch holds).  out [room]; info [8]: ints used, items, rows, shared keys saved (keys x further holders), most results of a
+// token, items that the batch has at the least.
+// Returns 0; 2: sizes that make no sense, or more than the caps hold; 4: `room` is too small (info[0] says what is needed); 7: a page number outside the pool.
+WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const int* q_len, const int* ctx_len, int page_size, int rep, int nkv, int tile_rows, int key_tile, int align,
+                              int min_keys, int pool_pages, int ctas, const int* caps, int* out, long long room, long long* info) {
+    try {
+        if (R < 0 || R > (1 << 20) || width < 0 || page_size < 1 || rep < 1 || nkv < 1 || tile_rows < rep || key_tile < 1 || align < 1 || ctas < 1 || pool_pages < 1) return WLLM_BAD_SIZE;
+        Planner p{tables, width, R, page_size, align, min_keys, {}, {}, {}, {}};
+        p.share.assign(R, 0);
+        p.cover.assign(R, 0);
+        std::vector<int> start(R + 1, 0), all;
+        long long total = 0;
+        for (int r = 0; r < R; ++r) {
+            if (q_len[r] < 0 || (q_len[r] > 0 && (ctx_len[r] < q_len[r] || ctx_len[r] > width * page_size))) return WLLM_BAD_SIZE;
+            start[r] = (int)total;
+            total += q_len[r];
+            if (total > (1 << 26)) return WLLM_BAD_SIZE;
+            if (q_len[r] == 0) continue;
+            for (int i = 0; i * (long long)page_size < ctx_len[r]; ++i)
+                if (p.page(r, i) < 0 || p.page(r, i) >= pool_pages) return PAGES_OUT_OF_RANGE;
+            p.share[r] = (ctx_len[r] - q_len[r]) / page_size;
+            all.push_back(r);
+        }
+        start[R] = (int)total;
+        p.walk(all, 0, 0);
+        long long saved = 0;
+        for (const Segment& s : p.segments) saved += (long long)(s.count - 1) * (s.key_hi - s.key_lo);
+        for (int r : all) {
+            p.segments.push_back({(int)p.members.size(), 1, p.cover[r], ctx_len[r], true});
+            p.members.push_back(r);
+        }
+        // tiles of rows: whole tokens of a segment's requests, one behind the other
+        const int per_tile = tile_rows / rep;
+        std::vector<Tile> tiles;
+        std::vector<int> tokens, at;              // of all segments, and their positions
+        for (const Segment& s : p.segments) {
+            const int first = (int)tokens.size();
+            for (int m = 0; m < s.count; ++m) {
+                const int r = p.members[s.first + m];
+                for (int t = 0; t < q_len[r]; ++t) {
+                    tokens.push_back(start[r] + t);
+                    at.push_back(ctx_len[r] - q_len[r] + t);
+                }
+            }
+            const int n = (int)tokens.size() - first;
+            for (int t = 0; t < n; t += per_tile) {
+                const int count = std::min(per_tile, n - t);
+                tiles.push_back({first + t, count, s.key_lo, s.own ? at[first + t + count - 1] + 1 : s.key_hi, p.members[s.first], s.own});
+            }
+            if (tokens.size() > (1u << 28)) return WLLM_BAD_SIZE;
+        }
+        // the length of the ranges
+        auto keys_of = [&](const Tile& t) { return (t.key_hi - t.key_lo + key_tile - 1) / key_tile; };
+        int longest = 1;
+        for (const Tile& t : tiles) longest = std::max(longest, keys_of(t));
+        const long long most_items = caps[0] > 0 ? caps[0] : (1 << 22);
+        const double beside = 1.5;
+        double best = 0;
+        int per = longest;
+        bool any = false;
+        for (int l = 1;; l = std::max(l + 1, l * 5 / 4)) {
+            const int len = std::min(l, longest);
+            long long n = 0;
+            double work = 0;
+            int top = 0;
+            for (const Tile& t : tiles) {
+                const int k = keys_of(t), parts = (k + len - 1) / len;
+                n += parts;
+                work += k + beside * parts;
+                top = std::max(top, (k + parts - 1) / parts);
+            }
+            const double end = n * nkv <= ctas ? top + beside : std::max(top + beside, work * nkv / ctas + 0.5 * (top + beside));
+            if (n <= most_items && (!any || end < best * 0.98)) {
+                best = end;
+                per = len;
+                any = true;
+            }
+            if (len == longest) break;
+        }
+        if (!any) return WLLM_BAD_SIZE;
+        // items: of the tiles that follow one another with the same keys, range by range
+        std::vector<Item> items;
+        long long rows = 0, results = 0;
+        for (size_t i = 0; i < tiles.size();) {
+            size_t j = i + 1;
+            while (j < tiles.size() && !tiles[i].own && !tiles[j].own && tiles[j].request == tiles[i].request && tiles[j].key_lo == tiles[i].key_lo && tiles[j].key_hi == tiles[i].key_hi) ++j;
+            const int k = keys_of(tiles[i]), parts = (k + per - 1) / per;
+            for (int s = 0; s < parts; ++s)
+                for (size_t t = i; t < j; ++t) {
+                    const int lo = tiles[i].key_lo + (int)((long long)k * s / parts) * key_tile, hi = std::min(tiles[i].key_hi, tiles[i].key_lo + (int)((long long)k * (s + 1) / parts) * key_tile);
+                    items.push_back({(int)t, lo, hi, (int)rows, (int)items.size()});
+                    rows += (long long)tiles[t].tokens * rep;
+                    results += tiles[t].tokens;
+                    if (rows > 0x7fffffff / nkv) return WLLM_BAD_SIZE;
+                }
+            i = j;
+        }
+        // results by token, in the order in which segments were found: ascending keys
+        std::vector<int> starts(total + 1, 0), listed(results);
+        for (const Item& it : items)
+            for (int t = 0; t < tiles[it.tile].tokens; ++t) ++starts[tokens[tiles[it.tile].token + t] + 1];
+        int most = 0;
+        for (long long t = 0; t < total; ++t) {
+            most = std::max(most, starts[t + 1]);
+            starts[t + 1] += starts[t];
+        }
+        {
+            std::vector<int> next(starts.begin(), starts.end() - 1);
+            for (const Item& it : items)
+                for (int t = 0; t < tiles[it.tile].tokens; ++t) listed[next[tokens[tiles[it.tile].token + t]]++] = it.row + t * rep;
+        }
+        std::stable_sort(items.begin(), items.end(), [&](const Item& a, const Item& b) { return (a.key_hi - a.key_lo + key_tile - 1) / key_tile > (b.key_hi - b.key_lo + key_tile - 1) / key_tile; });
+
+        const long long need[4] = {(long long)items.size(), (long long)tokens.size(), results, total};
+        long long cap[4];
+        for (int i = 0; i < 4; ++i) {
+            cap[i] = caps[i] > 0 ? caps[i] : need[i];
+            if (need[i] > cap[i]) return WLLM_BAD_SIZE;
+        }
+        const long long at_items = PLAN_HEADER, at_tokens = at_items + padded(cap[0] * PLAN_ITEM), at_starts = at_tokens + padded(cap[1] * 2), at_results = at_starts + padded(cap[3] + 1),
+                        at_positions = at_results + padded(cap[2]), used = at_positions + padded(cap[3]);
+        info[0] = used; info[1] = need[0]; info[2] = rows; info[3] = saved; info[4] = most; info[5] = (long long)tiles.size(); info[6] = need[1]; info[7] = results;
+        if (used > 0x7fffffff) return WLLM_BAD_SIZE;
+        if (used > room) return OUT_TOO_SMALL;
+        std::fill(out, out + used, 0);
+        out[PLAN_ITEMS] = (int)need[0]; out[PLAN_TOKENS] = (int)total; out[PLAN_AT_ITEMS] = (int)at_items; out[PLAN_AT_TOKENS] = (int)at_tokens;
+        out[PLAN_AT_STARTS] = (int)at_starts; out[PLAN_AT_RESULTS] = (int)at_results; out[PLAN_AT_POSITIONS] = (int)at_positions; out[PLAN_ROWS] = (int)rows;
+        for (size_t i = 0; i < items.size(); ++i) {
+            const Tile& t = tiles[items[i].tile];
+            int* o = out + at_items + i * PLAN_ITEM;
+            o[ITEM_TOKEN] = t.token; o[ITEM_TOKENS] = t.tokens; o[ITEM_KEY_LO] = items[i].key_lo; o[ITEM_KEY_HI] = items[i].key_hi;
+            o[ITEM_REQUEST] = t.request; o[ITEM_OWN] = t.own ? 1 : 0; o[ITEM_ROW] = items[i].row;
+        }
+        for (size_t i = 0; i < tokens.size(); ++i) {
+            out[at_tokens + 2 * i] = tokens[i];
+            out[at_tokens + 2 * i + 1] = at[i];
+        }
+        for (long long t = 0; t <= cap[3]; ++t) out[at_starts + t] = starts[std::min(t, total)];     // (tokens past the last have no results)
+        std::copy(listed.begin(), listed.end(), out + at_results);
+        for (int r = 0; r < R; ++r)
+            for (int t = 0; t < q_len[r]; ++t) out[at_positions + start[r] + t] = ctx_len[r] - q_len[r] + t;
+        return WLLM_OK;
+    } catch (const std::bad_alloc&) {
+        return WLLM_BAD_SIZE;
+    }
+}

@@ -12,6 +12,7 @@ FAMILIES = {
     "norm": [{}],
     "rope_cache": [{}],
     "cache_pages": [{}],
+    "prefix_plan": [{}],
     "attention_simt": [{}],
     "activation": [{}],
     "linear_attention": [{}],
@@ -31,6 +32,8 @@ FAMILIES = {
     # tensor-core attention is built per head size; others are built when a model first asks
     "attention_mma": [{"HEAD_DIM": 256}, {"HEAD_DIM": 32}, {"HEAD_DIM": 48}],
     "attention_decode_static": [{"HEAD_DIM": 256}],
+    # and so is attention over shared prefixes, per key and value head size
+    "prefix_attention": [{"HEAD_DIM": 256, "VALUE_DIM": 256}, {"HEAD_DIM": 128, "VALUE_DIM": 128}],
     # attention over latent rows on the tensor cores is built per row and value size, when a model first asks
     "latent_attention_mma": [],
 }

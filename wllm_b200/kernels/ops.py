@@ -768,6 +768,112 @@ def attention_mma_prefill(q, out, k_pages, v_pages, req_q_start, req_q_len, req_
     launches += 1
 
 
+class PrefixPlan:
+    """How a batch whose requests share pages is attended to (csrc/prefix_plan.cuh): made once for a step and a layout of heads, read by every layer of it."""
+
+    def __init__(self, key: tuple, requests: int, width: int, n_tokens: int, info, host: torch.Tensor, max_ctx: int, fixed: bool):
+        self.key, self.requests, self.width, self.n_tokens = key, requests, width, n_tokens
+        self.used, self.items, self.rows, self.saved_keys, self.most_results, self.tiles = (int(info[i]) for i in range(6))
+        self.host, self.fixed = host[:self.used], fixed      # int32 on the host, pinned where there is a device
+        page_size, nq, nkv, hd, vd, dtype = key
+        self.max_chunks = max(1, -(-max_ctx // SIMT_CHUNK))
+        self.scratch_floats = nkv * self.rows * (vd + 2) if dtype == torch.bfloat16 else n_tokens * nq * self.max_chunks * (vd + 2)
+
+    def to(self, device) -> torch.Tensor:
+        """The plan's array on the device, as prefix_attention takes it (in the current stream's order)."""
+        return torch.empty(self.used, dtype=torch.int32, device=device).copy_(self.host, non_blocking=True)
+
+
+PREFIX_MIN_KEYS = 128
+
+
+def prefix_rows(dtype: torch.dtype) -> int:
+    """Rows (token, query head of the group) of an item of a plan, at most."""
+    return 128 if dtype == torch.bfloat16 else 32
+
+
+def prefix_ok(nq: int, nkv: int, hd: int, vd: int, page_size: int, dtype: torch.dtype) -> bool:
+    """Head layouts and pages that prefix_attention is built for."""
+    return dtype in (torch.bfloat16, torch.float32) and nkv > 0 and nq % nkv == 0 and 0 < nq // nkv <= prefix_rows(dtype) and \
+        all(0 < d <= 256 and d % 8 == 0 for d in (hd, vd)) and page_size >= 16 and page_size & (page_size - 1) == 0
+
+
+def prefix_plan(tables, q_lens, ctx_lens, page_size: int, nq: int, nkv: int, hd: int, vd: int | None = None, dtype: torch.dtype = torch.bfloat16,
+                min_keys: int = PREFIX_MIN_KEYS) -> PrefixPlan:
+    """The plan of a batch's attention, from what the host knows of it: `tables` [requests, pages] (int32; an array or a tensor of the CPU), the requests' new tokens and contexts
+    (those included).  The batch's tokens stand request by request.  Requests that hold the same page at the same place share its keys and those in front of it; stretches of fewer than
+    `min_keys` shared keys are left to each request.  A plan holds for any pools and any queries of these tables and lengths."""
+    vd = hd if vd is None else vd
+    if not prefix_ok(nq, nkv, hd, vd, page_size, dtype):
+        raise KernelError(f"prefix_plan: {nq} query heads on {nkv}, sizes {hd}/{vd}, pages of {page_size}, {dtype}: up to {prefix_rows(dtype) if dtype in (torch.bfloat16, torch.float32) else 0} "
+                          "query heads a key/value head, head sizes in steps of 8 up to 256, pages of a power of two of at least 16 tokens, bfloat16 or float32")
+    if isinstance(tables, torch.Tensor):
+        if tables.is_cuda:
+            raise KernelError("prefix_plan: block tables on the host")
+        tables = tables.numpy()
+    if tables.ndim != 2 or tables.dtype != np.int32:
+        raise KernelError("prefix_plan: block tables [requests, pages] of int32")
+    tables = np.ascontiguousarray(tables)
+    R, width = tables.shape
+    q, ctx = _whole_numbers(q_lens, "q_lens", R), _whole_numbers(ctx_lens, "ctx_lens", R)
+    n, max_ctx = int(q.sum(dtype=np.int64)), int(ctx.max(initial=0))
+    bf16 = dtype == torch.bfloat16
+    lib = load_family("prefix_plan")
+    info = (ctypes.c_longlong * 8)()
+    room = 4096 + 32 * n
+    while True:
+        host = torch.empty(room, dtype=torch.int32, pin_memory=torch.cuda.is_available())
+        status = lib.wllm_prefix_plan(c_void_p(tables.ctypes.data), ctypes.c_longlong(width), R, c_void_p(q.ctypes.data), c_void_p(ctx.ctypes.data), page_size, nq // nkv, nkv,
+                                      prefix_rows(dtype), 128 if bf16 else SIMT_CHUNK, 1 if bf16 else SIMT_CHUNK, max(1, min_keys), 0x7fffffff, sm_count() if bf16 else 2 * sm_count(),
+                                      (ctypes.c_int * 4)(), c_void_p(host.data_ptr()), ctypes.c_longlong(room), info)
+        if status != 4:
+            break
+        room = int(info[0])
+    if status:
+        raise KernelError(f"prefix_plan: {_STATUS.get(status, status)}")
+    return PrefixPlan((page_size, nq, nkv, hd, vd, dtype), R, width, n, info, host, max_ctx, False)
+
+
+def prefix_attention(q, out, k_pages, v_pages, block_table, plan: PrefixPlan, arrays: torch.Tensor, nq: int, nkv: int, hd: int, page_size: int, scale: float, scratch: torch.Tensor,
+                     vd: int | None = None, sinks: torch.Tensor | None = None, cap: float = 0.0, slopes: torch.Tensor | None = None) -> None:
+    """Attention of a planned batch (csrc/prefix_attention.cu; 32-bit: csrc/attention_simt.cu, bit for bit what the other 32-bit kernels give): q [tokens, nq * hd] (row stride free),
+    out [tokens, nq * vd], pages [pages, nkv, page_size, hd | vd], `block_table` [requests, pages] the tables of the plan on the device, `arrays` = plan.to(device), `scratch` float32 of at
+    least plan.scratch_floats, which the call alone uses while it runs.  Every earlier key is seen (no window).  `sinks`, `cap`, `slopes`: as for attention_mma_decode."""
+    vd = hd if vd is None else vd
+
+    def need(ok, what):
+        if not ok:
+            raise KernelError("prefix_attention: " + what)
+    _one_device(q, out, k_pages, v_pages, block_table, arrays, scratch, sinks, slopes)
+    need(plan.key == (page_size, nq, nkv, hd, vd, q.dtype), f"a plan for (page size, heads, kv heads, sizes, type) {plan.key}, not {(page_size, nq, nkv, hd, vd, q.dtype)}")
+    need(q.dim() == 2 and q.shape == (plan.n_tokens, nq * hd) and q.stride(1) == 1, f"q [{plan.n_tokens}, {nq * hd}]")
+    need(out.dim() == 2 and out.shape == (plan.n_tokens, nq * vd) and out.stride(1) == 1 and out.dtype == q.dtype, f"out [{plan.n_tokens}, {nq * vd}]")
+    need(k_pages.dim() == 4 and k_pages.shape[1:] == (nkv, page_size, hd) and k_pages.is_contiguous() and k_pages.dtype == q.dtype, f"key pages [.., {nkv}, {page_size}, {hd}]")
+    need(v_pages.shape == (k_pages.shape[0], nkv, page_size, vd) and v_pages.is_contiguous() and v_pages.dtype == q.dtype, f"value pages [{k_pages.shape[0]}, {nkv}, {page_size}, {vd}]")
+    need(block_table.dtype == torch.int32 and block_table.shape == (plan.requests, plan.width) and block_table.is_contiguous(), f"block table [{plan.requests}, {plan.width}]")
+    need(arrays.dtype == torch.int32 and arrays.is_contiguous() and arrays.dim() == 1 and arrays.numel() >= plan.used, "the plan's arrays")
+    need(scratch.dtype == torch.float32 and scratch.is_contiguous() and scratch.numel() >= plan.scratch_floats, f"{plan.scratch_floats} floats of scratch")
+    for t, name in ((sinks, "sinks"), (slopes, "slopes")):
+        need(t is None or (t.dtype == torch.float32 and t.shape == (nq,) and t.is_contiguous()), f"{name} [{nq}] of float32")
+    need(scale > 0 and cap >= 0, "a scale above zero and a cap of zero (none) or above")
+    if plan.n_tokens == 0:
+        return
+    pairs = plan.items * nkv
+    if q.dtype == torch.bfloat16:
+        lib = load_family("prefix_attention", {"HEAD_DIM": hd, "VALUE_DIM": vd})
+        status = lib.wllm_prefix_attention(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(k_pages), _ptr(v_pages), ctypes.c_longlong(k_pages.shape[0]), _ptr(block_table),
+                                           plan.width, plan.n_tokens, nq, nkv, page_size, c_float(scale), c_float(cap), _ptr(sinks), _ptr(slopes), _ptr(arrays), _ptr(scratch),
+                                           ctypes.c_longlong(plan.rows), ctypes.c_longlong(pairs), sm_count(), _ptr(_device_status(q.device)), _stream())
+    else:
+        positions = c_void_p(arrays.data_ptr() + 4 * int(plan.host[6]))
+        status = load_family("attention_simt").wllm_paged_attention_simt_prefix(
+            _ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(k_pages), _ptr(v_pages), k_pages.shape[0], _ptr(block_table), plan.width, plan.n_tokens, nq, nkv, hd, vd, page_size,
+            c_float(scale), c_float(cap), _ptr(sinks), _ptr(slopes), _ptr(arrays), positions, _ptr(scratch), plan.max_chunks, ctypes.c_longlong(pairs), 2 * sm_count(), _stream())
+    _check(status, f"prefix_attention(head_dim={hd}/{vd}, heads={nq}/{nkv})")
+    global launches
+    launches += 1    # (with the merge kernel)
+
+
 class _PoolMoves(ctypes.Structure):
     _fields_ = [("src", c_void_p), ("dst", c_void_p)] + [(name, ctypes.c_longlong) for name in ("outer", "src_pages", "dst_pages", "heads", "slots", "row_bytes", "moves")] + \
         [(name, c_void_p) for name in ("src_list", "dst_list", "slot_list")]

@@ -9,10 +9,12 @@
 #include <Python.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/ops/empty.h>
 
 #include <initializer_list>
 #include <sstream>
 #include <string>
+#include <vector>
 
 namespace {
 
@@ -127,7 +129,7 @@ struct Branch {
     }
 };
 
-// -- the entry points (csrc/gemm_bf16_tc.cu, norm.cu, rope_cache.cu, attention_mma.cu) ---------------------------------------------------
+// -- the entry points (csrc/gemm_bf16_tc.cu, norm.cu, rope_cache.cu, attention_mma.cu, prefix_plan.cu, prefix_attention.cu, attention_simt.cu, cache_pages.cu) ---------------------------------------------------
 typedef int (*GemmFn)(const void*, int, const void*, int, void*, int, int, int, int, int, int, int, int*, int, float, float, void*);
 typedef int (*NormFn)(float*, const void*, int, int, long long, const void*, int, float, float, int, void*, int, const int*, int, int, void*);
 typedef int (*SandwichFn)(float*, const void*, int, int, long long, const void*, const void*, int, int, long long, const void*, float, float, const void*, float,
@@ -141,7 +143,24 @@ typedef int (*DecodeFn)(const void*, int, void*, int, const void*, const void*, 
 typedef int (*PrefillFn)(const void*, int, void*, int, const void*, const void*, long long, const int*, const int*, const int*, const int*, int, int, int, int, int,
                          int, int, float, int, int, int, float*, int*, const float*, float, int, const float*, void*);
 
+typedef int (*PlanFn)(const int*, long long, int, const int*, const int*, int, int, int, int, int, int, int, int, int, const int*, int*, long long, long long*);
+typedef int (*PrefixFn)(const void*, int, void*, int, const void*, const void*, long long, const int*, int, int, int, int, int, float, float, const float*, const float*, const int*,
+                        float*, long long, long long, int, int*, void*);
+typedef int (*PrefixSimtFn)(const void*, int, void*, int, const void*, const void*, int, const int*, int, int, int, int, int, int, int, float, float, const float*, const float*,
+                            const int*, const int*, float*, int, long long, int, void*);
+struct PagePoolMoves {                 // as csrc/cache_pages.cu has it
+    const void* src;
+    void* dst;
+    long long outer, src_pages, dst_pages, heads, slots, row_bytes, moves;
+    const int *src_list, *dst_list, *slot_list;
+};
+typedef int (*CopyPagesFn)(const PagePoolMoves*, int, int, int*, void*);
+
 GemmFn gemm_fn;
+PlanFn plan_fn;
+PrefixFn prefix_fn[33][33];            // by head sizes in steps of 8
+PrefixSimtFn prefix_simt_fn;
+CopyPagesFn copy_pages_fn;
 NormFn norm_fn;
 SandwichFn sandwich_fn;
 RopeFn rope_fn;
@@ -152,6 +171,8 @@ PrefillFn prefill_fn[257];
 // the binder hands the addresses over: of one entry point (its name), or of a head size's two (the size)
 PyObject* asked(const char* name) { return PyUnicode_FromString(name); }
 PyObject* asked(int head_size) { return PyLong_FromLong(head_size); }
+struct Heads { int key, value; };
+PyObject* asked(Heads h) { return Py_BuildValue("(ii)", h.key, h.value); }
 
 // (the arguments, and with them what is left to check in them, are worked out before this is entered)
 template <typename Fn, typename Which, typename... Args>
@@ -342,6 +363,179 @@ PyObject* attention_prefill(Args v, Py_ssize_t n) {
                   static_cast<int*>(at_(status)), floats(sinks), real(v[22]), small(v[23]), floats(slopes), stream());
 }
 
+// what the caller put together wrongly, in words
+#define REFUSE_UNLESS(condition, words) do { if (!(condition)) fail(kernel_error, words); } while (0)
+
+// tensors of one call on the current device, to whose current stream it goes
+void here(std::initializer_list<T> all) {
+    on_device(all);
+    const int now = c10::cuda::current_device();
+    for (T t : all)
+        if (t && t->get_device() != now) {
+            const std::string where = "a tensor on " + t->device().str() + " in a call on cuda:" + std::to_string(now) + "; make its device the current one (torch.cuda.device)";
+            fail(kernel_error, where.c_str());
+        }
+}
+
+// a list of numbers that the host knows (a list or a tuple; the caller makes one of anything else)
+std::vector<int> numbers(PyObject* o, const char* name, Py_ssize_t want = -1) {
+    const bool list = PyList_Check(o);
+    if (!list && !PyTuple_Check(o)) fail(PyExc_TypeError, "a list or a tuple expected");
+    const Py_ssize_t n = list ? PyList_GET_SIZE(o) : PyTuple_GET_SIZE(o);
+    std::vector<int> out;
+    bool good = want < 0 || n == want;
+    for (Py_ssize_t i = 0; good && i < n; ++i) {
+        PyObject* item = list ? PyList_GET_ITEM(o, i) : PyTuple_GET_ITEM(o, i);
+        int over = 0;
+        long long v = 0;
+        if (PyLong_Check(item)) v = PyLong_AsLongLongAndOverflow(item, &over);
+        else {
+            PyObject* whole_one = PyNumber_Index(item);       // (numpy's whole numbers; a list that changes under this is the caller's own doing and seen below)
+            if (!whole_one) { PyErr_Clear(); good = false; break; }
+            v = PyLong_AsLongLongAndOverflow(whole_one, &over);
+            Py_DECREF(whole_one);
+            if (list && PyList_GET_SIZE(o) != n) { good = false; break; }
+        }
+        if (over || v < INT32_MIN || v > INT32_MAX) good = false;
+        out.push_back(static_cast<int>(v));
+    }
+    if (!good) {
+        const std::string what = std::string(name) + " must be a list of whole numbers of 32 bits" + (want >= 0 ? ", " + std::to_string(want) + " of them" : "");
+        fail(kernel_error, what.c_str());
+    }
+    return out;
+}
+
+// pools (src, dst, src_pages, dst_pages, slots or None), multiprocessors -> (status, kernels launched)
+PyObject* copy_pages(Args v, Py_ssize_t n) {
+    count(n, 2);
+    if (!PyList_Check(v[0])) fail(PyExc_TypeError, "a list expected");
+    const Py_ssize_t pools = PyList_GET_SIZE(v[0]);
+    std::vector<PagePoolMoves> args(pools);
+    std::vector<std::vector<int>> lists(3 * pools);
+    std::vector<T> tensors;
+    bool any = false;
+    for (Py_ssize_t i = 0; i < pools; ++i) {
+        PyObject* one = PyList_GET_ITEM(v[0], i);
+        if (!PyTuple_Check(one) || PyTuple_GET_SIZE(one) != 5) fail(PyExc_TypeError, "pools as (src, dst, src_pages, dst_pages, slots)");
+        T src = tensor(PyTuple_GET_ITEM(one, 0)), dst = tensor(PyTuple_GET_ITEM(one, 1));
+        const int64_t d = src->dim();
+        bool alike = d >= 4 && dst->dim() == d && src->scalar_type() == dst->scalar_type();
+        for (int64_t k = 0; alike && k < d; ++k) alike = k == d - 4 || src->size(k) == dst->size(k);
+        if (!alike) {
+            std::ostringstream text;
+            text << "copy_pages: pools " << src->sizes() << " " << c10::toString(src->scalar_type()) << " and " << dst->sizes() << " " << c10::toString(dst->scalar_type())
+                 << " are alike in everything but their numbers of pages";
+            fail(kernel_error, text.str().c_str());
+        }
+        REFUSE_UNLESS(src->is_contiguous() && dst->is_contiguous(), "copy_pages: pools are contiguous");
+        std::vector<int>*mine = &lists[3 * i];
+        mine[0] = numbers(PyTuple_GET_ITEM(one, 2), "src_pages");
+        const Py_ssize_t moves = mine[0].size();
+        mine[1] = numbers(PyTuple_GET_ITEM(one, 3), "dst_pages", moves);
+        const bool some = PyTuple_GET_ITEM(one, 4) != Py_None;
+        if (some) mine[2] = numbers(PyTuple_GET_ITEM(one, 4), "slots", moves);
+        const bool nothing = src->numel() == 0 || dst->numel() == 0;
+        REFUSE_UNLESS(!nothing || moves == 0, "copy_pages: a page or a number of slots outside its pool");
+        int64_t outer = 1;
+        for (int64_t k = 0; k < d - 4; ++k) outer *= src->size(k);
+        auto least = [](int64_t x) { return x > 0 ? x : 1; };
+        args[i] = PagePoolMoves{src->data_ptr(), dst->data_ptr(), least(outer), src->size(d - 4), dst->size(d - 4), least(src->size(d - 3)), least(src->size(d - 2)),
+                                least(src->size(d - 1) * (int64_t)src->element_size()), (long long)moves, mine[0].data(), mine[1].data(), some ? mine[2].data() : nullptr};
+        any = any || moves > 0;
+        tensors.push_back(src);
+        tensors.push_back(dst);
+    }
+    if (!any) return Py_BuildValue("(ii)", 0, 0);
+    for (T t : tensors) here({t});
+    int launched = 0;
+    PyObject* status = launch(copy_pages_fn, "wllm_copy_pages", (const PagePoolMoves*)args.data(), (int)pools, small(v[1]), &launched, stream());
+    PyObject* both = status ? Py_BuildValue("(Ni)", status, launched) : nullptr;
+    return both;
+}
+
+// tables, q_lens, ctx_lens, page_size, query heads a kv head, kv heads, rows of an item, keys of a tile, align, min_keys, CTAs at once, pinned memory
+//   -> (status, the plan's array, ints used, items, rows, keys saved, most results, tiles, tokens, longest context)
+PyObject* prefix_plan(Args v, Py_ssize_t n) {
+    count(n, 12);
+    struct View {
+        Py_buffer b;
+        bool held = false;
+        ~View() { if (held) PyBuffer_Release(&b); }
+    } view;
+    const int* tables = nullptr;
+    int64_t R = 0, width = 0;
+    if (THPVariable_Check(v[0])) {
+        T t = tensor(v[0]);
+        REFUSE_UNLESS(!t->is_cuda() && t->dim() == 2 && t->scalar_type() == at::kInt && t->is_contiguous(), "prefix_plan: block tables [requests, pages] of int32 on the host, contiguous");
+        tables = static_cast<const int*>(t->data_ptr());
+        R = t->size(0);
+        width = t->size(1);
+    } else {
+        if (PyObject_GetBuffer(v[0], &view.b, PyBUF_C_CONTIGUOUS | PyBUF_FORMAT) != 0) {
+            PyErr_Clear();
+            fail(kernel_error, "prefix_plan: block tables [requests, pages] of int32 on the host, contiguous");
+        }
+        view.held = true;
+        REFUSE_UNLESS(view.b.ndim == 2 && view.b.itemsize == 4 && view.b.format && std::string(view.b.format) == "i", "prefix_plan: block tables [requests, pages] of int32 on the host, contiguous");
+        tables = static_cast<const int*>(view.b.buf);
+        R = view.b.shape[0];
+        width = view.b.shape[1];
+    }
+    const std::vector<int> q = numbers(v[1], "q_lens", R), ctx = numbers(v[2], "ctx_lens", R);
+    long long tokens = 0, longest = 0;
+    for (int x : q) tokens += x;
+    for (int x : ctx) longest = x > longest ? x : longest;
+    long long info[8] = {0}, room = 8192 + 64 * (tokens > 0 ? tokens : 0);
+    const int caps[4] = {0, 0, 0, 0};
+    at::Tensor host;
+    PyObject* status = nullptr;
+    for (int go = 0; go < 2; ++go) {
+        host = at::empty({room}, at::TensorOptions().dtype(at::kInt).pinned_memory(truth(v[11])));
+        Py_XDECREF(status);
+        status = launch(plan_fn, "wllm_prefix_plan", tables, (long long)width, (int)R, q.data(), ctx.data(), small(v[3]), small(v[4]), small(v[5]), small(v[6]), small(v[7]), small(v[8]),
+                        small(v[9]), (int)INT32_MAX, small(v[10]), caps, static_cast<int*>(host.data_ptr()), room, info);
+        if (!status || PyLong_AsLong(status) != 4) break;
+        room = info[0];
+    }
+    if (!status) return nullptr;
+    return Py_BuildValue("(NNLLLLLLLL)", status, THPVariable_Wrap(host), info[0], info[1], info[2], info[3], info[4], info[5], tokens, longest);
+}
+
+// q, out, k_pages, v_pages, block_table, arrays, scratch, status, sinks, slopes, tokens, requests, width, ints of the plan, floats of scratch, rows, pairs, place of the positions,
+// chunks, nq, nkv, hd, vd, page_size, scale, cap, multiprocessors
+PyObject* prefix_attention(Args v, Py_ssize_t n) {
+    count(n, 27);
+    T q = tensor(v[0]), out = tensor(v[1]), kp = tensor(v[2]), vp = tensor(v[3]), table = tensor(v[4]), arrays = tensor(v[5]), scratch = tensor(v[6]), status = tensor(v[7]),
+      sinks = maybe(v[8]), slopes = maybe(v[9]);
+    here({q, out, kp, vp, table, arrays, scratch, sinks, slopes});
+    const int64_t tokens = whole(v[10]), requests = whole(v[11]), width = whole(v[12]);
+    const int nq = small(v[19]), nkv = small(v[20]), hd = small(v[21]), vd = small(v[22]), ps = small(v[23]), sms = small(v[26]);
+    const long long rows = whole(v[15]), pairs = whole(v[16]);
+    const float scale = real(v[24]), cap = real(v[25]);
+    const auto type = q->scalar_type();
+    REFUSE_UNLESS(f32(q) || b16(q), "prefix_attention: bfloat16 or float32");
+    REFUSE_UNLESS(shaped(q, {tokens, (int64_t)nq * hd}) && q->stride(1) == 1, "prefix_attention: q is [tokens of the plan, nq * hd]");
+    REFUSE_UNLESS(shaped(out, {tokens, (int64_t)nq * vd}) && out->stride(1) == 1 && out->scalar_type() == type, "prefix_attention: out is [tokens of the plan, nq * vd], of q's type");
+    REFUSE_UNLESS(kp->dim() == 4 && shaped(kp, {kp->size(0), nkv, ps, hd}) && kp->is_contiguous() && kp->scalar_type() == type, "prefix_attention: key pages are [pages, nkv, page_size, hd], of q's type");
+    REFUSE_UNLESS(shaped(vp, {kp->size(0), nkv, ps, vd}) && vp->is_contiguous() && vp->scalar_type() == type, "prefix_attention: value pages are [pages, nkv, page_size, vd], of q's type");
+    REFUSE_UNLESS(shaped(table, {requests, width}) && table->scalar_type() == at::kInt && table->is_contiguous(), "prefix_attention: the block table is the plan's, int32");
+    REFUSE_UNLESS(arrays->dim() == 1 && arrays->scalar_type() == at::kInt && arrays->is_contiguous() && arrays->numel() >= whole(v[13]), "prefix_attention: the plan's arrays are an int32 tensor");
+    REFUSE_UNLESS(f32(scratch) && scratch->is_contiguous() && scratch->numel() >= whole(v[14]), "prefix_attention: scratch is float32, of the floats that the plan says");
+    for (T t : {sinks, slopes}) REFUSE_UNLESS(!t || (f32(t) && shaped(t, {nq}) && t->is_contiguous()), "prefix_attention: sinks and slopes are float32 [nq]");
+    REFUSE_UNLESS(scale > 0 && cap >= 0, "prefix_attention: a scale above zero and a cap of zero (none) or above");
+    const int* plan = static_cast<const int*>(at_(arrays));
+    if (b16(q)) {
+        REFUSE_UNLESS(hd > 0 && hd <= 256 && hd % 8 == 0 && vd > 0 && vd <= 256 && vd % 8 == 0, "prefix_attention: head sizes in steps of 8 up to 256");
+        return launch(prefix_fn[hd / 8][vd / 8], Heads{hd, vd}, at_(q), (int)q->stride(0), at_(out), (int)out->stride(0), at_(kp), at_(vp), (long long)kp->size(0),
+                      static_cast<const int*>(at_(table)), (int)width, (int)tokens, nq, nkv, ps, scale, cap, floats(sinks), floats(slopes), plan, static_cast<float*>(at_(scratch)), rows,
+                      pairs, sms, static_cast<int*>(at_(status)), stream());
+    }
+    return launch(prefix_simt_fn, "wllm_paged_attention_simt_prefix", at_(q), (int)q->stride(0), at_(out), (int)out->stride(0), at_(kp), at_(vp), (int)kp->size(0),
+                  static_cast<const int*>(at_(table)), (int)width, (int)tokens, nq, nkv, hd, vd, ps, scale, cap, floats(sinks), floats(slopes), plan, plan + whole(v[17]),
+                  static_cast<float*>(at_(scratch)), small(v[18]), pairs, 2 * sms, stream());
+}
+
 // -- the module ---------------------------------------------------------------------------------------------------------------------
 PyObject* bind(Args v, Py_ssize_t n) {           // name, address
     count(n, 2);
@@ -355,6 +549,9 @@ PyObject* bind(Args v, Py_ssize_t n) {           // name, address
     else if (which == "wllm_sandwich_norm_offset") sandwich_fn = reinterpret_cast<SandwichFn>(p);
     else if (which == "wllm_rope_kv_write_general") rope_fn = reinterpret_cast<RopeFn>(p);
     else if (which == "wllm_rope_row_norm_kv_write") rope_row_fn = reinterpret_cast<RopeRowFn>(p);
+    else if (which == "wllm_prefix_plan") plan_fn = reinterpret_cast<PlanFn>(p);
+    else if (which == "wllm_paged_attention_simt_prefix") prefix_simt_fn = reinterpret_cast<PrefixSimtFn>(p);
+    else if (which == "wllm_copy_pages") copy_pages_fn = reinterpret_cast<CopyPagesFn>(p);
     else fail(PyExc_ValueError, "no such entry point");
     Py_RETURN_NONE;
 }
@@ -366,6 +563,15 @@ PyObject* bind_attention(Args v, Py_ssize_t n) { // head size, address of decode
     if (!d || !p) fail(PyExc_ValueError, "no address");
     decode_fn[hd] = reinterpret_cast<DecodeFn>(d);
     prefill_fn[hd] = reinterpret_cast<PrefillFn>(p);
+    Py_RETURN_NONE;
+}
+PyObject* bind_prefix(Args v, Py_ssize_t n) {    // key and value head sizes, address
+    count(n, 3);
+    const long long hd = whole(v[0]), vd = whole(v[1]);
+    if (hd < 1 || hd > 256 || vd < 1 || vd > 256 || hd % 8 || vd % 8) fail(PyExc_ValueError, "head sizes in steps of 8 up to 256");
+    void* p = PyLong_AsVoidPtr(v[2]);
+    if (!p) fail(PyExc_ValueError, "no address");
+    prefix_fn[hd / 8][vd / 8] = reinterpret_cast<PrefixFn>(p);
     Py_RETURN_NONE;
 }
 PyObject* errors(Args v, Py_ssize_t n) {         // the class that ops.KernelError is; what binds an entry point
@@ -391,7 +597,8 @@ PyObject* guarded(PyObject*, Args v, Py_ssize_t n) {
 }
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<name>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(bind_attention), METHOD(errors), METHOD(tc_gemm_ok), METHOD(gemm), METHOD(norm), METHOD(sandwich), METHOD(rope),
-                         METHOD(rope_row), METHOD(attention_decode), METHOD(attention_prefill), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(rope_row), METHOD(attention_decode), METHOD(attention_prefill), METHOD(bind_prefix), METHOD(copy_pages), METHOD(prefix_plan),
+                         METHOD(prefix_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "wllm_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

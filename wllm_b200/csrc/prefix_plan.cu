@@ -9,6 +9,7 @@
 #include "prefix_plan.cuh"
 
 #include <algorithm>
+#include <cstring>
 #include <new>
 #include <vector>
 
@@ -39,12 +40,14 @@ struct Planner {
             if (j - i >= 2) {
                 std::vector<int> group(next.begin() + i, next.begin() + j);
                 std::sort(group.begin(), group.end());
-                int p = from + 1, most = share[group[0]];
-                for (int r : group) most = std::min(most, share[r]);
-                for (; p < most; ++p) {
-                    bool same = true;
-                    for (size_t m = 1; m < group.size() && same; ++m) same = page(group[m], p) == page(group[0], p);
-                    if (!same) break;
+                int p = share[group[0]];                   // the first page on which they do not agree, row by row of the tables
+                const int* first = tables + group[0] * width;
+                for (size_t m = 1; m < group.size(); ++m) {
+                    const int* other = tables + group[m] * width;
+                    const int most = std::min(p, share[group[m]]);
+                    if (most <= from) { p = from; break; }
+                    const bool same = memcmp(first + from, other + from, (size_t)(most - from) * sizeof(int)) == 0;
+                    p = same ? most : (int)(std::mismatch(first + from, first + most, other + from).first - first);
                 }
                 int hi = (int)((long long)p * ps / align * align);
                 if (hi - key >= min_keys) {
@@ -60,7 +63,7 @@ struct Planner {
 };
 
 struct Tile { int token, tokens, key_lo, key_hi, request; bool own; };
-struct Item { int tile, key_lo, key_hi, row, order; };
+struct Item { int tile, key_lo, key_hi, row, length; };      // length: in tiles of keys
 
 long long padded(long long n) { return (n + 3) & ~3ll; }
 
@@ -87,8 +90,6 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             total += q_len[r];
             if (total > (1 << 26)) return WLLM_BAD_SIZE;
             if (q_len[r] == 0) continue;
-            for (int i = 0; i * (long long)page_size < ctx_len[r]; ++i)
-                if (p.page(r, i) < 0 || p.page(r, i) >= pool_pages) return PAGES_OUT_OF_RANGE;
             p.share[r] = (ctx_len[r] - q_len[r]) / page_size;
             all.push_back(r);
         }
@@ -99,6 +100,13 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
         for (int r : all) {
             p.segments.push_back({(int)p.members.size(), 1, p.cover[r], ctx_len[r], true});
             p.members.push_back(r);
+        }
+        for (const Segment& s : p.segments) {             // (shared pages are looked at once)
+            const int* held = tables + p.members[s.first] * width;
+            const int end = (int)((s.key_hi + (long long)page_size - 1) / page_size);
+            unsigned top = 0;                             // (a number below zero is a large one)
+            for (int i = s.key_lo / page_size; i < end; ++i) top = std::max(top, (unsigned)held[i]);
+            if (top >= (unsigned)pool_pages) return PAGES_OUT_OF_RANGE;
         }
         // tiles of rows: whole tokens of a segment's requests, one behind the other
         const int per_tile = tile_rows / rep;
@@ -124,6 +132,10 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
         auto keys_of = [&](const Tile& t) { return (t.key_hi - t.key_lo + key_tile - 1) / key_tile; };
         int longest = 1;
         for (const Tile& t : tiles) longest = std::max(longest, keys_of(t));
+        std::vector<int> alike(longest + 1, 0), lengths;         // tiles by how many tiles of keys they meet
+        for (const Tile& t : tiles)
+            if (alike[keys_of(t)]++ == 0) lengths.push_back(keys_of(t));
+        std::sort(lengths.begin(), lengths.end());
         const long long most_items = caps[0] > 0 ? caps[0] : (1 << 22);
         const double beside = 1.5;
         double best = 0;
@@ -131,16 +143,15 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
         bool any = false;
         for (int l = 1;; l = std::max(l + 1, l * 5 / 4)) {
             const int len = std::min(l, longest);
-            long long n = 0;
-            double work = 0;
+            long long n = 0, work = 0;
             int top = 0;
-            for (const Tile& t : tiles) {
-                const int k = keys_of(t), parts = (k + len - 1) / len;
-                n += parts;
-                work += k + beside * parts;
+            for (int k : lengths) {
+                const int parts = (k + len - 1) / len;
+                n += (long long)parts * alike[k];
+                work += (long long)k * alike[k];
                 top = std::max(top, (k + parts - 1) / parts);
             }
-            const double end = n * nkv <= ctas ? top + beside : std::max(top + beside, work * nkv / ctas + 0.5 * (top + beside));
+            const double all = work + beside * n, end = n * nkv <= ctas ? top + beside : std::max(top + beside, all * nkv / ctas + 0.5 * (top + beside));
             if (n <= most_items && (!any || end < best * 0.98)) {
                 best = end;
                 per = len;
@@ -156,14 +167,15 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             size_t j = i + 1;
             while (j < tiles.size() && !tiles[i].own && !tiles[j].own && tiles[j].request == tiles[i].request && tiles[j].key_lo == tiles[i].key_lo && tiles[j].key_hi == tiles[i].key_hi) ++j;
             const int k = keys_of(tiles[i]), parts = (k + per - 1) / per;
-            for (int s = 0; s < parts; ++s)
+            for (int s = 0; s < parts; ++s) {
+                const int from = (int)((long long)k * s / parts), to = (int)((long long)k * (s + 1) / parts);
                 for (size_t t = i; t < j; ++t) {
-                    const int lo = tiles[i].key_lo + (int)((long long)k * s / parts) * key_tile, hi = std::min(tiles[i].key_hi, tiles[i].key_lo + (int)((long long)k * (s + 1) / parts) * key_tile);
-                    items.push_back({(int)t, lo, hi, (int)rows, (int)items.size()});
+                    items.push_back({(int)t, tiles[i].key_lo + from * key_tile, std::min(tiles[i].key_hi, tiles[i].key_lo + to * key_tile), (int)rows, to - from});
                     rows += (long long)tiles[t].tokens * rep;
                     results += tiles[t].tokens;
                     if (rows > 0x7fffffff / nkv) return WLLM_BAD_SIZE;
                 }
+            }
             i = j;
         }
         // results by token, in the order in which segments were found: ascending keys
@@ -180,7 +192,7 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             for (const Item& it : items)
                 for (int t = 0; t < tiles[it.tile].tokens; ++t) listed[next[tokens[tiles[it.tile].token + t]]++] = it.row + t * rep;
         }
-        std::stable_sort(items.begin(), items.end(), [&](const Item& a, const Item& b) { return (a.key_hi - a.key_lo + key_tile - 1) / key_tile > (b.key_hi - b.key_lo + key_tile - 1) / key_tile; });
+        std::stable_sort(items.begin(), items.end(), [](const Item& a, const Item& b) { return a.length > b.length; });
 
         const long long need[4] = {(long long)items.size(), (long long)tokens.size(), results, total};
         long long cap[4];

@@ -59,15 +59,6 @@ def _need_cuda(*tensors: torch.Tensor) -> None:
             raise KernelError("the engine's kernels run on a CUDA device only; got a tensor on " + str(t.device))
 
 
-def _one_device(*tensors) -> None:
-    """Tensors of one call lie on the current device: launches go to its current stream."""
-    _need_cuda(*tensors)
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != here:
-            raise KernelError(f"a tensor on {t.device} in a call on cuda:{here}; make its device the current one (torch.cuda.device)")
-
-
 def _ptr(t) -> c_void_p:
     return c_void_p(0 if t is None else t.data_ptr())
 
@@ -96,12 +87,17 @@ def _check(status: int, what: str) -> None:
 # The functions that a step calls most hand their arguments to csrc/host_calls.cpp, which checks them, calls the entry point and returns its status.
 _host = None
 _HOST_FAMILIES = {"wllm_gemm_bf16_tc_params": "gemm_bf16_tc", "wllm_norm": "norm", "wllm_sandwich_norm_offset": "norm",
-                  "wllm_rope_kv_write_general": "rope_cache", "wllm_rope_row_norm_kv_write": "rope_cache"}
+                  "wllm_rope_kv_write_general": "rope_cache", "wllm_rope_row_norm_kv_write": "rope_cache", "wllm_prefix_plan": "prefix_plan",
+                  "wllm_paged_attention_simt_prefix": "attention_simt", "wllm_copy_pages": "cache_pages"}
 
 
 def _bind(what) -> None:
-    """The module of native calls needs an entry point (its name), or the attention of a head size (the size), for a call that has passed its checks."""
-    if isinstance(what, int):
+    """The module of native calls needs an entry point (its name), the attention of a head size (the size) or that of shared prefixes (the key and value head
+    sizes), for a call that has passed its checks."""
+    if isinstance(what, tuple):
+        lib = load_family("prefix_attention", {"HEAD_DIM": what[0], "VALUE_DIM": what[1]})
+        _host.bind_prefix(*what, entry_address(lib, "wllm_prefix_attention"))
+    elif isinstance(what, int):
         lib = load_family("attention_mma", {"HEAD_DIM": what})
         _host.bind_attention(what, entry_address(lib, "wllm_attention_mma_decode_biased"), entry_address(lib, "wllm_attention_mma_prefill_biased"))
     else:
@@ -768,20 +764,34 @@ def attention_mma_prefill(q, out, k_pages, v_pages, req_q_start, req_q_len, req_
     launches += 1
 
 
+def _numbers(values) -> list:
+    """Numbers known on the host as a list (the native calls look at what stands in it)."""
+    if isinstance(values, (list, tuple)):
+        return values
+    if isinstance(values, torch.Tensor) and values.is_cuda:
+        raise KernelError("numbers that the host knows are asked for: a list, an array or a tensor of the CPU")
+    if isinstance(values, (torch.Tensor, np.ndarray)) and values.ndim == 1:
+        return values.tolist()
+    raise KernelError(f"a list of whole numbers is asked for, not {type(values).__name__}")
+
+
 class PrefixPlan:
     """How a batch whose requests share pages is attended to (csrc/prefix_plan.cuh): made once for a step and a layout of heads, read by every layer of it."""
+    __slots__ = ("key", "requests", "width", "n_tokens", "host", "used", "items", "rows", "saved_keys", "most_results", "tiles", "max_chunks", "scratch_floats", "launch")
 
-    def __init__(self, key: tuple, requests: int, width: int, n_tokens: int, info, host: torch.Tensor, max_ctx: int, fixed: bool):
+    def __init__(self, key: tuple, requests: int, width: int, host: torch.Tensor, used: int, items: int, rows: int, saved: int, most: int, tiles: int, n_tokens: int, max_ctx: int):
         self.key, self.requests, self.width, self.n_tokens = key, requests, width, n_tokens
-        self.used, self.items, self.rows, self.saved_keys, self.most_results, self.tiles = (int(info[i]) for i in range(6))
-        self.host, self.fixed = host[:self.used], fixed      # int32 on the host, pinned where there is a device
+        self.host = host[:used]                # int32 on the host, pinned where there is a device
+        self.used, self.items, self.rows, self.saved_keys, self.most_results, self.tiles = used, items, rows, saved, most, tiles
         page_size, nq, nkv, hd, vd, dtype = key
         self.max_chunks = max(1, -(-max_ctx // SIMT_CHUNK))
-        self.scratch_floats = nkv * self.rows * (vd + 2) if dtype == torch.bfloat16 else n_tokens * nq * self.max_chunks * (vd + 2)
+        self.scratch_floats = nkv * rows * (vd + 2) if dtype == torch.bfloat16 else n_tokens * nq * self.max_chunks * (vd + 2)
+        # what the native call takes of it
+        self.launch = (n_tokens, requests, width, used, self.scratch_floats, rows, items * nkv, int(host[6]) if used else 0, self.max_chunks, nq, nkv, hd, vd, page_size)
 
     def to(self, device) -> torch.Tensor:
         """The plan's array on the device, as prefix_attention takes it (in the current stream's order)."""
-        return torch.empty(self.used, dtype=torch.int32, device=device).copy_(self.host, non_blocking=True)
+        return self.host.to(device, non_blocking=True)
 
 
 PREFIX_MIN_KEYS = 128
@@ -795,7 +805,7 @@ def prefix_rows(dtype: torch.dtype) -> int:
 def prefix_ok(nq: int, nkv: int, hd: int, vd: int, page_size: int, dtype: torch.dtype) -> bool:
     """Head layouts and pages that prefix_attention is built for."""
     return dtype in (torch.bfloat16, torch.float32) and nkv > 0 and nq % nkv == 0 and 0 < nq // nkv <= prefix_rows(dtype) and \
-        all(0 < d <= 256 and d % 8 == 0 for d in (hd, vd)) and page_size >= 16 and page_size & (page_size - 1) == 0
+        0 < hd <= 256 and hd % 8 == 0 and 0 < vd <= 256 and vd % 8 == 0 and page_size >= 16 and page_size & (page_size - 1) == 0
 
 
 def prefix_plan(tables, q_lens, ctx_lens, page_size: int, nq: int, nkv: int, hd: int, vd: int | None = None, dtype: torch.dtype = torch.bfloat16,
@@ -805,33 +815,14 @@ def prefix_plan(tables, q_lens, ctx_lens, page_size: int, nq: int, nkv: int, hd:
     `min_keys` shared keys are left to each request.  A plan holds for any pools and any queries of these tables and lengths."""
     vd = hd if vd is None else vd
     if not prefix_ok(nq, nkv, hd, vd, page_size, dtype):
-        raise KernelError(f"prefix_plan: {nq} query heads on {nkv}, sizes {hd}/{vd}, pages of {page_size}, {dtype}: up to {prefix_rows(dtype) if dtype in (torch.bfloat16, torch.float32) else 0} "
-                          "query heads a key/value head, head sizes in steps of 8 up to 256, pages of a power of two of at least 16 tokens, bfloat16 or float32")
-    if isinstance(tables, torch.Tensor):
-        if tables.is_cuda:
-            raise KernelError("prefix_plan: block tables on the host")
-        tables = tables.numpy()
-    if tables.ndim != 2 or tables.dtype != np.int32:
-        raise KernelError("prefix_plan: block tables [requests, pages] of int32")
-    tables = np.ascontiguousarray(tables)
-    R, width = tables.shape
-    q, ctx = _whole_numbers(q_lens, "q_lens", R), _whole_numbers(ctx_lens, "ctx_lens", R)
-    n, max_ctx = int(q.sum(dtype=np.int64)), int(ctx.max(initial=0))
+        raise KernelError(f"prefix_plan: {nq} query heads on {nkv}, sizes {hd}/{vd}, pages of {page_size}, {dtype}: up to 128 query heads a key/value head in bfloat16, 32 in float32, "
+                          "head sizes in steps of 8 up to 256, pages of a power of two of at least 16 tokens")
     bf16 = dtype == torch.bfloat16
-    lib = load_family("prefix_plan")
-    info = (ctypes.c_longlong * 8)()
-    room = 4096 + 32 * n
-    while True:
-        host = torch.empty(room, dtype=torch.int32, pin_memory=torch.cuda.is_available())
-        status = lib.wllm_prefix_plan(c_void_p(tables.ctypes.data), ctypes.c_longlong(width), R, c_void_p(q.ctypes.data), c_void_p(ctx.ctypes.data), page_size, nq // nkv, nkv,
-                                      prefix_rows(dtype), 128 if bf16 else SIMT_CHUNK, 1 if bf16 else SIMT_CHUNK, max(1, min_keys), 0x7fffffff, sm_count() if bf16 else 2 * sm_count(),
-                                      (ctypes.c_int * 4)(), c_void_p(host.data_ptr()), ctypes.c_longlong(room), info)
-        if status != 4:
-            break
-        room = int(info[0])
+    status, *made = _host_calls().prefix_plan(tables, _numbers(q_lens), _numbers(ctx_lens), page_size, nq // nkv, nkv, prefix_rows(dtype), 128 if bf16 else SIMT_CHUNK,
+                                              1 if bf16 else SIMT_CHUNK, max(1, min_keys), sm_count() if bf16 else 2 * sm_count(), torch.cuda.is_available())
     if status:
         raise KernelError(f"prefix_plan: {_STATUS.get(status, status)}")
-    return PrefixPlan((page_size, nq, nkv, hd, vd, dtype), R, width, n, info, host, max_ctx, False)
+    return PrefixPlan((page_size, nq, nkv, hd, vd, dtype), tables.shape[0], tables.shape[1], *made)
 
 
 def prefix_attention(q, out, k_pages, v_pages, block_table, plan: PrefixPlan, arrays: torch.Tensor, nq: int, nkv: int, hd: int, page_size: int, scale: float, scratch: torch.Tensor,
@@ -839,60 +830,15 @@ def prefix_attention(q, out, k_pages, v_pages, block_table, plan: PrefixPlan, ar
     """Attention of a planned batch (csrc/prefix_attention.cu; 32-bit: csrc/attention_simt.cu, bit for bit what the other 32-bit kernels give): q [tokens, nq * hd] (row stride free),
     out [tokens, nq * vd], pages [pages, nkv, page_size, hd | vd], `block_table` [requests, pages] the tables of the plan on the device, `arrays` = plan.to(device), `scratch` float32 of at
     least plan.scratch_floats, which the call alone uses while it runs.  Every earlier key is seen (no window).  `sinks`, `cap`, `slopes`: as for attention_mma_decode."""
-    vd = hd if vd is None else vd
-
-    def need(ok, what):
-        if not ok:
-            raise KernelError("prefix_attention: " + what)
-    _one_device(q, out, k_pages, v_pages, block_table, arrays, scratch, sinks, slopes)
-    need(plan.key == (page_size, nq, nkv, hd, vd, q.dtype), f"a plan for (page size, heads, kv heads, sizes, type) {plan.key}, not {(page_size, nq, nkv, hd, vd, q.dtype)}")
-    need(q.dim() == 2 and q.shape == (plan.n_tokens, nq * hd) and q.stride(1) == 1, f"q [{plan.n_tokens}, {nq * hd}]")
-    need(out.dim() == 2 and out.shape == (plan.n_tokens, nq * vd) and out.stride(1) == 1 and out.dtype == q.dtype, f"out [{plan.n_tokens}, {nq * vd}]")
-    need(k_pages.dim() == 4 and k_pages.shape[1:] == (nkv, page_size, hd) and k_pages.is_contiguous() and k_pages.dtype == q.dtype, f"key pages [.., {nkv}, {page_size}, {hd}]")
-    need(v_pages.shape == (k_pages.shape[0], nkv, page_size, vd) and v_pages.is_contiguous() and v_pages.dtype == q.dtype, f"value pages [{k_pages.shape[0]}, {nkv}, {page_size}, {vd}]")
-    need(block_table.dtype == torch.int32 and block_table.shape == (plan.requests, plan.width) and block_table.is_contiguous(), f"block table [{plan.requests}, {plan.width}]")
-    need(arrays.dtype == torch.int32 and arrays.is_contiguous() and arrays.dim() == 1 and arrays.numel() >= plan.used, "the plan's arrays")
-    need(scratch.dtype == torch.float32 and scratch.is_contiguous() and scratch.numel() >= plan.scratch_floats, f"{plan.scratch_floats} floats of scratch")
-    for t, name in ((sinks, "sinks"), (slopes, "slopes")):
-        need(t is None or (t.dtype == torch.float32 and t.shape == (nq,) and t.is_contiguous()), f"{name} [{nq}] of float32")
-    need(scale > 0 and cap >= 0, "a scale above zero and a cap of zero (none) or above")
+    if plan.key != (page_size, nq, nkv, hd, hd if vd is None else vd, q.dtype):
+        raise KernelError(f"prefix_attention: a plan for (page size, heads, kv heads, sizes, type) {plan.key}, not {(page_size, nq, nkv, hd, hd if vd is None else vd, q.dtype)}")
     if plan.n_tokens == 0:
         return
-    pairs = plan.items * nkv
-    if q.dtype == torch.bfloat16:
-        lib = load_family("prefix_attention", {"HEAD_DIM": hd, "VALUE_DIM": vd})
-        status = lib.wllm_prefix_attention(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(k_pages), _ptr(v_pages), ctypes.c_longlong(k_pages.shape[0]), _ptr(block_table),
-                                           plan.width, plan.n_tokens, nq, nkv, page_size, c_float(scale), c_float(cap), _ptr(sinks), _ptr(slopes), _ptr(arrays), _ptr(scratch),
-                                           ctypes.c_longlong(plan.rows), ctypes.c_longlong(pairs), sm_count(), _ptr(_device_status(q.device)), _stream())
-    else:
-        positions = c_void_p(arrays.data_ptr() + 4 * int(plan.host[6]))
-        status = load_family("attention_simt").wllm_paged_attention_simt_prefix(
-            _ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(k_pages), _ptr(v_pages), k_pages.shape[0], _ptr(block_table), plan.width, plan.n_tokens, nq, nkv, hd, vd, page_size,
-            c_float(scale), c_float(cap), _ptr(sinks), _ptr(slopes), _ptr(arrays), positions, _ptr(scratch), plan.max_chunks, ctypes.c_longlong(pairs), 2 * sm_count(), _stream())
-    _check(status, f"prefix_attention(head_dim={hd}/{vd}, heads={nq}/{nkv})")
+    status = _host_calls().prefix_attention(q, out, k_pages, v_pages, block_table, arrays, scratch, _device_status(q.device), sinks, slopes, *plan.launch, scale, cap, sm_count())
+    if status:
+        _check(status, f"prefix_attention(head_dim={hd}/{vd}, heads={nq}/{nkv})")
     global launches
-    launches += 1    # (with the merge kernel)
-
-
-class _PoolMoves(ctypes.Structure):
-    _fields_ = [("src", c_void_p), ("dst", c_void_p)] + [(name, ctypes.c_longlong) for name in ("outer", "src_pages", "dst_pages", "heads", "slots", "row_bytes", "moves")] + \
-        [(name, c_void_p) for name in ("src_list", "dst_list", "slot_list")]
-
-
-def _whole_numbers(values, name: str, count: int | None = None) -> np.ndarray:
-    """A list of page numbers, slots or lengths known on the host as an int32 array."""
-    if isinstance(values, torch.Tensor):
-        if values.is_cuda:
-            raise KernelError(f"{name} is known on the host: a list, an array or a tensor of the CPU")
-        values = values.numpy()
-    a = np.asarray(values)
-    if a.size == 0:
-        a = a.astype(np.int32)
-    if a.ndim != 1 or a.dtype.kind not in "iu" or (count is not None and a.shape[0] != count):
-        raise KernelError(f"{name} must be a list of whole numbers" + (f", {count} of them" if count is not None else ""))
-    if a.size and not (-(1 << 31) <= int(a.min()) and int(a.max()) < 1 << 31):
-        raise KernelError(f"{name}: {_STATUS[7]}")
-    return np.ascontiguousarray(a, dtype=np.int32)
+    launches += 2    # (with the merge kernel)
 
 
 MAX_COPY_POOLS = 16
@@ -903,42 +849,12 @@ def copy_pages(moves) -> None:
     `src` and `dst` [..., pages, heads, slots of a page, row], contiguous, alike but for their numbers of pages (`dst` may be `src`); the lists of pages are known
     on the host (lists, arrays); `slots`: how many slots of each page hold tokens (of every head's run the first that many rows are copied, the others stay as they
     are), or None: all.  All of it happens at once: no page is a destination twice, none is destination and source, and no destination pool overlaps another pool."""
-    moves = list(moves)
+    moves = [(src, dst, _numbers(a), _numbers(b), None if slots is None else _numbers(slots)) for src, dst, a, b, slots in moves]
     if len(moves) > MAX_COPY_POOLS:
         raise KernelError(f"copy_pages: {len(moves)} pools in one call, at most {MAX_COPY_POOLS}")
-    args, kept = (_PoolMoves * max(1, len(moves)))(), []
-    device = None
-    for a, (src, dst, src_pages, dst_pages, slots) in zip(args, moves):
-        if src.dim() < 4 or src.dim() != dst.dim() or src.dtype != dst.dtype or src.shape[:-4] != dst.shape[:-4] or src.shape[-3:] != dst.shape[-3:]:
-            raise KernelError(f"copy_pages: pools {tuple(src.shape)} {src.dtype} and {tuple(dst.shape)} {dst.dtype} are alike in everything but their numbers of pages")
-        if not (src.is_contiguous() and dst.is_contiguous()):
-            raise KernelError("copy_pages: pools are contiguous")
-        if src.device != dst.device or (device is not None and src.device != device):
-            raise KernelError("copy_pages: the pools of a call lie on one device")
-        device = src.device
-        from_list = _whole_numbers(src_pages, "src_pages")
-        n = from_list.shape[0]
-        lists = [from_list, _whole_numbers(dst_pages, "dst_pages", n), None if slots is None else _whole_numbers(slots, "slots", n)]
-        kept.append(lists)
-        outer = 1
-        for d in src.shape[:-4]:
-            outer *= d
-        if src.numel() == 0 or dst.numel() == 0:
-            if n:
-                raise KernelError(f"copy_pages: {_STATUS[7]}")
-            outer = 1
-        a.src, a.dst = src.data_ptr(), dst.data_ptr()
-        a.outer, a.src_pages, a.dst_pages, a.heads, a.slots = outer, src.shape[-4], dst.shape[-4], max(1, src.shape[-3]), max(1, src.shape[-2])
-        a.row_bytes, a.moves = max(1, src.shape[-1] * src.element_size()), n
-        a.src_list, a.dst_list = lists[0].ctypes.data, lists[1].ctypes.data
-        a.slot_list = None if slots is None else lists[2].ctypes.data
-    if not any(lists[0].shape[0] for lists in kept):
-        return
-    _one_device(*[t for src, dst, *_ in moves for t in (src, dst)])
-    done = ctypes.c_int(0)
-    status = load_family("cache_pages").wllm_copy_pages(args, len(moves), sm_count(), ctypes.byref(done), _stream())
+    status, launched = _host_calls().copy_pages(moves, sm_count())
     global launches
-    launches += done.value
+    launches += launched
     if status:
         _check(status, "copy_pages")
 

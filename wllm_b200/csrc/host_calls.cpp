@@ -145,7 +145,7 @@ typedef int (*PrefillFn)(const void*, int, void*, int, const void*, const void*,
 
 typedef int (*PlanFn)(const int*, long long, int, const int*, const int*, int, int, int, int, int, int, int, int, int, const int*, int*, long long, long long*);
 typedef int (*PrefixFn)(const void*, int, void*, int, const void*, const void*, long long, const int*, int, int, int, int, int, float, float, const float*, const float*, const int*,
-                        float*, long long, long long, int, int*, void*);
+                        int, int, int, float*, long long, long long, int, int*, void*);
 typedef int (*PrefixSimtFn)(const void*, int, void*, int, const void*, const void*, int, const int*, int, int, int, int, int, int, int, float, float, const float*, const float*,
                             const int*, const int*, float*, int, long long, int, void*);
 struct PagePoolMoves {                 // as csrc/cache_pages.cu has it
@@ -503,9 +503,9 @@ PyObject* prefix_plan(Args v, Py_ssize_t n) {
 }
 
 // q, out, k_pages, v_pages, block_table, arrays, scratch, status, sinks, slopes, tokens, requests, width, ints of the plan, floats of scratch, rows, pairs, place of the positions,
-// chunks, nq, nkv, hd, vd, page_size, scale, cap, multiprocessors
+// chunks, nq, nkv, hd, vd, page_size, scale, cap, multiprocessors, places of the items and the tokens, items (-1: the header says)
 PyObject* prefix_attention(Args v, Py_ssize_t n) {
-    count(n, 27);
+    count(n, 30);
     T q = tensor(v[0]), out = tensor(v[1]), kp = tensor(v[2]), vp = tensor(v[3]), table = tensor(v[4]), arrays = tensor(v[5]), scratch = tensor(v[6]), status = tensor(v[7]),
       sinks = maybe(v[8]), slopes = maybe(v[9]);
     here({q, out, kp, vp, table, arrays, scratch, sinks, slopes});
@@ -528,8 +528,8 @@ PyObject* prefix_attention(Args v, Py_ssize_t n) {
     if (b16(q)) {
         REFUSE_UNLESS(hd > 0 && hd <= 256 && hd % 8 == 0 && vd > 0 && vd <= 256 && vd % 8 == 0, "prefix_attention: head sizes in steps of 8 up to 256");
         return launch(prefix_fn[hd / 8][vd / 8], Heads{hd, vd}, at_(q), (int)q->stride(0), at_(out), (int)out->stride(0), at_(kp), at_(vp), (long long)kp->size(0),
-                      static_cast<const int*>(at_(table)), (int)width, (int)tokens, nq, nkv, ps, scale, cap, floats(sinks), floats(slopes), plan, static_cast<float*>(at_(scratch)), rows,
-                      pairs, sms, static_cast<int*>(at_(status)), stream());
+                      static_cast<const int*>(at_(table)), (int)width, (int)tokens, nq, nkv, ps, scale, cap, floats(sinks), floats(slopes), plan, small(v[27]), small(v[28]), small(v[29]),
+                      static_cast<float*>(at_(scratch)), rows, pairs, sms, static_cast<int*>(at_(status)), stream());
     }
     return launch(prefix_simt_fn, "wllm_paged_attention_simt_prefix", at_(q), (int)q->stride(0), at_(out), (int)out->stride(0), at_(kp), at_(vp), (int)kp->size(0),
                   static_cast<const int*>(at_(table)), (int)width, (int)tokens, nq, nkv, hd, vd, ps, scale, cap, floats(sinks), floats(slopes), plan, plan + whole(v[17]),

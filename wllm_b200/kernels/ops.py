@@ -777,7 +777,7 @@ def _numbers(values) -> list:
 
 class PrefixPlan:
     """How a batch whose requests share pages is attended to (csrc/prefix_plan.cuh): made once for a step and a layout of heads, read by every layer of it."""
-    __slots__ = ("key", "requests", "width", "n_tokens", "host", "used", "items", "rows", "saved_keys", "most_results", "tiles", "max_chunks", "scratch_floats", "launch")
+    __slots__ = ("key", "requests", "width", "n_tokens", "host", "used", "items", "rows", "saved_keys", "most_results", "tiles", "max_chunks", "scratch_floats", "launch", "places")
 
     def __init__(self, key: tuple, requests: int, width: int, host: torch.Tensor, used: int, items: int, rows: int, saved: int, most: int, tiles: int, n_tokens: int, max_ctx: int):
         self.key, self.requests, self.width, self.n_tokens = key, requests, width, n_tokens
@@ -788,6 +788,7 @@ class PrefixPlan:
         self.scratch_floats = nkv * rows * (vd + 2) if dtype == torch.bfloat16 else n_tokens * nq * self.max_chunks * (vd + 2)
         # what the native call takes of it
         self.launch = (n_tokens, requests, width, used, self.scratch_floats, rows, items * nkv, int(host[6]) if used else 0, self.max_chunks, nq, nkv, hd, vd, page_size)
+        self.places = (int(host[2]), int(host[3]), items) if used else (0, 0, 0)
 
     def to(self, device) -> torch.Tensor:
         """The plan's array on the device, as prefix_attention takes it (in the current stream's order)."""
@@ -797,14 +798,14 @@ class PrefixPlan:
 PREFIX_MIN_KEYS = 128
 
 
-def prefix_rows(dtype: torch.dtype) -> int:
-    """Rows (token, query head of the group) of an item of a plan, at most."""
-    return 128 if dtype == torch.bfloat16 else 32
+def prefix_rows(dtype: torch.dtype, hd: int, vd: int) -> int:
+    """Rows (token, query head of the group) of an item of a plan, at most (csrc/prefix_attention.cu: ROWS)."""
+    return 32 if dtype == torch.float32 else 256 if hd <= 128 and vd <= 128 else 128
 
 
 def prefix_ok(nq: int, nkv: int, hd: int, vd: int, page_size: int, dtype: torch.dtype) -> bool:
     """Head layouts and pages that prefix_attention is built for."""
-    return dtype in (torch.bfloat16, torch.float32) and nkv > 0 and nq % nkv == 0 and 0 < nq // nkv <= prefix_rows(dtype) and \
+    return dtype in (torch.bfloat16, torch.float32) and nkv > 0 and nq % nkv == 0 and 0 < nq // nkv <= (128 if dtype == torch.bfloat16 else 32) and \
         0 < hd <= 256 and hd % 8 == 0 and 0 < vd <= 256 and vd % 8 == 0 and page_size >= 16 and page_size & (page_size - 1) == 0
 
 
@@ -818,7 +819,7 @@ def prefix_plan(tables, q_lens, ctx_lens, page_size: int, nq: int, nkv: int, hd:
         raise KernelError(f"prefix_plan: {nq} query heads on {nkv}, sizes {hd}/{vd}, pages of {page_size}, {dtype}: up to 128 query heads a key/value head in bfloat16, 32 in float32, "
                           "head sizes in steps of 8 up to 256, pages of a power of two of at least 16 tokens")
     bf16 = dtype == torch.bfloat16
-    status, *made = _host_calls().prefix_plan(tables, _numbers(q_lens), _numbers(ctx_lens), page_size, nq // nkv, nkv, prefix_rows(dtype), 128 if bf16 else SIMT_CHUNK,
+    status, *made = _host_calls().prefix_plan(tables, _numbers(q_lens), _numbers(ctx_lens), page_size, nq // nkv, nkv, prefix_rows(dtype, hd, vd), 128 if bf16 else SIMT_CHUNK,
                                               1 if bf16 else SIMT_CHUNK, max(1, min_keys), sm_count() if bf16 else 2 * sm_count(), torch.cuda.is_available())
     if status:
         raise KernelError(f"prefix_plan: {_STATUS.get(status, status)}")
@@ -834,7 +835,7 @@ def prefix_attention(q, out, k_pages, v_pages, block_table, plan: PrefixPlan, ar
         raise KernelError(f"prefix_attention: a plan for (page size, heads, kv heads, sizes, type) {plan.key}, not {(page_size, nq, nkv, hd, hd if vd is None else vd, q.dtype)}")
     if plan.n_tokens == 0:
         return
-    status = _host_calls().prefix_attention(q, out, k_pages, v_pages, block_table, arrays, scratch, _device_status(q.device), sinks, slopes, *plan.launch, scale, cap, sm_count())
+    status = _host_calls().prefix_attention(q, out, k_pages, v_pages, block_table, arrays, scratch, _device_status(q.device), sinks, slopes, *plan.launch, scale, cap, sm_count(), *plan.places)
     if status:
         _check(status, f"prefix_attention(head_dim={hd}/{vd}, heads={nq}/{nkv})")
     global launches

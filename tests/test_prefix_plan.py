@@ -49,8 +49,13 @@ def check(plan, tables, q_lens, ctx_lens, ps, rep, tile_rows, align):
         assert mine and all(m[0] == t for m in mine) and [m[1] for m in mine] == sorted(m[1] for m in mine)
     taken = sorted(rows)
     assert all(b - a >= rep for a, b in zip(taken, taken[1:]))
-    lengths = [-(-int(i[3] - i[2]) // (64 if tile_rows == 32 else 128)) for i in items]
-    assert lengths == sorted(lengths, reverse=True)
+    costs = ops._prefix_costs(torch.float32 if tile_rows == 32 else torch.bfloat16, 8, 8)
+    keys = 64 if tile_rows == 32 else 128
+    dear = [-(-int(i[3] - i[2]) // keys) * costs[2 if i[1] * rep <= costs[4] else 0] for i in items]
+    assert dear == sorted(dear, reverse=True)
+    for first, count, *_, begins in items.tolist():
+        mine = [int(tokens[2 * (first + i)]) for i in range(count)]
+        assert begins == (mine[0] if mine == list(range(mine[0], mine[0] + count)) else -1)
 
 
 TREES = [
@@ -76,7 +81,7 @@ def test_every_key_stands_in_one_item(tree, nq, nkv, dtype, ps):
     plan = ops.prefix_plan(b.table, b.q_lens, b.ctx_lens, ps, nq, nkv, 8, 8, dtype)
     assert plan.n_tokens == b.n
     bf16 = dtype == torch.bfloat16
-    check(plan, b.table.tolist(), b.q_lens, b.ctx_lens, ps, nq // nkv, ops.prefix_rows(dtype, 8, 8), 1 if bf16 else 64)
+    check(plan, b.table.tolist(), b.q_lens, b.ctx_lens, ps, nq // nkv, ops.prefix_rows(dtype), 1 if bf16 else 64)
 
 
 def test_shared_keys_are_counted_once_for_all():
@@ -94,7 +99,7 @@ def test_shared_keys_are_counted_once_for_all():
 def test_requests_that_bring_nothing_and_empty_batches():
     table = np.array([[3, 4], [-1, -1], [3, 9]], dtype=np.int32)
     plan = ops.prefix_plan(table, [1, 0, 2], [70, 0, 71], 64, 4, 2, 8, min_keys=64)
-    check(plan, table.tolist(), [1, 0, 2], [70, 0, 71], 64, 2, 256, 1)
+    check(plan, table.tolist(), [1, 0, 2], [70, 0, 71], 64, 2, 128, 1)
     empty = ops.prefix_plan(np.zeros((2, 3), dtype=np.int32), [0, 0], [0, 5], 64, 4, 2, 8)
     assert empty.n_tokens == empty.items == empty.rows == 0
     none = ops.prefix_plan(np.zeros((0, 3), dtype=np.int32), [], [], 64, 4, 2, 8)
@@ -126,4 +131,4 @@ def test_random_trees(seed):
     for dtype in (torch.bfloat16, torch.float32):
         plan = ops.prefix_plan(b.table, b.q_lens, b.ctx_lens, ps, nkv * rep, nkv, 8, 8, dtype, min_keys=rng.choice([1, 64, 128]))
         bf16 = dtype == torch.bfloat16
-        check(plan, b.table.tolist(), b.q_lens, b.ctx_lens, ps, rep, ops.prefix_rows(dtype, 8, 8), 1 if bf16 else 64)
+        check(plan, b.table.tolist(), b.q_lens, b.ctx_lens, ps, rep, ops.prefix_rows(dtype), 1 if bf16 else 64)

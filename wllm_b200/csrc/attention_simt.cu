@@ -761,8 +761,8 @@ paged_attention_simt_prefix_kernel(const float* __restrict__ q, int q_stride, co
                                    const int* __restrict__ block_table, int max_pages, const int* __restrict__ plan, int nq, int nkv, int hd, int page_size, float scale, int vd,
                                    float cap, const float* __restrict__ slopes, float* __restrict__ scratch, int max_chunks) {
     extern __shared__ __align__(16) unsigned char tl_smem[];
-    __shared__ size_t row_of[CHUNK];
-    pdl_begin();
+    __shared__ size_t row_of[CHUNK], q_of[TL_ROWS];
+    pdl_wait();                          // (the merge's CTAs would crowd on the SMs that this launch leaves free)
     const int rep = nq / nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, total = plan[PLAN_ITEMS] * nkv;
     float* qs = reinterpret_cast<float*>(tl_smem);                          // [32 rows][hd]
     float* ks = qs + TL_ROWS * hd;                                          // [32 keys][hd + 4]
@@ -783,6 +783,10 @@ paged_attention_simt_prefix_kernel(const float* __restrict__ q, int q_stride, co
         }
         for (int c = item[ITEM_KEY_LO] / CHUNK; c * CHUNK < key_hi; ++c) {
             __syncthreads();                                                // everyone is done with the chunk (and the queries) before
+            if (c == item[ITEM_KEY_LO] / CHUNK && threadIdx.x >= CHUNK && threadIdx.x < CHUNK + TL_ROWS) {
+                const int m = threadIdx.x - CHUNK;
+                if (m < rows) q_of[m] = (size_t)mine[2 * (m / rep)] * q_stride + (size_t)(g * rep + m % rep) * hd;
+            }
             if (threadIdx.x < CHUNK) {
                 const int key = min(c * CHUNK + (int)threadIdx.x, key_hi - 1), page = min(max(table[min(key / page_size, max_pages - 1)], 0), pool_pages - 1);
                 row_of[threadIdx.x] = ((size_t)page * nkv + g) * page_size + key % page_size;
@@ -793,8 +797,8 @@ paged_attention_simt_prefix_kernel(const float* __restrict__ q, int q_stride, co
             chunk_of_rows<float, NE>(qs, ks, vs, row_of, k_pages, v_pages, hd, vd, c, key_hi, scale, cap, pos_r, slope_r, [&]() {
                 if (first)
                     for (int idx = threadIdx.x; idx < TL_ROWS * hd; idx += blockDim.x) {
-                        const int m = idx / hd, d = idx % hd;
-                        qs[idx] = m < rows ? q[(size_t)mine[2 * (m / rep)] * q_stride + (size_t)(g * rep + m % rep) * hd + d] : 0.f;
+                        const int m = idx / hd, d = idx - m * hd;
+                        qs[idx] = m < rows ? q[q_of[m] + d] : 0.f;
                     }
             }, m_c, l_c, o_c);
 #pragma unroll

@@ -143,7 +143,7 @@ typedef int (*DecodeFn)(const void*, int, void*, int, const void*, const void*, 
 typedef int (*PrefillFn)(const void*, int, void*, int, const void*, const void*, long long, const int*, const int*, const int*, const int*, int, int, int, int, int,
                          int, int, float, int, int, int, float*, int*, const float*, float, int, const float*, void*);
 
-typedef int (*PlanFn)(const int*, long long, int, const int*, const int*, int, int, int, int, int, int, int, int, int, const int*, int*, long long, long long*);
+typedef int (*PlanFn)(const int*, long long, int, const int*, const int*, int, int, int, int, int, int, int, int, int, const int*, const int*, int*, long long, long long*);
 typedef int (*PrefixFn)(const void*, int, void*, int, const void*, const void*, long long, const int*, int, int, int, int, int, float, float, const float*, const float*, const int*,
                         int, int, int, float*, long long, long long, int, int*, void*);
 typedef int (*PrefixSimtFn)(const void*, int, void*, int, const void*, const void*, int, const int*, int, int, int, int, int, int, int, float, float, const float*, const float*,
@@ -454,10 +454,11 @@ PyObject* copy_pages(Args v, Py_ssize_t n) {
     return both;
 }
 
-// tables, q_lens, ctx_lens, page_size, query heads a kv head, kv heads, rows of an item, keys of a tile, align, min_keys, CTAs at once, pinned memory
+// tables, q_lens, ctx_lens, page_size, query heads a kv head, kv heads, rows of an item, keys of a tile, align, min_keys, CTAs at once, pinned memory, costs (six)
 //   -> (status, the plan's array, ints used, items, rows, keys saved, most results, tiles, tokens, longest context)
 PyObject* prefix_plan(Args v, Py_ssize_t n) {
-    count(n, 12);
+    count(n, 13);
+    const std::vector<int> costs = numbers(v[12], "costs", 6);
     struct View {
         Py_buffer b;
         bool held = false;
@@ -494,7 +495,7 @@ PyObject* prefix_plan(Args v, Py_ssize_t n) {
         host = at::empty({room}, at::TensorOptions().dtype(at::kInt).pinned_memory(truth(v[11])));
         Py_XDECREF(status);
         status = launch(plan_fn, "wllm_prefix_plan", tables, (long long)width, (int)R, q.data(), ctx.data(), small(v[3]), small(v[4]), small(v[5]), small(v[6]), small(v[7]), small(v[8]),
-                        small(v[9]), (int)INT32_MAX, small(v[10]), caps, static_cast<int*>(host.data_ptr()), room, info);
+                        small(v[9]), (int)INT32_MAX, small(v[10]), costs.data(), caps, static_cast<int*>(host.data_ptr()), room, info);
         if (!status || PyLong_AsLong(status) != 4) break;
         room = info[0];
     }

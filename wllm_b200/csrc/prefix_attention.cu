@@ -10,16 +10,22 @@
 // product have one type, and a relative rounding of 2^-9 a weight is that of the values themselves).
 //
 // A CTA takes (item, key/value head) pairs off the plan's list, to and fro (the list is sorted, longest first), so that a captured launch serves plans of any number of items.  Roles:
-//   warp 0      brings key and value tiles of 128 keys by TMA through the block table of the item's request, box by box of a page, into a ring of stages;
+//   warp 0      brings key and value tiles of 128 keys by TMA through the block table of the item's request, box by box of a page, into a ring of stages (the numbers of 32 boxes' pages
+//               are read at once and handed out by shuffle: a load of its own for every tile cost it 700 cycles);
 //   warp 1      one lane issues tcgen05.mma: S = Q K^T (Q and K from shared memory, M 128, N 128) into one of two score buffers, and O += P V (P from tensor memory, over the
-//               scores that it came from; V as it lies in the pages, MN-major);
-//   warps 4-11  two groups of four, a thread per row: the rows of Q into shared memory, then per tile the scores out of tensor memory, mask, exponentials, running maximum and sum, P
-//               back; the row of O is scaled again only when its maximum has grown by more than 2^8.
-// Two groups, because one alone spends most of its time on latencies: a tile's exponentials are 1,024 cycles of the SM's special function units, a group took 2.3 times that.  An item of more than
-// 128 rows gives each group 128 rows of its own (value heads of up to 128, whose two outputs fit tensor memory; the keys come into shared memory once for both).  In an item of up to 128
-// rows the groups take its tiles in turn: tile n's maxima need those of tile n - 1, which the other group hands over before it begins its exponentials.
+//               scores that it came from; V as it lies in the pages, MN-major).  It is one thread, so its descriptors are additions to precomputed ones (made one by one they cost 100 cycles a
+//               product, three times what the tensor core takes);
+//   warps 2-3   bring an item's rows of Q into shared memory while the item before is still in its last tiles;
+//   warps 4-11  two groups of four, a thread per row: per tile the scores out of tensor memory, mask, exponentials, running maximum and sum, P back; the row of O is scaled again only
+//               when its maximum has grown by more than 2^8.
+// The two groups take an item's tiles in turn, because one alone spends most of its time on latencies: tile n's maxima need those of tile n - 1, which the other group hands over before
+// it begins its exponentials.  Tensor memory: O in columns 0 .. 255 and two score buffers behind it, or, where O has at most 128 columns, three: then the scores of tile n + 2 need not wait for the
+// output of tile n, which a group's turn (600 cycles to read and compare 128 scores a row, 1,700 for the exponentials, 350 to hand them over) else has to wait out.
 // A warp without rows leaves the tensor core to multiply what lies there: row m of a product depends on row m of its operand alone, and such rows are stored nowhere.
-// Tensor memory: O (of the first group's rows, of the second's behind it) in columns 0 .. 255, the score buffers at 256 and 384.
+//
+// An item of up to 16 rows (a decoding request's own keys) would fill an eighth of such a tile, and its chain of waits (queries, scores, exponentials, output, each a round trip through
+// tensor memory) would be as long as a full one's.  There the eight warps multiply on mma.sync, straight from the ring: 16 keys of a tile each for the scores, an eighth of the values'
+// columns each for the output, with two barriers a tile (row maxima, weights).  8 x 8 requests on 4,000 keys, 16 heads of 256, half of whose items are such: see the table's figures below.
 //
 // Head sizes that are no multiple of 64 are widened to one in shared memory: a box copy that reaches past a row's end fills with zeros.  Boxes that hold none of an item's keys are not
 // copied; values behind its last key are cleared in shared memory before they are multiplied with their weight of zero (0 x NaN is no zero).
@@ -42,25 +48,26 @@ constexpr int BM = 128, BN = 128;
 constexpr int KW = HDP == 256 ? 128 : HDP, VW = VDP == 256 ? 128 : VDP;
 constexpr int KC = HDP / KW, VC = VDP / VW;
 constexpr int STAGE = BN * (KW > VW ? KW : VW) * 2;
-// groups of 128 rows that an item may have: two where both outputs fit tensor memory and both groups' queries leave the ring room for several tiles
-constexpr int GROUPS = VDP <= 128 && HDP <= 128 ? 2 : 1;
-constexpr int ROWS = GROUPS * BM;
-constexpr int Q_BYTES = BM * HDP * 2;              // of one group of rows
-constexpr int SMALL = ROWS * 8 + BM * 4 + 512;      // rows' places, maxima that the groups hand over, barriers
-constexpr int MOST_STAGES = (227 * 1024 - 1024 - GROUPS * Q_BYTES - SMALL) / STAGE;
+constexpr int BUFS = VDP <= 128 ? 3 : 2;           // score buffers
+constexpr int THIN = 16;                           // rows of an item that runs on mma.sync
+constexpr int Q_BYTES = BM * HDP * 2;
+constexpr int SMALL = 2 * BM * 4 + BM * 4 + 2 * BM * 4 + 512;      // rows' positions, maxima that the groups hand over, sums of the second group, barriers
+constexpr int MOST_STAGES = (227 * 1024 - Q_BYTES - SMALL) / STAGE;
 constexpr int STAGES = MOST_STAGES > 8 ? 8 : MOST_STAGES;
-static_assert(STAGES >= KC + VC || GROUPS == 1, "a tile's keys are in use while the values of the one before are");
 static_assert(STAGES >= 2, "a stage for keys and one for values");
-constexpr int SMEM = 1024 + GROUPS * Q_BYTES + STAGES * STAGE + SMALL;
+constexpr int SMEM = Q_BYTES + STAGES * STAGE + SMALL;
+// what a thin item keeps where it has no queries (rows 16 .. 127 of their first 64 columns): weights [2][16][128] bfloat16, row maxima [2][8][16], sums [8][16]
+constexpr int THIN_P = THIN * 128, THIN_M = THIN_P + 2 * THIN * BN * 2, THIN_L = THIN_M + 2 * 8 * THIN * 4;
+static_assert(THIN_L + 8 * THIN * 4 <= BM * 128, "behind the queries of 16 rows");
 constexpr int THREADS = 128 + 256;
 // registers a thread: 168 at the launch; the groups that hold a row's 128 scores take what the other four warps leave (128 x 80 + 256 x 208 <= 384 x 168)
 constexpr int REGS_FEW = 80, REGS_MANY = 208;
 static_assert(128 * REGS_FEW + 256 * REGS_MANY <= THREADS * 168, "a split of what the launch has");
-constexpr int S_COL = 256;
+constexpr int S_COL = BUFS == 3 ? 128 : 256;
 constexpr float SLACK = 8.0f;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr uint32_t IDESC_S = umma_idesc(BM, BN, false, false), IDESC_PV = umma_idesc(BM, VW, false, true);
-enum { GAVE_UP_LOAD = 31, GAVE_UP_MMA = 32, GAVE_UP_SOFTMAX = 33 };
+enum { GAVE_UP_LOAD = 31, GAVE_UP_MMA = 32, GAVE_UP_SOFTMAX = 33, GAVE_UP_QUERIES = 34, NOT_ALIGNED = 35 };
 
 __device__ __forceinline__ float fast_exp2(float x) {       // ex2.approx: 2 ulp, exp2(-inf) = 0
     float y;
@@ -86,6 +93,38 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 __device__ __forceinline__ void store8(float* to, const uint32_t* v) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
+// Products with their operands' descriptors in two halves: the upper one is a constant, an offset is added to the lower one (addresses of shared memory stay below 2^18, so no carry leaves the
+// field).  A K-major tile of 128-byte rows, and an MN-major one whose 64-column blocks lie `block` bytes apart, both in groups of eight rows of 1,024 bytes (tc_common.cuh).
+constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return ((addr >> 4) & 0x3FFF) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_lo_mn(uint32_t addr, uint32_t block) { return ((addr >> 4) & 0x3FFF) | ((block >> 4) << 16); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(DESC_HI) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d), "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(DESC_HI) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm2t(uint32_t addr, uint32_t& a, uint32_t& b) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the 256 threads of the groups: true if all of them say so
+__device__ __forceinline__ bool all_of_groups(bool ok) {
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\tbar.red.and.pred b, 1, 256, a;\n\tselp.u32 %0, 1, 0, b;\n\t}" : "=r"(all) : "r"(ok ? 1u : 0u) : "memory");
+    return all != 0;
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     const int n = valid ? 16 : 0;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(n));
@@ -101,37 +140,55 @@ struct Prefix {
     const int *plan, *items, *tokens;
     int n_items;                         // -1: the plan's header says (a captured step)
     long long rows;                      // results of a kv head
-    float *part_o, *part_ml;             // [kv heads][rows][VD], [kv heads][rows][2]
+    float *part_o, *part_ml;             // [kv heads][VD / 8][rows][8] (a warp's rows of eight columns are whole lines), [kv heads][rows][2]
     int* status;
 };
 
+struct Item { int token, tokens, lo, hi, request, own, row, first; };      // first: the batch's token that it begins with, if the others follow it one by one (else -1)
+
+// Rows r0 .. r0 + 31 (those below `end`) of an item into shared memory, by one warp: queries, positions.
+__device__ __forceinline__ void load_rows(const Prefix& p, const Item& item, int g, int rep, int r0, int end, uint32_t q_s, int* at_of) {
+    const int lane = threadIdx.x & 31, r = r0 + lane;
+    int src = 0;                                                 // in steps of 8 elements
+    if (r < end) {
+        const int2* t = reinterpret_cast<const int2*>(p.tokens) + item.token + r / rep;
+        const int token = item.first >= 0 ? item.first + r / rep : t->x;
+        src = token * (p.q_stride / 8) + (g * rep + r % rep) * (HD / 8);
+        at_of[r] = t->y;
+    }
+    constexpr int CH = HDP / 8;                                  // 16-byte pieces of a row: 8 to 32
+    const int n = min(32, end - r0);
+    for (int i = lane; i - lane < n * CH; i += 32) {
+        const int j = i / CH, chunk = i % CH, at = __shfl_sync(0xffffffffu, src, j & 31), rr = r0 + j;
+        if (j < n)
+            cp_async16(q_s + (chunk >> 3) * (BM * 128) + rr * 128 + (((chunk ^ rr) & 7) << 4), p.q + (chunk < HD / 8 ? (size_t)(at + chunk) * 8 : 0), chunk < HD / 8);
+    }
+}
+
 __global__ void __launch_bounds__(THREADS, 1)
 prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
-    extern __shared__ unsigned char smem_raw[];
-    pdl_begin();
+    extern __shared__ __align__(1024) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
-    const uint32_t q_s = base, ring = q_s + GROUPS * Q_BYTES, rows_s = ring + STAGES * STAGE, bars = rows_s + ROWS * 8 + BM * 4;
-    // by score buffer: s_full, p_full, pv_done; by group and warp of it: its maxima are there
-    const uint32_t full = bars, empty = full + 8 * STAGES, s_full = empty + 8 * STAGES, p_full = s_full + 16, pv_done = p_full + 16, q_full = pv_done + 16, edge_full = q_full + 8,
-                   m_ready = edge_full + 8, tmem_slot = m_ready + 64;
-    unsigned char* smem = smem_raw + (base - smem_addr(smem_raw));
-    struct Row { int src, at; };                             // a row's place in q (in steps of 8 elements), its position
-    Row* row_of = reinterpret_cast<Row*>(smem + (rows_s - base));
-    // an item's rows are looked up at its beginning; at its end the second group leaves its maximum and sum of a row in the row's place
-    volatile float* second = reinterpret_cast<volatile float*>(row_of);
-    volatile float* m_of = reinterpret_cast<volatile float*>(row_of + ROWS);
+    const uint32_t base = smem_addr(smem);
+    const uint32_t q_s = base, ring = q_s + Q_BYTES, small = ring + STAGES * STAGE, bars = small + 5 * BM * 4;
+    // by score buffer: s_full, p_full, pv_done; by group and warp of it: its maxima are there.  What the tensor core or else the groups' eight warps hand back (stages, queries) counts
+    // eight arrivals: the products' thread makes seven of them itself and leaves the last to the products' end.
+    const uint32_t full = bars, empty = full + 8 * STAGES, s_full = empty + 8 * STAGES, p_full = s_full + 8 * BUFS, pv_done = p_full + 8 * BUFS, q_full = pv_done + 8 * BUFS,
+                   q_empty = q_full + 8, begun = q_empty + 8, o_free = begun + 8, edge_full = o_free + 8, m_ready = edge_full + 8, tmem_slot = m_ready + 64;
+    int* at_of = reinterpret_cast<int*>(smem + (small - base));                   // [2][128] positions of an item's rows, items in turn
+    volatile float* m_of = reinterpret_cast<volatile float*>(at_of + 2 * BM);     // [128]
+    volatile float* l_of = m_of + BM;                                             // [2][128] the second group's sums, items in turn
     volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
-
-    const int total = (p.n_items >= 0 ? p.n_items : p.plan[PLAN_ITEMS]) * p.nkv;
-    const int rep = p.nq / p.nkv, page_shift = 31 - __clz(p.page_size);
-    // the CTA's kth pair; the last one lies past the end
-    auto pair_at = [&](int k) { return k * (int)gridDim.x + ((k & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x); };
+    if (base & 1023) {                   // (tiles of swizzled rows begin at multiples of 1,024 bytes)
+        if (threadIdx.x == 0) atomicExch(p.status, NOT_ALIGNED);
+        return;
+    }
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(s_full + 8 * b, 1); mbar_init(p_full + 8 * b, 4); mbar_init(pv_done + 8 * b, 1); }
-        mbar_init(q_full, 8);
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 8); }
+        for (int b = 0; b < BUFS; ++b) { mbar_init(s_full + 8 * b, 1); mbar_init(p_full + 8 * b, 4); mbar_init(pv_done + 8 * b, 1); }
+        mbar_init(q_full, 2); mbar_init(q_empty, 8);
+        mbar_init(begun, 8); mbar_init(o_free, 8);
         mbar_init(edge_full, 1);
         for (int i = 0; i < 8; ++i) mbar_init(m_ready + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -142,185 +199,351 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot_ptr;
+    pdl_wait();                          // the kernel behind this one may start when its CTAs leave: earlier, the merge's would crowd on the SMs that this launch leaves free
+
+    const int total = (p.n_items >= 0 ? p.n_items : p.plan[PLAN_ITEMS]) * p.nkv;
+    const int rep = p.nq / p.nkv, page_shift = 31 - __clz(p.page_size);
+    // the CTA's kth pair, to and fro
+    auto pair_at = [&](int k) { return k * (int)gridDim.x + ((k & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x); };
+    auto item_of = [&](int it) {
+        const int4* at = reinterpret_cast<const int4*>(p.items) + (it < total ? it : 0) / p.nkv * 2;
+        const int4 a = at[0], b = at[1];
+        return Item{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    };
 
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
-    if (warp == 0) {
-        // ---------------- keys and values ----------------
-        const int box_rows = p.page_size < BN ? p.page_size : BN;
-        bool ok = true;
-        int fill = 0, edges = 0;
-        auto load = [&](const int* table, int g, int key0, int key_hi, bool value) {
-            const int width = value ? VW : KW, chunks = value ? VC : KC;
-            const int held = min(BN, key_hi - key0), copied = (held + box_rows - 1) / box_rows * box_rows;      // rows of keys, rows that are copied
-            const bool edge = value && held < BN;
-            // this lane's box (pages of 16 or more: at most eight of a tile)
-            int row0 = 0;
-            if (lane * box_rows < copied) {
-                const int key = key0 + lane * box_rows, index = key >> page_shift;
-                int page = index < p.max_pages ? table[index] : 0;
-                if (page < 0) page = 0;
-                row0 = (page * p.nkv + g) * p.page_size + (key & (p.page_size - 1));
-            }
-            for (int c = 0; c < chunks; ++c) {
-                const int s = fill % STAGES;
-                if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ((fill / STAGES) & 1) ^ 1))) { ok = false; return; }
-                const uint32_t dst = ring + s * STAGE;
-                // values that reach past the item's last key land on a barrier of their own, are cleared there, and are announced then
-                const uint32_t bar = edge ? edge_full : full + 8 * s;
-                if (lane == 0) mbar_expect_tx(bar, copied * width * 2);
-                __syncwarp();
-                if (lane * box_rows < copied)
-                    for (int cb = 0; cb < width / 64; ++cb)
-                        tma_load_2d(dst + cb * (BN * 128) + lane * box_rows * 128, value ? &v_map : &k_map, bar, c * width + cb * 64, row0);
-                if (edge) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(edge_full, edges & 1))) { ok = false; return; }
-                    ++edges;
-                    for (int i = lane; i < (BN - held) * (VW / 8); i += 32) {
-                        const int row = held + i / (VW / 8), rest = i % (VW / 8);
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + (rest >> 3) * (BN * 128) + row * 128 + (rest & 7) * 16), "r"(0u) : "memory");
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full + 8 * s);
-                }
-                ++fill;
-            }
-        };
-        for (int k = 0, it; ok && (it = pair_at(k)) < total; ++k) {
-            const int* item = p.items + (it / p.nkv) * PLAN_ITEM;
-            const int g = it % p.nkv, lo = item[ITEM_KEY_LO], hi = item[ITEM_KEY_HI], T = (hi - lo + BN - 1) / BN;
-            const bool two = item[ITEM_TOKENS] * rep > BM;
-            const int* table = p.block_table + (size_t)item[ITEM_REQUEST] * p.max_pages;
-            const int ahead = two ? 1 : 2;                       // keys are asked for that many tiles before the values
-            for (int n = 0; n < ahead && n < T && ok; ++n) load(table, g, lo + n * BN, hi, false);
-            for (int n = 0; n < T && ok; ++n) {
-                load(table, g, lo + n * BN, hi, true);
-                if (ok && n + ahead < T) load(table, g, lo + (n + ahead) * BN, hi, false);
-            }
-        }
-        for (int k = 0; k < STAGES && ok; ++k, ++fill)           // nothing in flight at the exit
-            if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * (fill % STAGES), ((fill / STAGES) & 1) ^ 1))) ok = false;
-        if (!ok) {
-            for (int k = fill > STAGES ? fill - STAGES : 0; k < fill; ++k) mbar_wait(full + 8 * (k % STAGES), (k / STAGES) & 1);
-            if (lane == 0) atomicExch(p.status, GAVE_UP_LOAD);
-        }
-        __syncwarp();
-    } else if (warp == 1) {
-        // ---------------- products ----------------
-        if (lane == 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
+        if (warp == 0) {
+            // ---------------- keys and values ----------------
+            const int box_rows = p.page_size < BN ? p.page_size : BN, boxes = BN / box_rows, box_shift = 31 - __clz(box_rows);      // boxes of a tile: one to eight
             bool ok = true;
-            int use = 0, done = 0;                               // stages used, items
-            int turn[2] = {0, 0};                                // uses of the score buffers
-            // S = Q K^T of rows `rows_at` with the tile whose first stage is `at`, into buffer b; `last`: the stages are free behind it
-            auto scores = [&](int at, int group, int b, bool wait, bool last) -> bool {
-                for (int c = 0; c < KC; ++c) {
-                    const int s = (at + c) % STAGES;
-                    if (wait && !mbar_wait(full + 8 * s, ((at + c) / STAGES) & 1)) return false;
-                    tc_fence_after();
-                    const uint32_t kb = ring + s * STAGE, qb = q_s + group * Q_BYTES;
-                    const int steps = min(KW, HD - c * KW + 15) / 16;          // (columns behind the head's are zeros)
-                    for (int k = 0; k < steps; ++k) {
-                        const int col = c * (KW / 64) + (k >> 2);
-                        tc_mma(tmem + S_COL + b * BN, smem_desc(qb + col * (BM * 128) + (k & 3) * 32), smem_desc(kb + (k >> 2) * (BN * 128) + (k & 3) * 32), IDESC_S, c > 0 || k > 0 ? 1u : 0u);
+            int fill = 0, edges = 0;
+            Item next = item_of(pair_at(0));
+            for (int k = 0, it; ok && (it = pair_at(k)) < total; ++k) {
+                const Item item = next;
+                next = item_of(pair_at(k + 1));
+                const int g = it % p.nkv, lo = item.lo, hi = item.hi, T = (hi - lo + BN - 1) / BN;
+                const int* table = p.block_table + (size_t)item.request * p.max_pages;
+                // this lane's box of 32 in a row: the row of the pool that it begins with
+                auto row_of_box = [&](int window) {
+                    const int key = lo + ((window * 32 + lane) << box_shift), index = key >> page_shift;
+                    int page = key < hi && index < p.max_pages ? table[index] : 0;
+                    if (page < 0) page = 0;
+                    return (page * p.nkv + g) * p.page_size + (key & (p.page_size - 1));
+                };
+                // keys are asked for at most three tiles before the values, so these windows hold both
+                int window = 0, before = 0, now = row_of_box(0), later = row_of_box(1);
+                auto load = [&](int n, bool value) {
+                    const int width = value ? VW : KW, chunks = value ? VC : KC;
+                    const int held = min(BN, hi - lo - n * BN), copied = (held + box_rows - 1) >> box_shift;       // rows of keys; boxes that hold some
+                    const bool edge = value && held < BN;
+                    if (!value && (n * boxes) >> 5 > window) { ++window; before = now; now = later; later = row_of_box(window + 1); }
+                    const int box = n * boxes + lane;
+                    const int row = __shfl_sync(0xffffffffu, (n * boxes) >> 5 == window ? now : before, box & 31);
+                    for (int c = 0; c < chunks; ++c) {
+                        const int s = fill % STAGES;
+                        if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ((fill / STAGES) & 1) ^ 1))) { ok = false; return; }
+                        const uint32_t dst = ring + s * STAGE;
+                        // values that reach past the item's last key land on a barrier of their own, are cleared there, and are announced then
+                        const uint32_t bar = edge ? edge_full : full + 8 * s;
+                        if (lane == 0) mbar_expect_tx(bar, (copied << box_shift) * width * 2);
+                        __syncwarp();
+                        if (lane < copied)
+                            for (int cb = 0; cb < width / 64; ++cb)
+                                tma_load_2d(dst + cb * (BN * 128) + (lane << box_shift) * 128, value ? &v_map : &k_map, bar, c * width + cb * 64, row);
+                        if (edge) {
+                            if (!__all_sync(0xffffffffu, mbar_wait(edge_full, edges & 1))) { ok = false; return; }
+                            ++edges;
+                            for (int i = lane; i < (BN - held) * (VW / 8); i += 32) {
+                                const int r = held + i / (VW / 8), rest = i % (VW / 8);
+                                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + (rest >> 3) * (BN * 128) + r * 128 + (rest & 7) * 16), "r"(0u) : "memory");
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(full + 8 * s);
+                        }
+                        ++fill;
                     }
-                    if (last) tc_commit(empty + 8 * s);
+                };
+                const int ahead = item.tokens * rep <= THIN ? 1 : BUFS;
+                for (int n = 0; n < ahead && n < T && ok; ++n) load(n, false);
+                for (int n = 0; n < T && ok; ++n) {
+                    load(n, true);
+                    if (ok && n + ahead < T) load(n + ahead, false);
                 }
-                tc_commit(s_full + 8 * b);
-                return true;
-            };
-            auto output = [&](int at, int group, int b, bool first, bool wait, bool last) -> bool {
-                if (!mbar_wait(p_full + 8 * b, turn[b] & 1)) return false;
-                ++turn[b];
-                const uint32_t pa = tmem + S_COL + b * BN;
-                for (int c = 0; c < VC; ++c) {
-                    const int s = (at + c) % STAGES;
-                    if (wait && !mbar_wait(full + 8 * s, ((at + c) / STAGES) & 1)) return false;
-                    tc_fence_after();
-                    const uint32_t vb = ring + s * STAGE;
+            }
+            for (int k = 0; k < STAGES && ok; ++k, ++fill)           // nothing in flight at the exit
+                if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * (fill % STAGES), ((fill / STAGES) & 1) ^ 1))) ok = false;
+            if (!ok) {
+                for (int k = fill > STAGES ? fill - STAGES : 0; k < fill; ++k) mbar_wait(full + 8 * (k % STAGES), (k / STAGES) & 1);
+                if (lane == 0) atomicExch(p.status, GAVE_UP_LOAD);
+            }
+            __syncwarp();
+        } else if (warp == 1) {
+            // ---------------- products ----------------
+            if (lane == 0) {
+                bool ok = true;
+                int use = 0, tile = 0;                               // stages used, tiles begun before this item's
+                const uint32_t q_lo = desc_lo(q_s), k_lo = desc_lo(ring), v_lo = desc_lo_mn(ring, BN * 128);
+                auto hand_back = [&](uint32_t bar) { mbar_arrive_n(bar, 7); tc_commit(bar); };
+                auto scores = [&](int t) -> bool {                   // S = Q K^T of tile t (counted over all items) into its buffer
+                    const uint32_t d = tmem + S_COL + t % BUFS * BN;
 #pragma unroll
-                    for (int k = 0; k < BN / 16; ++k)
-                        tc_mma_ts(tmem + group * VDP + c * VW, pa + k * 8, smem_desc_mn(vb + k * (16 * 128), BN * 128), IDESC_PV, first && k == 0 ? 0u : 1u);
-                    if (last) tc_commit(empty + 8 * s);
-                }
-                tc_commit(pv_done + 8 * b);
-                return true;
-            };
-            for (int k = 0, it; ok && (it = pair_at(k)) < total; ++k, ++done) {
-                const int* item = p.items + (it / p.nkv) * PLAN_ITEM;
-                const int T = (item[ITEM_KEY_HI] - item[ITEM_KEY_LO] + BN - 1) / BN;
-                if (!mbar_wait(q_full, done & 1)) { ok = false; break; }
-                tc_fence_after();
-                if (GROUPS == 2 && item[ITEM_TOKENS] * rep > BM) {
-                    // both groups' rows against each tile: K 0, V 0, K 1, V 1, ...
-                    ok = scores(use, 0, 0, true, false) && scores(use, 1, 1, false, true);
-                    use += KC;
-                    for (int n = 0; n < T && ok; ++n) {
-                        const int v = use, next = use + VC;
-                        ok = output(v, 0, 0, n == 0, true, false);
-                        if (ok && n + 1 < T) ok = scores(next, 0, 0, true, false);
-                        ok = ok && output(v, 1, 1, n == 0, false, true);
-                        if (ok && n + 1 < T) ok = scores(next, 1, 1, false, true);
-                        use += VC + (n + 1 < T ? KC : 0);
+                    for (int c = 0; c < KC; ++c, ++use) {
+                        const int s = use % STAGES;
+                        if (!mbar_wait(full + 8 * s, (use / STAGES) & 1)) return false;
+                        tc_fence_after();
+                        const uint32_t kb = k_lo + s * (STAGE >> 4);
+#pragma unroll
+                        for (int i = 0; i < KW / 16; ++i) {
+                            if (c * KW + i * 16 >= HD) continue;     // (columns behind the head's are zeros)
+                            const int col = c * (KW / 64) + (i >> 2);
+                            mma_ss(d, q_lo + ((col * (BM * 128) + (i & 3) * 32) >> 4), kb + (((i >> 2) * (BN * 128) + (i & 3) * 32) >> 4), IDESC_S, c > 0 || i > 0 ? 1u : 0u);
+                        }
+                        hand_back(empty + 8 * s);
                     }
-                } else {
-                    // tiles in turn: K 0, K 1, V 0, K 2, V 1, ...
-                    for (int n = 0; n < 2 && n < T && ok; ++n, use += KC) ok = scores(use, 0, n, true, true);
+                    tc_commit(s_full + 8 * (t % BUFS));
+                    return true;
+                };
+                auto output = [&](int t, bool first) -> bool {       // O += P V
+                    if (!mbar_wait(p_full + 8 * (t % BUFS), (t / BUFS) & 1)) return false;
+                    const uint32_t pa = tmem + S_COL + t % BUFS * BN;
+#pragma unroll
+                    for (int c = 0; c < VC; ++c, ++use) {
+                        const int s = use % STAGES;
+                        if (!mbar_wait(full + 8 * s, (use / STAGES) & 1)) return false;
+                        tc_fence_after();
+                        const uint32_t vb = v_lo + s * (STAGE >> 4), d = tmem + c * VW;
+#pragma unroll
+                        for (int i = 0; i < BN / 16; ++i) mma_ts(d, pa + i * 8, vb + ((i * (16 * 128)) >> 4), IDESC_PV, first && i == 0 ? 0u : 1u);
+                        hand_back(empty + 8 * s);
+                    }
+                    tc_commit(pv_done + 8 * (t % BUFS));
+                    return true;
+                };
+                Item next = item_of(pair_at(0));
+                for (int k = 0; ok && pair_at(k) < total; ++k) {
+                    const Item item = next;
+                    next = item_of(pair_at(k + 1));
+                    const int T = (item.hi - item.lo + BN - 1) / BN;
+                    if (!mbar_wait(q_full, k & 1)) { ok = false; break; }
+                    if (item.tokens * rep <= THIN) {
+                        use += T * (KC + VC);
+                        if (k > 0 && !mbar_wait(o_free, (k - 1) & 1)) ok = false;
+                        continue;
+                    }
+                    tc_fence_after();
+                    // K 0, K 1, (K 2,) V 0, K 2 (3), V 1, ...
+                    for (int n = 0; n < BUFS && n < T && ok; ++n) ok = scores(tile + n);
+                    if (T <= BUFS) hand_back(q_empty);
+                    // the first product with the values waits until the groups have read the outputs of the item before
+                    if (ok && k > 0) ok = mbar_wait(o_free, (k - 1) & 1);
+                    tc_fence_after();
                     for (int n = 0; n < T && ok; ++n) {
-                        ok = output(use, 0, n & 1, n == 0, true, true);
-                        use += VC;
-                        if (ok && n + 2 < T) {
-                            ok = scores(use, 0, n & 1, true, true);
-                            use += KC;
+                        ok = output(tile + n, n == 0);
+                        if (ok && n + BUFS < T) {
+                            ok = scores(tile + n + BUFS);
+                            if (n + BUFS + 1 == T) hand_back(q_empty);
                         }
                     }
+                    tile += T;
                 }
+                if (!ok) atomicExch(p.status, GAVE_UP_MMA);
             }
-            if (!ok) atomicExch(p.status, GAVE_UP_MMA);
+        } else {
+            // ---------------- queries: a warp takes every other 32 rows (of the first item the groups take them) ----------------
+            bool ok = true;
+            Item next = item_of(pair_at(1));
+            for (int k = 1, it; (it = pair_at(k)) < total; ++k) {
+                const Item item = next;
+                next = item_of(pair_at(k + 1));
+                const int rows = item.tokens * rep;
+                // where they go: the products of the item before have read the queries, its rows' positions of two items ago have been looked up
+                if (!__all_sync(0xffffffffu, mbar_wait(q_empty, (k - 1) & 1) && mbar_wait(begun, (k - 1) & 1))) { ok = false; break; }
+                for (int r0 = (warp - 2) * 32; r0 < rows; r0 += 64) load_rows(p, item, it % p.nkv, rep, r0, rows, q_s, at_of + (k & 1) * BM);
+                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+            }
+            if (!ok && lane == 0) atomicExch(p.status, GAVE_UP_QUERIES);
+            __syncwarp();
         }
-    }
     } else {
         // ---------------- softmax: a thread per row ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
-        const int group = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, tid = threadIdx.x - 128;
-        const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16), scores_at = t_lane + S_COL + group * BN;
+        const int group = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t mine_ready = m_ready + 8 * (group * 4 + quarter), other_ready = m_ready + 8 * ((group ^ 1) * 4 + quarter);
         const float sc = (p.capl > 0.f || p.slopes != nullptr) ? 1.0f : p.scale2;        // capped and biased scores are in powers of two already
         const float pre = p.capl > 0.f ? 1.0f : p.scale2;
         const float cap_in = p.capl > 0.f ? 2.0f * p.scale2 / p.capl : 0.f;
         bool ok = true;
-        int turn = 0, other_turn = 0, other_handed = 0;          // uses of this group's score buffer, of the other's, maxima that the other has handed over, before this item
-        for (int k = 0, it; (it = pair_at(k)) < total; ++k) {
-            const int* item = p.items + (it / p.nkv) * PLAN_ITEM;
-            const int g = it % p.nkv, lo = item[ITEM_KEY_LO], hi = item[ITEM_KEY_HI], T = (hi - lo + BN - 1) / BN, rows = item[ITEM_TOKENS] * rep;
-            const bool own = item[ITEM_OWN] != 0, two = rows > BM;
-            const int m_row = two ? group * BM + row : row;
-            const bool live = m_row < rows, warp_live = m_row - lane < rows;
-            if (m_row < rows && (two || group == 0)) {
-                const int* t = p.tokens + 2 * (item[ITEM_TOKEN] + m_row / rep);
-                row_of[m_row] = Row{t[0] * (p.q_stride / 8) + (g * rep + m_row % rep) * (HD / 8), t[1]};
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            for (int i = tid; i < rows * (HDP / 8); i += 256) {
-                const int r = i / (HDP / 8), chunk = i % (HDP / 8);
-                cp_async16(q_s + (r >> 7) * Q_BYTES + (chunk >> 3) * (BM * 128) + (r & 127) * 128 + (((chunk ^ r) & 7) << 4), p.q + (chunk < HD / 8 ? (size_t)(row_of[r].src + chunk) * 8 : 0),
-                           chunk < HD / 8);
-            }
+        int use = 0, tile = 0, other_handed = 0;                 // stages used, tiles, maxima that the other group has handed over, before this item
+        Item next = item_of(pair_at(0));
+        if ((int)blockIdx.x < total) {                           // the first item's queries: nobody else has anything to do yet
+            const int end = min((warp - 3) * 16, next.tokens * rep);
+            if ((warp - 4) * 16 < end) load_rows(p, next, (int)blockIdx.x % p.nkv, rep, (warp - 4) * 16, end, q_s, at_of);
             asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            const int pos = live ? row_of[m_row].at : 0;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (warp < 6 && lane == 0) mbar_arrive(q_full);
+        }
+        for (int k = 0, it; (it = pair_at(k)) < total; ++k) {
+            const Item item = next;
+            next = item_of(pair_at(k + 1));
+            const int g = it % p.nkv, lo = item.lo, hi = item.hi, T = (hi - lo + BN - 1) / BN, rows = item.tokens * rep;
+            if (!__all_sync(0xffffffffu, mbar_wait(q_full, k & 1))) ok = false;
+            if (rows <= THIN) {
+                // ---- up to 16 rows: mma.sync; this thread holds parts of rows lane / 4 and lane / 4 + 8 ----
+                const int w = warp - 4;
+                constexpr int NT = VDP / 64;                     // this warp's blocks of 8 value columns: w * NT ...
+                float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope2[2];
+                int last[2], pos[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = (lane >> 2) + 8 * i;
+                    pos[i] = r < rows ? at_of[(k & 1) * BM + r] : 0;
+                    last[i] = r >= rows ? -1 : item.own ? min(pos[i], hi - 1) : hi - 1;
+                    slope2[i] = (p.slopes != nullptr && r < rows) ? p.slopes[g * rep + r % rep] * LOG2E : 0.f;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(begun);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+                volatile float* mx_all = reinterpret_cast<volatile float*>(smem + THIN_M);
+                volatile float* l_all = reinterpret_cast<volatile float*>(smem + THIN_L);
+                for (int n = 0; n < T; ++n) {
+                    const int key0 = lo + n * BN;
+                    // scores of this warp's 16 keys
+                    float sv[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                    const int a_row = lane & 15, a_chunk = lane >> 4, b_row = w * 16 + (lane & 7) + (lane >> 4) * 8, b_chunk = (lane >> 3) & 1;
+#pragma unroll
+                    for (int c = 0; c < KC; ++c, ++use) {
+                        const int s = use % STAGES;
+                        if (ok && !__all_sync(0xffffffffu, mbar_wait(full + 8 * s, (use / STAGES) & 1))) ok = false;
+                        const uint32_t kb = ring + s * STAGE;
+#pragma unroll
+                        for (int i = 0; i < KW / 16; ++i) {
+                            if (c * KW + i * 16 >= HD) continue;
+                            uint32_t a[4], b[4];
+                            const int qa = c * (KW / 8) + i * 2 + a_chunk, ka = i * 2 + b_chunk;
+                            ldsm4(q_s + (qa >> 3) * (BM * 128) + a_row * 128 + (((qa ^ a_row) & 7) << 4), a);
+                            ldsm4(kb + (ka >> 3) * (BN * 128) + b_row * 128 + (((ka ^ b_row) & 7) << 4), b);
+                            mma16816(sv[0], a, b[0], b[1]);
+                            mma16816(sv[1], a, b[2], b[3]);
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(empty + 8 * s);
+                    }
+                    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = e >> 1, key = key0 + w * 16 + j * 8 + (lane & 3) * 2 + (e & 1);
+                            float x = sv[j][e];
+                            if (p.capl > 0.f) x = p.capl * (1.0f - __fdividef(2.0f, 1.0f + __expf(x * cap_in)));
+                            else x *= p.scale2;
+                            if (p.slopes != nullptr) x = fmaf(-slope2[i], (float)(pos[i] - key), x);
+                            sv[j][e] = key <= last[i] ? x : -INFINITY;
+                            mx[i] = fmaxf(mx[i], sv[j][e]);
+                        }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+                        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+                        if ((lane & 3) == 0) mx_all[((n & 1) * 8 + w) * THIN + (lane >> 2) + 8 * i] = mx[i];
+                    }
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    const uint32_t p_s = q_s + THIN_P + (n & 1) * (THIN * BN * 2);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int r = (lane >> 2) + 8 * i;
+                        float top = m[i];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) top = fmaxf(top, mx_all[((n & 1) * 8 + j) * THIN + r]);
+                        const float base_now = top == -INFINITY ? 0.f : top, corr = exp2f(m[i] - base_now);
+                        m[i] = top;
+                        l[i] *= corr;
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) { o[j][2 * i] *= corr; o[j][2 * i + 1] *= corr; }
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float e0 = exp2f(sv[j][2 * i] - base_now), e1 = exp2f(sv[j][2 * i + 1] - base_now);
+                            l[i] += e0 + e1;
+                            const int chunk = w * 2 + j;         // eight keys
+                            asm volatile("st.shared.b32 [%0], %1;" ::"r"(p_s + r * (BN * 2) + ((chunk ^ (r & 7)) << 4) + (lane & 3) * 4), "r"(pack_bf16(e0, e1)) : "memory");
+                        }
+                    }
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    // this warp's columns of the output
+                    uint32_t a[BN / 16][4];
+#pragma unroll
+                    for (int i = 0; i < BN / 16; ++i) ldsm4(p_s + a_row * (BN * 2) + (((i * 2 + a_chunk) ^ (a_row & 7)) << 4), a[i]);
+#pragma unroll
+                    for (int c = 0; c < VC; ++c, ++use) {
+                        const int s = use % STAGES;
+                        if (ok && !__all_sync(0xffffffffu, mbar_wait(full + 8 * s, (use / STAGES) & 1))) ok = false;
+                        const uint32_t vb = ring + s * STAGE;
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            const int col = w * NT + j - c * (VW / 8);       // the block's place in this chunk
+                            if (col < 0 || col >= VW / 8) continue;
+#pragma unroll
+                            for (int i = 0; i < BN / 16; ++i) {
+                                uint32_t b0, b1;
+                                const int key = i * 16 + (lane & 15);
+                                ldsm2t(vb + (col >> 3) * (BN * 128) + key * 128 + (((col ^ key) & 7) << 4), b0, b1);
+                                mma16816(o[j], a[i], b0, b1);
+                            }
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(empty + 8 * s);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+                    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+                    if ((lane & 3) == 0) l_all[w * THIN + (lane >> 2) + 8 * i] = l[i];
+                }
+                if (!all_of_groups(ok)) {
+                    if (!ok) atomicExch(p.status, GAVE_UP_SOFTMAX);
+                    break;
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = (lane >> 2) + 8 * i;
+                    if (w == 0 && (lane & 3) == 0 && r < rows) {
+                        float sum = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) sum += l_all[j * THIN + r];
+                        *reinterpret_cast<float2*>(p.part_ml + ((size_t)g * p.rows + item.row + r) * 2) = make_float2(m[i], sum);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const int col = w * NT + j;
+                        if (r < rows && col < VD / 8)
+                            *reinterpret_cast<float2*>(p.part_o + (((size_t)g * (VD / 8) + col) * p.rows + item.row + r) * 8 + (lane & 3) * 2) = make_float2(o[j][2 * i], o[j][2 * i + 1]);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(q_empty); mbar_arrive(o_free); }
+                continue;
+            }
+            const bool live = row < rows, warp_live = row - lane < rows;
+            const int pos = live ? at_of[(k & 1) * BM + row] : 0;
             __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-            asm volatile("bar.sync 1, 256;" ::: "memory");                 // nobody looks a row up any more: `second` may be written
-            const int last = own ? min(pos, hi - 1) : hi - 1;              // the last key that the row sees
-            const float slope2 = (p.slopes != nullptr && live) ? p.slopes[g * rep + m_row % rep] * LOG2E : 0.f;
-            const uint32_t o_at = t_lane + (two ? group * VDP : 0);
+            if (lane == 0) mbar_arrive(begun);
+            const int last = item.own ? min(pos, hi - 1) : hi - 1;         // the last key that the row sees
+            const float slope2 = (p.slopes != nullptr && live) ? p.slopes[g * rep + row % rep] * LOG2E : 0.f;
             float m_run = -INFINITY, l_run = 0.f;                          // m_run: what l_run is relative to
-            for (int n = two ? 0 : group; n < T; n += two ? 1 : 2, ++turn) {
-                const int key0 = lo + n * BN;
-                if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * group, turn & 1))) { ok = false; break; }
-                // tiles in turn: the maxima up to tile n - 1 are the other group's; its P V comes before this one's
-                const bool behind = !two && n > 0;
+            for (int n = group; ok && n < T; n += 2) {
+                const int key0 = lo + n * BN, t = tile + n;
+                const uint32_t scores_at = t_lane + S_COL + t % BUFS * BN;
+                if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * (t % BUFS), (t / BUFS) & 1))) { ok = false; break; }
+                // (the maxima up to tile n - 1 are the other group's; its P V comes before this one's)
                 float corr = 1.f;
                 bool changed = false;
                 if (warp_live) {
@@ -347,18 +570,16 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
 #pragma unroll
                     for (int c = 0; c < BN; c += 2) mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(sv[c >> 5][c & 31]), __uint_as_float(sv[c >> 5][(c & 31) + 1]));
                     const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                    float m_before = m_run;
-                    if (behind) {
+                    float m_before = -INFINITY;
+                    if (n > 0) {
                         if (!__all_sync(0xffffffffu, mbar_wait(other_ready, (other_handed + (n - 1) / 2) & 1))) { ok = false; break; }
                         m_before = m_of[row];
                     }
                     const float m_tile = fmaxf(m_before, mx * sc);
                     const float m_new = m_tile > m_before + SLACK ? m_tile : m_before;     // m_before = -inf: takes m_tile
-                    if (!two) {
-                        m_of[row] = m_new;
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(mine_ready);
-                    }
+                    m_of[row] = m_new;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(mine_ready);
                     const float mbase = m_new == -INFINITY ? 0.f : m_new;
                     corr = fast_exp2(m_before - mbase);
                     l_run *= fast_exp2(m_run - mbase);
@@ -384,63 +605,65 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                 }
                 // O holds the products of all tiles before this one: it is scaled when they are complete
                 if (n > 0 && __any_sync(0xffffffffu, changed)) {
-                    const bool there = two ? mbar_wait(pv_done + 8 * group, (turn - 1) & 1) : mbar_wait(pv_done + 8 * (group ^ 1), (other_turn + (n - 1) / 2) & 1);
-                    if (!__all_sync(0xffffffffu, there)) { ok = false; break; }
+                    if (!__all_sync(0xffffffffu, mbar_wait(pv_done + 8 * ((t - 1) % BUFS), ((t - 1) / BUFS) & 1))) { ok = false; break; }
                     tc_fence_after();
 #pragma unroll 1
                     for (int c0 = 0; c0 < VDP; c0 += 32) {
                         uint32_t ov[32];
-                        tc_ld32(o_at + c0, ov);
+                        tc_ld32(t_lane + c0, ov);
                         tc_wait_ld();
 #pragma unroll
                         for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * corr);
-                        tc_st32(o_at + c0, ov);
+                        tc_st32(t_lane + c0, ov);
                     }
                 }
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * group);
+                if (lane == 0) mbar_arrive(p_full + 8 * (t % BUFS));
             }
             // the last product of the item (every one before it is complete then), by the group that it belongs to
-            if (ok && (two || ((T - 1) & 1) == group) && !__all_sync(0xffffffffu, mbar_wait(pv_done + 8 * group, (turn - 1) & 1))) ok = false;
-            const int others = two ? T : group == 0 ? T / 2 : (T + 1) / 2;
-            other_turn += others;
-            if (!two && warp_live) other_handed += others;
-            if (!two && group == 1) { second[2 * row] = m_run; second[2 * row + 1] = l_run; }
-            uint32_t all;                                // they go on or give up together
-            asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\tbar.red.and.pred b, 1, 256, a;\n\tselp.u32 %0, 1, 0, b;\n\t}" : "=r"(all) : "r"(ok ? 1u : 0u) : "memory");
-            if (!all) {
+            const int end = tile + T - 1;
+            const bool ends = ((T - 1) & 1) == group;
+            if (ok && ends && !__all_sync(0xffffffffu, mbar_wait(pv_done + 8 * (end % BUFS), (end / BUFS) & 1))) ok = false;
+            if (group == 1) {                            // the second group's sum, relative to the last maximum
+                float m = m_run;
+                if (ok && !ends && warp_live) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(other_ready, (other_handed + (T - 1) / 2) & 1))) ok = false;
+                    m = m_of[row];
+                }
+                l_of[(k & 1) * BM + row] = l_run * fast_exp2(m_run - (m == -INFINITY ? 0.f : m));
+            }
+            tile += T;
+            use += T * (KC + VC);
+            if (warp_live) other_handed += group == 0 ? T / 2 : (T + 1) / 2;
+            if (!all_of_groups(ok)) {                    // they go on or give up together
                 if (!ok) atomicExch(p.status, GAVE_UP_SOFTMAX);
                 break;
             }
             if (warp_live) {
                 tc_fence_after();
-                const size_t at = (size_t)g * p.rows + item[ITEM_ROW] + m_row;
-                if (live && (two || group == 0)) {
-                    float m = m_run, l = l_run;
-                    if (!two) {
-                        m = m_of[row];
-                        const float mbase = m == -INFINITY ? 0.f : m;
-                        l = l_run * fast_exp2(m_run - mbase) + second[2 * row + 1] * fast_exp2(second[2 * row] - mbase);
-                    }
-                    *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l);
+                const size_t at = (size_t)item.row + row;
+                if (live && group == 0) {
+                    const float m = m_of[row], l = l_run * fast_exp2(m_run - (m == -INFINITY ? 0.f : m)) + l_of[(k & 1) * BM + row];
+                    *reinterpret_cast<float2*>(p.part_ml + ((size_t)g * p.rows + at) * 2) = make_float2(m, l);
                 }
-                // of an item of up to 128 rows each group stores half the columns
+                // each group stores half the columns
                 constexpr int HALF = (VD + 63) / 64 * 32;
-                const int c_lo = two ? 0 : group * HALF, c_hi = two ? VD : min(VD, c_lo + HALF);
 #pragma unroll 1
-                for (int c0 = c_lo; c0 < c_hi; c0 += 32) {
+                for (int c0 = group * HALF; c0 < min(VD, group * HALF + HALF); c0 += 32) {
                     uint32_t ov[32];
-                    tc_ld32(o_at + c0, ov);
+                    tc_ld32(t_lane + c0, ov);
                     tc_wait_ld();
                     if (live)
 #pragma unroll
                         for (int c = 0; c < 32; c += 8)
-                            if (c0 + c < VD) store8(p.part_o + at * VD + c0 + c, ov + c);
+                            if (c0 + c < VD) store8(p.part_o + (((size_t)g * (VD / 8) + (c0 + c) / 8) * p.rows + at) * 8, ov + c);
                 }
-                tc_fence_before();                       // read before the next item's products are let loose on O (by q_full)
+                tc_fence_before();
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free);
         }
     }
     tc_fence_before();
@@ -451,54 +674,69 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
     }
 }
 
-// The merge of a token's results: grid (tokens, kv heads, groups of warps), a warp per (query head, 128 columns).  Bound by the latency of its chain of loads (starts, list, maxima and sums,
-// results) where results are few, so a unit's loads are asked for eight at a time and every unit has a warp of its own.
-constexpr int MERGE_WARPS = 4, MERGE_BLOCKS = (VD + 127) / 128;
+// The merge of a token's results: grid (tokens, kv heads, groups of warps), a warp a query head.  VD / 8 lanes take a result, 8 columns each, so as many results at once as fit a warp.  Bound
+// by the latency of its chain of loads (starts, list, maxima and sums, results) where results are few: a lane's results are asked for four at a time.
+constexpr int MERGE_WARPS = 4;
 __global__ void __launch_bounds__(MERGE_WARPS * 32)
 prefix_merge_kernel(bf16* __restrict__ out, int out_stride, const int* __restrict__ plan, int rep, long long rows, const float* __restrict__ part_o, const float* __restrict__ part_ml,
                     const float* __restrict__ sinks) {
     pdl_begin();
-    const int token = blockIdx.x, g = blockIdx.y, unit = (int)blockIdx.z * MERGE_WARPS + (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (unit >= rep * MERGE_BLOCKS) return;
+    const int token = blockIdx.x, g = blockIdx.y, h = (int)blockIdx.z * MERGE_WARPS + (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (h >= rep) return;
     const int* starts = plan + plan[PLAN_AT_STARTS];
     const int first = starts[token], n = starts[token + 1] - first;
     if (n <= 0) return;
     const int* list = plan + plan[PLAN_AT_RESULTS] + first;
-    const size_t head0 = (size_t)g * rows;
-    const int h = unit / MERGE_BLOCKS, col = (unit % MERGE_BLOCKS) * 128 + lane * 4, head = g * rep + h;
-    float M = -INFINITY, L = 0.f;
-    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int PER = VD / 8, SIDE = 32 / PER;             // lanes a result, results side by side
+    const int side = lane / PER, col = lane % PER, head = g * rep + h;
+    const float* mine_o = part_o + ((size_t)g * PER + col) * rows * 8;
+    float M = -INFINITY, L = 0.f, O[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0; i0 < n; i0 += 32) {
-        const size_t row = i0 + lane < n ? head0 + list[i0 + lane] + h : 0;
-        const float2 ml = i0 + lane < n ? *reinterpret_cast<const float2*>(part_ml + row * 2) : make_float2(-INFINITY, 0.f);
+        const size_t row = i0 + lane < n ? (size_t)list[i0 + lane] + h : 0;
+        const float2 ml = i0 + lane < n ? *reinterpret_cast<const float2*>(part_ml + ((size_t)g * rows + row) * 2) : make_float2(-INFINITY, 0.f);
         const int count = min(32, n - i0);
-        float keep = 1.f, mine = 0.f;
-        for (int u0 = 0; u0 < count; u0 += 8) {
-            float4 v[8];
+        float weight = 0.f;
+        for (int u0 = 0; u0 < count; u0 += 4 * SIDE) {
+            float4 v[4][2];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const size_t at = __shfl_sync(0xffffffffu, row, (u0 + u) & 31);
-                v[u] = u0 + u < count && col < VD ? *reinterpret_cast<const float4*>(part_o + at * VD + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int u = 0; u < 4; ++u) {
+                const int i = u0 + u * SIDE + side;
+                const size_t at = __shfl_sync(0xffffffffu, row, i & 31);
+                const bool there = side < SIDE && i < count;
+                const float4* src = reinterpret_cast<const float4*>(mine_o + at * 8);
+                v[u][0] = there ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[u][1] = there ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
             }
             if (u0 == 0) {                       // while they are on their way
                 const float M_new = fmaxf(M, warp_max(ml.x)), base = M_new == -INFINITY ? 0.f : M_new;
-                keep = exp2f(M - base);
-                mine = exp2f(ml.x - base);
-                L = L * keep + warp_sum(ml.y * mine);
-                O.x *= keep; O.y *= keep; O.z *= keep; O.w *= keep;
+                const float keep = exp2f(M - base);
+                weight = exp2f(ml.x - base);
+                L = L * keep + warp_sum(ml.y * weight);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) O[j] *= keep;
                 M = M_new;
             }
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float f = __shfl_sync(0xffffffffu, mine, (u0 + u) & 31);       // (a result past the end weighs nothing and is zero)
-                O.x += v[u].x * f; O.y += v[u].y * f; O.z += v[u].z * f; O.w += v[u].w * f;
+            for (int u = 0; u < 4; ++u) {        // (a result past the end is zero)
+                const float f = __shfl_sync(0xffffffffu, weight, (u0 + u * SIDE + side) & 31);
+                O[0] += v[u][0].x * f; O[1] += v[u][0].y * f; O[2] += v[u][0].z * f; O[3] += v[u][0].w * f;
+                O[4] += v[u][1].x * f; O[5] += v[u][1].y * f; O[6] += v[u][1].z * f; O[7] += v[u][1].w * f;
             }
         }
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float sum = O[j];
+        for (int s = 1; s < SIDE; ++s) sum += __shfl_sync(0xffffffffu, O[j], (col + s * PER) & 31);
+        O[j] = sum;
+    }
     if (sinks) L += exp2f(sinks[head] * LOG2E - (M == -INFINITY ? 0.f : M));
-    if (col < VD) {
+    if (side == 0) {
         const float inv = 1.0f / L;
-        *reinterpret_cast<uint2*>(out + (size_t)token * out_stride + (size_t)head * VD + col) = uint2{pack_bf16(O.x * inv, O.y * inv), pack_bf16(O.z * inv, O.w * inv)};
+        uint4 o{pack_bf16(O[0] * inv, O[1] * inv), pack_bf16(O[2] * inv, O[3] * inv), pack_bf16(O[4] * inv, O[5] * inv), pack_bf16(O[6] * inv, O[7] * inv)};
+        bf16* to = out + (size_t)token * out_stride + (size_t)head * VD + col * 8;
+        *reinterpret_cast<uint2*>(to) = uint2{o.x, o.y};
+        *reinterpret_cast<uint2*>(to + 4) = uint2{o.z, o.w};
     }
 }
 
@@ -529,7 +767,7 @@ static int pool_map(const void* ptr, long long rows, int box_rows, int head, CUt
 }
 
 // Rows of an item at most.
-WLLM_API int wllm_prefix_attention_rows() { return ROWS; }
+WLLM_API int wllm_prefix_attention_rows() { return BM; }
 
 // The attention of a planned batch.  pool_pages: pages of the pools; n_tokens: rows of q and out; scratch: nkv * rows * (VD + 2) floats, rows as the plan has them (or the most that a plan of
 // this array may have); items_at, tokens_at: their places in the plan; n_items: its items, or -1: its header says; pairs: (item, kv head) pairs, or the most that there may be; ctas: SMs.  sinks, slopes: 32-bit [nq] or null; cap > 0: scores become cap tanh(score / cap).
@@ -537,11 +775,11 @@ WLLM_API int wllm_prefix_attention(const void* q, int q_stride, void* out, int o
                                    int max_pages, int n_tokens, int nq, int nkv, int page_size, float scale, float cap, const float* sinks, const float* slopes, const int* plan,
                                    int items_at, int tokens_at, int n_items, float* scratch, long long rows, long long pairs, int ctas, int* status, cudaStream_t stream) {
     if (n_tokens <= 0 || pairs <= 0) return WLLM_OK;
-    if (nq <= 0 || nkv <= 0 || nq % nkv != 0 || nq / nkv > ROWS || page_size < 16 || (page_size & (page_size - 1)) || pool_pages < 1 || max_pages < 1 || nkv > 65535 || ctas < 1 ||
+    if (nq <= 0 || nkv <= 0 || nq % nkv != 0 || nq / nkv > BM || page_size < 16 || (page_size & (page_size - 1)) || pool_pages < 1 || max_pages < 1 || nkv > 65535 || ctas < 1 ||
         !(scale > 0.f) || !(cap >= 0.f) || rows < 1 || items_at < 0 || tokens_at < 0 || pool_pages * nkv > 0x7fffffffLL / page_size ||
         (long long)n_tokens * (q_stride / 8) > 0x7fffffffLL)
         return WLLM_BAD_SIZE;
-    if (q_stride % 8 != 0 || out_stride % 4 != 0 || ((uintptr_t)q & 15) || ((uintptr_t)out & 7) || ((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15) || ((uintptr_t)scratch & 15))
+    if (q_stride % 8 != 0 || out_stride % 4 != 0 || ((uintptr_t)q & 15) || ((uintptr_t)out & 7) || ((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15) || ((uintptr_t)scratch & 31) || ((uintptr_t)plan & 15) || items_at % 4 != 0 || tokens_at % 2 != 0)
         return WLLM_BAD_ALIGN;
     CUtensorMap km, vm;
     const int box = page_size < BN ? page_size : BN;
@@ -562,6 +800,6 @@ WLLM_API int wllm_prefix_attention(const void* q, int q_stride, void* out, int o
     const int st = wllm_launch(prefix_kernel, dim3((unsigned)(pairs < ctas ? pairs : ctas)), THREADS, SMEM, stream, p, km, vm);
     if (st) return st;
     const int rep = nq / nkv;
-    return wllm_launch(prefix_merge_kernel, dim3(n_tokens, nkv, (rep * MERGE_BLOCKS + MERGE_WARPS - 1) / MERGE_WARPS), MERGE_WARPS * 32, 0, stream, (bf16*)out, out_stride, plan, rep, rows,
+    return wllm_launch(prefix_merge_kernel, dim3(n_tokens, nkv, (rep + MERGE_WARPS - 1) / MERGE_WARPS), MERGE_WARPS * 32, 0, stream, (bf16*)out, out_stride, plan, rep, rows,
                        (const float*)p.part_o, (const float*)p.part_ml, sinks);
 }

@@ -3,8 +3,9 @@
 // Requests that hold the same page at the same place of their tables have the same tokens up to its end.  So the tables are walked as a tree: the requests that agree on
 // the next page stay together, and every stretch of pages on which a set of two or more agrees is one *segment*, attended to by the rows of all of them; what is left of a
 // request's keys is its own segment.  Segments are cut into items, (tile of rows) x (range of keys), one CTA each and key/value head.  How long the ranges are decides
-// between SMs without work (long ranges) and results that have to be written and merged (short ones): of a few lengths the one with the earliest estimated end is
-// taken, an item costing its tiles of keys and a tile and a half beside them.  Items are listed longest first, those that read the same keys side by side (for the L2).
+// between SMs without work (long ranges) and results that have to be written and merged (short ones): of a few bounds on what an item may cost the one with the earliest
+// estimated end is taken.  The caller says what its kernel takes for a tile of keys, for an item beside them and for a row of results.  Items are listed dearest first, those that read
+// the same keys side by side (for the L2).
 #include "common.cuh"
 #include "prefix_plan.cuh"
 
@@ -63,7 +64,7 @@ struct Planner {
 };
 
 struct Tile { int token, tokens, key_lo, key_hi, request; bool own; };
-struct Item { int tile, key_lo, key_hi, row, length; };      // length: in tiles of keys
+struct Item { int tile, key_lo, key_hi, row, cost; };
 
 long long padded(long long n) { return (n + 3) & ~3ll; }
 
@@ -71,12 +72,13 @@ long long padded(long long n) { return (n + 3) & ~3ll; }
 
 // tables [R][width] (pages that hold no key of a request are not looked at), q_len, ctx_len [R] on the host.  rep: query heads a key/value head; tile_rows: rows of an item at
 // most; key_tile: keys of a tile, whole tiles make an item's range; align: segments end at multiples of it; min_keys: no shared segment is shorter; pool_pages: one past the largest
-// page number; ctas: CTAs that run at once; caps: {items, tokens, results, tokens of the batch} that the array is laid out for, zeros: what this plan needs (a captured
+// page number; ctas: CTAs that run at once; costs: {a tile of keys, an item beside its tiles; the same two for items of at most `thin` rows; thin; a thousand rows of results and
+// kv heads}, in the caller's units; caps: {items, tokens, results, tokens of the batch} that the array is laid out for, zeros: what this plan needs (a captured
 // step's array lies at fixed places whatever the batch holds).  out [room]; info [8]: ints used, items, rows, shared keys saved (keys x further holders), most results of a
 // token, items that the batch has at the least.
 // Returns 0; 2: sizes that make no sense, or more than the caps hold; 4: `room` is too small (info[0] says what is needed); 7: a page number outside the pool.
 WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const int* q_len, const int* ctx_len, int page_size, int rep, int nkv, int tile_rows, int key_tile, int align,
-                              int min_keys, int pool_pages, int ctas, const int* caps, int* out, long long room, long long* info) {
+                              int min_keys, int pool_pages, int ctas, const int* costs, const int* caps, int* out, long long room, long long* info) {
     try {
         if (R < 0 || R > (1 << 20) || width < 0 || page_size < 1 || rep < 1 || nkv < 1 || tile_rows < rep || key_tile < 1 || align < 1 || ctas < 1 || pool_pages < 1) return WLLM_BAD_SIZE;
         Planner p{tables, width, R, page_size, align, min_keys, {}, {}, {}, {}};
@@ -128,49 +130,61 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             }
             if (tokens.size() > (1u << 28)) return WLLM_BAD_SIZE;
         }
-        // the length of the ranges
+        // what an item may cost at most: tiles by their keys, thin ones apart
         auto keys_of = [&](const Tile& t) { return (t.key_hi - t.key_lo + key_tile - 1) / key_tile; };
-        int longest = 1;
-        for (const Tile& t : tiles) longest = std::max(longest, keys_of(t));
-        std::vector<int> alike(longest + 1, 0), lengths;         // tiles by how many tiles of keys they meet
-        for (const Tile& t : tiles)
-            if (alike[keys_of(t)]++ == 0) lengths.push_back(keys_of(t));
-        std::sort(lengths.begin(), lengths.end());
-        const long long most_items = caps[0] > 0 ? caps[0] : (1 << 22);
-        const double beside = 1.5;
-        double best = 0;
-        int per = longest;
-        bool any = false;
-        for (int l = 1;; l = std::max(l + 1, l * 5 / 4)) {
-            const int len = std::min(l, longest);
-            long long n = 0, work = 0;
-            int top = 0;
-            for (int k : lengths) {
-                const int parts = (k + len - 1) / len;
-                n += (long long)parts * alike[k];
-                work += (long long)k * alike[k];
-                top = std::max(top, (k + parts - 1) / parts);
+        auto is_thin = [&](const Tile& t) { return t.tokens * rep <= costs[4] ? 1 : 0; };
+        struct Alike { int keys, thin, count; long long rows; };
+        std::vector<Alike> alike;
+        {
+            int longest = 0;
+            for (const Tile& t : tiles) longest = std::max(longest, keys_of(t));
+            std::vector<int> place(2 * (longest + 1), -1);
+            for (const Tile& t : tiles) {
+                int& at = place[2 * keys_of(t) + is_thin(t)];
+                if (at < 0) {
+                    at = (int)alike.size();
+                    alike.push_back({keys_of(t), is_thin(t), 0, 0});
+                }
+                ++alike[at].count;
+                alike[at].rows += (long long)t.tokens * rep;
             }
-            const double all = work + beside * n, end = n * nkv <= ctas ? top + beside : std::max(top + beside, all * nkv / ctas + 0.5 * (top + beside));
-            if (n <= most_items && (!any || end < best * 0.98)) {
-                best = end;
-                per = len;
-                any = true;
-            }
-            if (len == longest) break;
         }
-        if (!any) return WLLM_BAD_SIZE;
+        auto parts_of = [&](int keys, int thin, int most) { return std::min(keys, std::max(1, (int)(((long long)keys * costs[2 * thin] + most - 1) / most))); };
+        const long long most_items = caps[0] > 0 ? caps[0] : (1 << 22);
+        int dearest = 1;
+        for (const Alike& a : alike) dearest = (int)std::min<long long>(std::max<long long>(dearest, (long long)a.keys * costs[2 * a.thin]), 1 << 30);
+        double best = 0;
+        int most = 0;
+        for (long long m = std::max(1, std::min(costs[0], costs[2]));; m = m * 6 / 5 + 1) {
+            const int bound = (int)std::min<long long>(m, dearest);
+            long long n = 0, results_rows = 0;
+            double all = 0, top = 0;
+            for (const Alike& a : alike) {
+                const int parts = parts_of(a.keys, a.thin, bound);
+                n += (long long)parts * a.count;
+                results_rows += parts * a.rows;
+                all += ((double)a.keys * costs[2 * a.thin] + (double)parts * costs[2 * a.thin + 1]) * a.count;
+                top = std::max(top, (double)((a.keys + parts - 1) / parts) * costs[2 * a.thin] + costs[2 * a.thin + 1]);
+            }
+            const double end = (n * nkv <= ctas ? top : std::max(top, all * nkv / ctas + 0.5 * top)) + (double)results_rows * nkv * costs[5] / 1000;
+            if (n <= most_items && (most == 0 || end < best * 0.99)) {
+                best = end;
+                most = bound;
+            }
+            if (bound == dearest) break;
+        }
+        if (most == 0 && !tiles.empty()) return WLLM_BAD_SIZE;
         // items: of the tiles that follow one another with the same keys, range by range
         std::vector<Item> items;
         long long rows = 0, results = 0;
         for (size_t i = 0; i < tiles.size();) {
             size_t j = i + 1;
-            while (j < tiles.size() && !tiles[i].own && !tiles[j].own && tiles[j].request == tiles[i].request && tiles[j].key_lo == tiles[i].key_lo && tiles[j].key_hi == tiles[i].key_hi) ++j;
-            const int k = keys_of(tiles[i]), parts = (k + per - 1) / per;
+            while (j < tiles.size() && !tiles[i].own && !tiles[j].own && is_thin(tiles[j]) == is_thin(tiles[i]) && tiles[j].request == tiles[i].request && tiles[j].key_lo == tiles[i].key_lo && tiles[j].key_hi == tiles[i].key_hi) ++j;
+            const int k = keys_of(tiles[i]), parts = parts_of(k, is_thin(tiles[i]), most);
             for (int s = 0; s < parts; ++s) {
                 const int from = (int)((long long)k * s / parts), to = (int)((long long)k * (s + 1) / parts);
                 for (size_t t = i; t < j; ++t) {
-                    items.push_back({(int)t, tiles[i].key_lo + from * key_tile, std::min(tiles[i].key_hi, tiles[i].key_lo + to * key_tile), (int)rows, to - from});
+                    items.push_back({(int)t, tiles[i].key_lo + from * key_tile, std::min(tiles[i].key_hi, tiles[i].key_lo + to * key_tile), (int)rows, (to - from) * costs[2 * is_thin(tiles[t])]});
                     rows += (long long)tiles[t].tokens * rep;
                     results += tiles[t].tokens;
                     if (rows > 0x7fffffff / nkv) return WLLM_BAD_SIZE;
@@ -182,9 +196,9 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
         std::vector<int> starts(total + 1, 0), listed(results);
         for (const Item& it : items)
             for (int t = 0; t < tiles[it.tile].tokens; ++t) ++starts[tokens[tiles[it.tile].token + t] + 1];
-        int most = 0;
+        int most_listed = 0;
         for (long long t = 0; t < total; ++t) {
-            most = std::max(most, starts[t + 1]);
+            most_listed = std::max(most_listed, starts[t + 1]);
             starts[t + 1] += starts[t];
         }
         {
@@ -192,7 +206,7 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             for (const Item& it : items)
                 for (int t = 0; t < tiles[it.tile].tokens; ++t) listed[next[tokens[tiles[it.tile].token + t]]++] = it.row + t * rep;
         }
-        std::stable_sort(items.begin(), items.end(), [](const Item& a, const Item& b) { return a.length > b.length; });
+        std::stable_sort(items.begin(), items.end(), [](const Item& a, const Item& b) { return a.cost > b.cost; });
 
         const long long need[4] = {(long long)items.size(), (long long)tokens.size(), results, total};
         long long cap[4];
@@ -202,7 +216,7 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
         }
         const long long at_items = PLAN_HEADER, at_tokens = at_items + padded(cap[0] * PLAN_ITEM), at_starts = at_tokens + padded(cap[1] * 2), at_results = at_starts + padded(cap[3] + 1),
                         at_positions = at_results + padded(cap[2]), used = at_positions + padded(cap[3]);
-        info[0] = used; info[1] = need[0]; info[2] = rows; info[3] = saved; info[4] = most; info[5] = (long long)tiles.size(); info[6] = need[1]; info[7] = results;
+        info[0] = used; info[1] = need[0]; info[2] = rows; info[3] = saved; info[4] = most_listed; info[5] = (long long)tiles.size(); info[6] = need[1]; info[7] = results;
         if (used > 0x7fffffff) return WLLM_BAD_SIZE;
         if (used > room) return OUT_TOO_SMALL;
         std::fill(out, out + used, 0);
@@ -213,6 +227,9 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             int* o = out + at_items + i * PLAN_ITEM;
             o[ITEM_TOKEN] = t.token; o[ITEM_TOKENS] = t.tokens; o[ITEM_KEY_LO] = items[i].key_lo; o[ITEM_KEY_HI] = items[i].key_hi;
             o[ITEM_REQUEST] = t.request; o[ITEM_OWN] = t.own ? 1 : 0; o[ITEM_ROW] = items[i].row;
+            bool follow = true;
+            for (int j = 1; j < t.tokens && follow; ++j) follow = tokens[t.token + j] == tokens[t.token] + j;
+            o[ITEM_FIRST] = follow ? tokens[t.token] : -1;
         }
         for (size_t i = 0; i < tokens.size(); ++i) {
             out[at_tokens + 2 * i] = tokens[i];

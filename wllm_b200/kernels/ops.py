@@ -798,9 +798,21 @@ class PrefixPlan:
 PREFIX_MIN_KEYS = 128
 
 
-def prefix_rows(dtype: torch.dtype, hd: int, vd: int) -> int:
-    """Rows (token, query head of the group) of an item of a plan, at most (csrc/prefix_attention.cu: ROWS)."""
-    return 32 if dtype == torch.float32 else 256 if hd <= 128 and vd <= 128 else 128
+def prefix_rows(dtype: torch.dtype) -> int:
+    """Rows (token, query head of the group) of an item of a plan, at most."""
+    return 128 if dtype == torch.bfloat16 else 32
+
+
+@functools.lru_cache(maxsize=None)
+def _prefix_costs(dtype: torch.dtype, hd: int, vd: int) -> tuple:
+    """What a plan weighs, in cycles: a tile of keys and an item beside its tiles, for items of many rows and for those of at most 16, which run on other instructions; those 16; a
+    thousand rows of results.  bfloat16: the tensor core's products (100 cycles a step of 16 for the scores, 85 for 128 columns of the output), but no less than a group's turn with three
+    buffers, or two, takes; thin items at the rate of the device's memory (22 bytes a cycle and SM), but no less than their chain.  32 bits: 32 rows by 64 keys on the FMA pipes."""
+    if dtype == torch.float32:
+        return 40 * (hd + vd), 6000, 40 * (hd + vd), 6000, 0, 4 * vd
+    wide, out = -(-hd // 64) * 64, -(-vd // 64) * 64
+    tile = max(100 * wide // 16 + 85 * 8 * out // 128, 1500 if out <= 128 else 3000)
+    return tile, 3500, max(256 * (hd + vd) // 44, 1500), 2500, 16, 3 * vd
 
 
 def prefix_ok(nq: int, nkv: int, hd: int, vd: int, page_size: int, dtype: torch.dtype) -> bool:
@@ -819,8 +831,8 @@ def prefix_plan(tables, q_lens, ctx_lens, page_size: int, nq: int, nkv: int, hd:
         raise KernelError(f"prefix_plan: {nq} query heads on {nkv}, sizes {hd}/{vd}, pages of {page_size}, {dtype}: up to 128 query heads a key/value head in bfloat16, 32 in float32, "
                           "head sizes in steps of 8 up to 256, pages of a power of two of at least 16 tokens")
     bf16 = dtype == torch.bfloat16
-    status, *made = _host_calls().prefix_plan(tables, _numbers(q_lens), _numbers(ctx_lens), page_size, nq // nkv, nkv, prefix_rows(dtype, hd, vd), 128 if bf16 else SIMT_CHUNK,
-                                              1 if bf16 else SIMT_CHUNK, max(1, min_keys), sm_count() if bf16 else 2 * sm_count(), torch.cuda.is_available())
+    status, *made = _host_calls().prefix_plan(tables, _numbers(q_lens), _numbers(ctx_lens), page_size, nq // nkv, nkv, prefix_rows(dtype), 128 if bf16 else SIMT_CHUNK,
+                                              1 if bf16 else SIMT_CHUNK, max(1, min_keys), sm_count() if bf16 else 2 * sm_count(), torch.cuda.is_available(), _prefix_costs(dtype, hd, vd))
     if status:
         raise KernelError(f"prefix_plan: {_STATUS.get(status, status)}")
     return PrefixPlan((page_size, nq, nkv, hd, vd, dtype), tables.shape[0], tables.shape[1], *made)

@@ -25,7 +25,7 @@
 //
 // An item of up to 16 rows (a decoding request's own keys) would fill an eighth of such a tile, and its chain of waits (queries, scores, exponentials, output, each a round trip through
 // tensor memory) would be as long as a full one's.  There the eight warps multiply on mma.sync, straight from the ring: 16 keys of a tile each for the scores, an eighth of the values'
-// columns each for the output, with two barriers a tile (row maxima, weights).  8 x 8 requests on 4,000 keys, 16 heads of 256, half of whose items are such: see the table's figures below.
+// columns each for the output, with one barrier a tile.  8 x 8 requests on 4,000 keys, 16 heads of 256, half of whose items are such: see the table's figures below.
 //
 // Head sizes that are no multiple of 64 are widened to one in shared memory: a box copy that reaches past a row's end fills with zeros.  Boxes that hold none of an item's keys are not
 // copied; values behind its last key are cleared in shared memory before they are multiplied with their weight of zero (0 x NaN is no zero).
@@ -54,9 +54,9 @@ constexpr int Q_BYTES = BM * HDP * 2;
 constexpr int SMALL = 2 * BM * 4 + BM * 4 + 2 * BM * 4 + 512;      // rows' positions, maxima that the groups hand over, sums of the second group, barriers
 constexpr int MOST_STAGES = (227 * 1024 - Q_BYTES - SMALL) / STAGE;
 constexpr int STAGES = MOST_STAGES > 8 ? 8 : MOST_STAGES;
-static_assert(STAGES >= 2, "a stage for keys and one for values");
+static_assert(STAGES >= 2 && STAGES >= BUFS * VC, "when a tile's scores are there, what its values' stages held before has been used");
 constexpr int SMEM = Q_BYTES + STAGES * STAGE + SMALL;
-// what a thin item keeps where it has no queries (rows 16 .. 127 of their first 64 columns): weights [2][16][128] bfloat16, row maxima [2][8][16], sums [8][16]
+// what a thin item keeps where it has no queries (rows 16 .. 127 of their first 64 columns): weights [2][16][128] bfloat16, row maxima [2][16][8], sums [8][16]
 constexpr int THIN_P = THIN * 128, THIN_M = THIN_P + 2 * THIN * BN * 2, THIN_L = THIN_M + 2 * 8 * THIN * 4;
 static_assert(THIN_L + 8 * THIN * 4 <= BM * 128, "behind the queries of 16 rows");
 constexpr int THREADS = 128 + 256;
@@ -112,11 +112,11 @@ __device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void ldsm2t(uint32_t addr, uint32_t& a, uint32_t& b) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // the 256 threads of the groups: true if all of them say so
@@ -174,7 +174,7 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
     // by score buffer: s_full, p_full, pv_done; by group and warp of it: its maxima are there.  What the tensor core or else the groups' eight warps hand back (stages, queries) counts
     // eight arrivals: the products' thread makes seven of them itself and leaves the last to the products' end.
     const uint32_t full = bars, empty = full + 8 * STAGES, s_full = empty + 8 * STAGES, p_full = s_full + 8 * BUFS, pv_done = p_full + 8 * BUFS, q_full = pv_done + 8 * BUFS,
-                   q_empty = q_full + 8, begun = q_empty + 8, o_free = begun + 8, edge_full = o_free + 8, m_ready = edge_full + 8, tmem_slot = m_ready + 64;
+                   q_empty = q_full + 8, begun = q_empty + 8, o_free = begun + 8, m_ready = o_free + 8, tmem_slot = m_ready + 64;
     int* at_of = reinterpret_cast<int*>(smem + (small - base));                   // [2][128] positions of an item's rows, items in turn
     volatile float* m_of = reinterpret_cast<volatile float*>(at_of + 2 * BM);     // [128]
     volatile float* l_of = m_of + BM;                                             // [2][128] the second group's sums, items in turn
@@ -189,7 +189,6 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
         for (int b = 0; b < BUFS; ++b) { mbar_init(s_full + 8 * b, 1); mbar_init(p_full + 8 * b, 4); mbar_init(pv_done + 8 * b, 1); }
         mbar_init(q_full, 2); mbar_init(q_empty, 8);
         mbar_init(begun, 8); mbar_init(o_free, 8);
-        mbar_init(edge_full, 1);
         for (int i = 0; i < 8; ++i) mbar_init(m_ready + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -199,7 +198,6 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot_ptr;
-    pdl_wait();                          // the kernel behind this one may start when its CTAs leave: earlier, the merge's would crowd on the SMs that this launch leaves free
 
     const int total = (p.n_items >= 0 ? p.n_items : p.plan[PLAN_ITEMS]) * p.nkv;
     const int rep = p.nq / p.nkv, page_shift = 31 - __clz(p.page_size);
@@ -210,6 +208,10 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
         const int4 a = at[0], b = at[1];
         return Item{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     };
+    // The plan was copied before the step's first kernel started: the first item is looked up while the kernel before this one may still run.  (The kernel behind this one starts when
+    // its CTAs leave: earlier, the merge's would crowd on the SMs that this launch leaves free.)
+    Item next = item_of(blockIdx.x);
+    pdl_wait();
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
@@ -217,8 +219,7 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
             // ---------------- keys and values ----------------
             const int box_rows = p.page_size < BN ? p.page_size : BN, boxes = BN / box_rows, box_shift = 31 - __clz(box_rows);      // boxes of a tile: one to eight
             bool ok = true;
-            int fill = 0, edges = 0;
-            Item next = item_of(pair_at(0));
+            int fill = 0;
             for (int k = 0, it; ok && (it = pair_at(k)) < total; ++k) {
                 const Item item = next;
                 next = item_of(pair_at(k + 1));
@@ -235,37 +236,22 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                 int window = 0, before = 0, now = row_of_box(0), later = row_of_box(1);
                 auto load = [&](int n, bool value) {
                     const int width = value ? VW : KW, chunks = value ? VC : KC;
-                    const int held = min(BN, hi - lo - n * BN), copied = (held + box_rows - 1) >> box_shift;       // rows of keys; boxes that hold some
-                    const bool edge = value && held < BN;
+                    const int copied = (min(BN, hi - lo - n * BN) + box_rows - 1) >> box_shift;       // boxes that hold keys of the item
                     if (!value && (n * boxes) >> 5 > window) { ++window; before = now; now = later; later = row_of_box(window + 1); }
                     const int box = n * boxes + lane;
                     const int row = __shfl_sync(0xffffffffu, (n * boxes) >> 5 == window ? now : before, box & 31);
-                    for (int c = 0; c < chunks; ++c) {
+                    for (int c = 0; c < chunks; ++c, ++fill) {
                         const int s = fill % STAGES;
                         if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ((fill / STAGES) & 1) ^ 1))) { ok = false; return; }
                         const uint32_t dst = ring + s * STAGE;
-                        // values that reach past the item's last key land on a barrier of their own, are cleared there, and are announced then
-                        const uint32_t bar = edge ? edge_full : full + 8 * s;
-                        if (lane == 0) mbar_expect_tx(bar, (copied << box_shift) * width * 2);
+                        if (lane == 0) mbar_expect_tx(full + 8 * s, (copied << box_shift) * width * 2);
                         __syncwarp();
                         if (lane < copied)
                             for (int cb = 0; cb < width / 64; ++cb)
-                                tma_load_2d(dst + cb * (BN * 128) + (lane << box_shift) * 128, value ? &v_map : &k_map, bar, c * width + cb * 64, row);
-                        if (edge) {
-                            if (!__all_sync(0xffffffffu, mbar_wait(edge_full, edges & 1))) { ok = false; return; }
-                            ++edges;
-                            for (int i = lane; i < (BN - held) * (VW / 8); i += 32) {
-                                const int r = held + i / (VW / 8), rest = i % (VW / 8);
-                                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + (rest >> 3) * (BN * 128) + r * 128 + (rest & 7) * 16), "r"(0u) : "memory");
-                            }
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(full + 8 * s);
-                        }
-                        ++fill;
+                                tma_load_2d(dst + cb * (BN * 128) + (lane << box_shift) * 128, value ? &v_map : &k_map, full + 8 * s, c * width + cb * 64, row);
                     }
                 };
-                const int ahead = item.tokens * rep <= THIN ? 1 : BUFS;
+                const int ahead = item.tokens * rep <= THIN ? 2 : BUFS;
                 for (int n = 0; n < ahead && n < T && ok; ++n) load(n, false);
                 for (int n = 0; n < T && ok; ++n) {
                     load(n, true);
@@ -321,7 +307,6 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                     tc_commit(pv_done + 8 * (t % BUFS));
                     return true;
                 };
-                Item next = item_of(pair_at(0));
                 for (int k = 0; ok && pair_at(k) < total; ++k) {
                     const Item item = next;
                     next = item_of(pair_at(k + 1));
@@ -353,7 +338,7 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
         } else {
             // ---------------- queries: a warp takes every other 32 rows (of the first item the groups take them) ----------------
             bool ok = true;
-            Item next = item_of(pair_at(1));
+            next = item_of(pair_at(1));
             for (int k = 1, it; (it = pair_at(k)) < total; ++k) {
                 const Item item = next;
                 next = item_of(pair_at(k + 1));
@@ -380,7 +365,6 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
         const float cap_in = p.capl > 0.f ? 2.0f * p.scale2 / p.capl : 0.f;
         bool ok = true;
         int use = 0, tile = 0, other_handed = 0;                 // stages used, tiles, maxima that the other group has handed over, before this item
-        Item next = item_of(pair_at(0));
         if ((int)blockIdx.x < total) {                           // the first item's queries: nobody else has anything to do yet
             const int end = min((warp - 3) * 16, next.tokens * rep);
             if ((warp - 4) * 16 < end) load_rows(p, next, (int)blockIdx.x % p.nkv, rep, (warp - 4) * 16, end, q_s, at_of);
@@ -396,9 +380,19 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
             if (!__all_sync(0xffffffffu, mbar_wait(q_full, k & 1))) ok = false;
             if (rows <= THIN) {
                 // ---- up to 16 rows: mma.sync; this thread holds parts of rows lane / 4 and lane / 4 + 8 ----
-                const int w = warp - 4;
-                constexpr int NT = VDP / 64;                     // this warp's blocks of 8 value columns: w * NT ...
-                float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope2[2];
+                // A warp weighs its 16 keys of a tile relative to a maximum of its own, rounded up to a whole number: what brings its weights to the maximum of all warps is a power of
+                // two then, by which bfloat16 weights are multiplied without a rounding when the output's products read them.  So the warps meet once a tile, with the next tile's scores
+                // worked out in between.
+                const int w = warp - 4, a_row = lane & 15, a_chunk = lane >> 4;
+                static_assert((VW / 8) % (VDP / 64) == 0, "a warp's value columns lie in one stage");
+                constexpr int NT = VDP / 64, STEPS = (HD + 15) / 16;   // this warp's blocks of 8 value columns: w * NT ...; products of 16 of the head's columns
+                uint32_t qf[STEPS][4];
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const int c = i * 2 + a_chunk;
+                    ldsm4(q_s + (c >> 3) * (BM * 128) + a_row * 128 + (((c ^ a_row) & 7) << 4), qf[i]);
+                }
+                float o[NT][4], sv[2][4], mw[2] = {-INFINITY, -INFINITY}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope2[2];
                 int last[2], pos[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -408,34 +402,54 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                     slope2[i] = (p.slopes != nullptr && r < rows) ? p.slopes[g * rep + r % rep] * LOG2E : 0.f;
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(begun);
+                // The queries are in registers: those of another thin item may come at once.  (A wide one's would overwrite the weights.)
+                const bool early = pair_at(k + 1) < total && next.tokens * rep <= THIN;
+                if (lane == 0) {
+                    mbar_arrive(begun);
+                    if (early) mbar_arrive(q_empty);
+                }
 #pragma unroll
                 for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
                 volatile float* mx_all = reinterpret_cast<volatile float*>(smem + THIN_M);
                 volatile float* l_all = reinterpret_cast<volatile float*>(smem + THIN_L);
-                for (int n = 0; n < T; ++n) {
-                    const int key0 = lo + n * BN;
-                    // scores of this warp's 16 keys
-                    float sv[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-                    const int a_row = lane & 15, a_chunk = lane >> 4, b_row = w * 16 + (lane & 7) + (lane >> 4) * 8, b_chunk = (lane >> 3) & 1;
+                auto scores = [&]() {                            // of this warp's 16 keys of the next tile
+                    const int b_row = w * 16 + (lane & 7) + (lane >> 4) * 8, b_chunk = (lane >> 3) & 1;
+                    float even[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, odd[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
                     for (int c = 0; c < KC; ++c, ++use) {
                         const int s = use % STAGES;
                         if (ok && !__all_sync(0xffffffffu, mbar_wait(full + 8 * s, (use / STAGES) & 1))) ok = false;
                         const uint32_t kb = ring + s * STAGE;
+                        // (64 columns' fragments at once: a load's latency is that of the two products behind it)
 #pragma unroll
-                        for (int i = 0; i < KW / 16; ++i) {
-                            if (c * KW + i * 16 >= HD) continue;
-                            uint32_t a[4], b[4];
-                            const int qa = c * (KW / 8) + i * 2 + a_chunk, ka = i * 2 + b_chunk;
-                            ldsm4(q_s + (qa >> 3) * (BM * 128) + a_row * 128 + (((qa ^ a_row) & 7) << 4), a);
-                            ldsm4(kb + (ka >> 3) * (BN * 128) + b_row * 128 + (((ka ^ b_row) & 7) << 4), b);
-                            mma16816(sv[0], a, b[0], b[1]);
-                            mma16816(sv[1], a, b[2], b[3]);
+                        for (int i0 = 0; i0 < KW / 16; i0 += 4) {
+                            uint32_t b[4][4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                if (c * KW + (i0 + u) * 16 >= HD) continue;
+                                const int ka = (i0 + u) * 2 + b_chunk;
+                                ldsm4(kb + (ka >> 3) * (BN * 128) + b_row * 128 + (((ka ^ b_row) & 7) << 4), b[u]);
+                            }
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                if (c * KW + (i0 + u) * 16 >= HD) continue;
+                                mma16816(u & 1 ? odd[0] : even[0], qf[c * (KW / 16) + i0 + u], b[u][0], b[u][1]);
+                                mma16816(u & 1 ? odd[1] : even[1], qf[c * (KW / 16) + i0 + u], b[u][2], b[u][3]);
+                            }
                         }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(empty + 8 * s);
                     }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sv[j][e] = even[j][e] + odd[j][e];
+                };
+                auto power = [](float d) { return d < -126.f ? 0u : (uint32_t)(127 + (int)d) << 23; };      // 2^d for a whole d <= 0, as the bits of a float
+                scores();
+                for (int n = 0; n < T; ++n) {
+                    const int key0 = lo + n * BN;
+                    const uint32_t p_s = q_s + THIN_P + (n & 1) * (THIN * BN * 2);
                     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
@@ -451,51 +465,72 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                         }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
+                        const int r = (lane >> 2) + 8 * i;
                         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
                         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-                        if ((lane & 3) == 0) mx_all[((n & 1) * 8 + w) * THIN + (lane >> 2) + 8 * i] = mx[i];
-                    }
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    const uint32_t p_s = q_s + THIN_P + (n & 1) * (THIN * BN * 2);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int r = (lane >> 2) + 8 * i;
-                        float top = m[i];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) top = fmaxf(top, mx_all[((n & 1) * 8 + j) * THIN + r]);
-                        const float base_now = top == -INFINITY ? 0.f : top, corr = exp2f(m[i] - base_now);
-                        m[i] = top;
-                        l[i] *= corr;
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) { o[j][2 * i] *= corr; o[j][2 * i + 1] *= corr; }
+                        const float top = fmaxf(mw[i], ceilf(mx[i])), from = top == -INFINITY ? 0.f : top;
+                        l[i] *= fast_exp2(mw[i] - from);
+                        mw[i] = top;
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const float e0 = exp2f(sv[j][2 * i] - base_now), e1 = exp2f(sv[j][2 * i + 1] - base_now);
+                            const float e0 = fast_exp2(sv[j][2 * i] - from), e1 = fast_exp2(sv[j][2 * i + 1] - from);
                             l[i] += e0 + e1;
-                            const int chunk = w * 2 + j;         // eight keys
-                            asm volatile("st.shared.b32 [%0], %1;" ::"r"(p_s + r * (BN * 2) + ((chunk ^ (r & 7)) << 4) + (lane & 3) * 4), "r"(pack_bf16(e0, e1)) : "memory");
+                            asm volatile("st.shared.b32 [%0], %1;" ::"r"(p_s + r * (BN * 2) + (((w * 2 + j) ^ (r & 7)) << 4) + (lane & 3) * 4), "r"(pack_bf16(e0, e1)) : "memory");
                         }
+                        if ((lane & 3) == 0) mx_all[((n & 1) * THIN + r) * 8 + w] = top;
                     }
+                    if (n + 1 < T) scores();
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                     // this warp's columns of the output
-                    uint32_t a[BN / 16][4];
+                    uint32_t a[BN / 16][4], f[2][8];             // weights; what brings the warps' weights of the two rows to one reference, twice in a register
 #pragma unroll
                     for (int i = 0; i < BN / 16; ++i) ldsm4(p_s + a_row * (BN * 2) + (((i * 2 + a_chunk) ^ (a_row & 7)) << 4), a[i]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float4* all = reinterpret_cast<const float4*>(smem + THIN_M) + ((n & 1) * THIN + (lane >> 2) + 8 * i) * 2;
+                        const float4 u = all[0], v = all[1];
+                        const float mj[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+                        const float top = fmaxf(max3(m[i], fmaxf(u.x, u.y), fmaxf(u.z, u.w)), max3(fmaxf(v.x, v.y), v.z, v.w)), from = top == -INFINITY ? 0.f : top;
+                        const float corr = __uint_as_float(power(m[i] - from));
+                        m[i] = top;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) { const uint32_t x = power(mj[j] - from); f[i][j] = __byte_perm(x, x, 0x3232); }
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) { o[j][2 * i] *= corr; o[j][2 * i + 1] *= corr; }
+                    }
+#pragma unroll
+                    for (int i = 0; i < BN / 16; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a[i][e]), *reinterpret_cast<__nv_bfloat162*>(&f[e & 1][i]));
+                            a[i][e] = *reinterpret_cast<const uint32_t*>(&v);
+                        }
+                    // (a warp's columns lie in one stage)
 #pragma unroll
                     for (int c = 0; c < VC; ++c, ++use) {
                         const int s = use % STAGES;
                         if (ok && !__all_sync(0xffffffffu, mbar_wait(full + 8 * s, (use / STAGES) & 1))) ok = false;
-                        const uint32_t vb = ring + s * STAGE;
+                        const int col0 = w * NT - c * (VW / 8);          // the first block's place in this chunk
+                        if (col0 >= 0 && col0 < VW / 8) {
+                            const uint32_t vb = ring + s * STAGE;
+                            if (key0 + BN > hi) {                // (slots behind the last key hold whatever lay there: 0 x NaN is no zero)
+                                for (int r = hi - key0 + lane; r < BN; r += 32)
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            const int col = w * NT + j - c * (VW / 8);       // the block's place in this chunk
-                            if (col < 0 || col >= VW / 8) continue;
+                                    for (int j = 0; j < NT; ++j)
+                                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + ((col0 + j) >> 3) * (BN * 128) + r * 128 + ((((col0 + j) ^ r) & 7) << 4)), "r"(0u)
+                                                     : "memory");
+                                __syncwarp();
+                            }
 #pragma unroll
-                            for (int i = 0; i < BN / 16; ++i) {
-                                uint32_t b0, b1;
-                                const int key = i * 16 + (lane & 15);
-                                ldsm2t(vb + (col >> 3) * (BN * 128) + key * 128 + (((col ^ key) & 7) << 4), b0, b1);
-                                mma16816(o[j], a[i], b0, b1);
+                            for (int i = 0; i < BN / 16; i += 2) {
+                                uint32_t b[NT][4];
+                                const int key = i * 16 + lane;
+#pragma unroll
+                                for (int j = 0; j < NT; ++j) ldsm4t(vb + ((col0 + j) >> 3) * (BN * 128) + key * 128 + ((((col0 + j) ^ key) & 7) << 4), b[j]);
+#pragma unroll
+                                for (int j = 0; j < NT; ++j) mma16816(o[j], a[i], b[j][0], b[j][1]);
+#pragma unroll
+                                for (int j = 0; j < NT; ++j) mma16816(o[j], a[i + 1], b[j][2], b[j][3]);
                             }
                         }
                         __syncwarp();
@@ -506,7 +541,7 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                 for (int i = 0; i < 2; ++i) {
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-                    if ((lane & 3) == 0) l_all[w * THIN + (lane >> 2) + 8 * i] = l[i];
+                    if ((lane & 3) == 0) l_all[w * THIN + (lane >> 2) + 8 * i] = l[i] * __uint_as_float(power(mw[i] - (m[i] == -INFINITY ? 0.f : m[i])));
                 }
                 if (!all_of_groups(ok)) {
                     if (!ok) atomicExch(p.status, GAVE_UP_SOFTMAX);
@@ -529,7 +564,10 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                     }
                 }
                 __syncwarp();
-                if (lane == 0) { mbar_arrive(q_empty); mbar_arrive(o_free); }
+                if (lane == 0) {
+                    if (!early) mbar_arrive(q_empty);
+                    mbar_arrive(o_free);
+                }
                 continue;
             }
             const bool live = row < rows, warp_live = row - lane < rows;
@@ -617,6 +655,22 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                         tc_st32(t_lane + c0, ov);
                     }
                 }
+                // Behind the item's last key the tile holds whatever lay there; its weights are zeros, but 0 x NaN is no zero.  The values' stages are not handed back before this
+                // tile's output, and what was in them before has been used (the scores of this tile come behind it).
+                if (key0 + BN > hi) {
+                    const int first = use + min(T, n + BUFS) * KC + n * VC, held = hi - key0;
+                    bool there = true;
+                    for (int c = 0; c < VC; ++c) {
+                        const int s = (first + c) % STAGES;
+                        there = there && mbar_wait(full + 8 * s, ((first + c) / STAGES) & 1);
+                        for (int i = row; i < (BN - held) * (VW / 8); i += 128) {
+                            const int r = held + i / (VW / 8), rest = i % (VW / 8);
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + s * STAGE + (rest >> 3) * (BN * 128) + r * 128 + (rest & 7) * 16), "r"(0u) : "memory");
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    if (!__all_sync(0xffffffffu, there)) { ok = false; break; }
+                }
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -674,70 +728,67 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
     }
 }
 
-// The merge of a token's results: grid (tokens, kv heads, groups of warps), a warp a query head.  VD / 8 lanes take a result, 8 columns each, so as many results at once as fit a warp.  Bound
-// by the latency of its chain of loads (starts, list, maxima and sums, results) where results are few: a lane's results are asked for four at a time.
+// The merge of a token's results: grid (tokens, kv heads, groups of warps).  A warp takes up to four neighbouring query heads, whose rows of eight columns are one line, by 32 / heads blocks
+// of eight columns, a lane each; results eight at a time, with a running maximum.  Bound by the latency of its chain of loads (starts, list, results), hence the eight in flight.
 constexpr int MERGE_WARPS = 4;
+__host__ __device__ __forceinline__ int merge_heads(int rep) { return rep >= 4 ? 4 : rep >= 2 ? 2 : 1; }
+__host__ __device__ __forceinline__ int merge_units(int rep) {
+    const int heads = merge_heads(rep), blocks = 32 / heads;
+    return (rep + heads - 1) / heads * ((VD / 8 + blocks - 1) / blocks);
+}
 __global__ void __launch_bounds__(MERGE_WARPS * 32)
 prefix_merge_kernel(bf16* __restrict__ out, int out_stride, const int* __restrict__ plan, int rep, long long rows, const float* __restrict__ part_o, const float* __restrict__ part_ml,
                     const float* __restrict__ sinks) {
     pdl_begin();
-    const int token = blockIdx.x, g = blockIdx.y, h = (int)blockIdx.z * MERGE_WARPS + (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (h >= rep) return;
+    const int token = blockIdx.x, g = blockIdx.y, unit = (int)blockIdx.z * MERGE_WARPS + (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (unit >= merge_units(rep)) return;
+    const int heads = merge_heads(rep), groups = (rep + heads - 1) / heads;
+    const int h = unit % groups * heads + lane % heads, col = unit / groups * (32 / heads) + lane / heads;
+    if (h >= rep || col >= VD / 8) return;
     const int* starts = plan + plan[PLAN_AT_STARTS];
     const int first = starts[token], n = starts[token + 1] - first;
     if (n <= 0) return;
     const int* list = plan + plan[PLAN_AT_RESULTS] + first;
-    constexpr int PER = VD / 8, SIDE = 32 / PER;             // lanes a result, results side by side
-    const int side = lane / PER, col = lane % PER, head = g * rep + h;
-    const float* mine_o = part_o + ((size_t)g * PER + col) * rows * 8;
+    const float* mine_o = part_o + ((size_t)g * (VD / 8) + col) * rows * 8;
+    const float2* mine_ml = reinterpret_cast<const float2*>(part_ml) + (size_t)g * rows;
     float M = -INFINITY, L = 0.f, O[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        const size_t row = i0 + lane < n ? (size_t)list[i0 + lane] + h : 0;
-        const float2 ml = i0 + lane < n ? *reinterpret_cast<const float2*>(part_ml + ((size_t)g * rows + row) * 2) : make_float2(-INFINITY, 0.f);
-        const int count = min(32, n - i0);
-        float weight = 0.f;
-        for (int u0 = 0; u0 < count; u0 += 4 * SIDE) {
-            float4 v[4][2];
+    constexpr int AHEAD = 8;
+    for (int i0 = 0; i0 < n; i0 += AHEAD) {
+        float4 v[AHEAD][2];
+        float2 ml[AHEAD];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int i = u0 + u * SIDE + side;
-                const size_t at = __shfl_sync(0xffffffffu, row, i & 31);
-                const bool there = side < SIDE && i < count;
-                const float4* src = reinterpret_cast<const float4*>(mine_o + at * 8);
-                v[u][0] = there ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
-                v[u][1] = there ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            if (u0 == 0) {                       // while they are on their way
-                const float M_new = fmaxf(M, warp_max(ml.x)), base = M_new == -INFINITY ? 0.f : M_new;
-                const float keep = exp2f(M - base);
-                weight = exp2f(ml.x - base);
-                L = L * keep + warp_sum(ml.y * weight);
+        for (int u = 0; u < AHEAD; ++u) {
+            const size_t at = (size_t)list[min(i0 + u, n - 1)] + h;
+            ml[u] = mine_ml[at];
+            v[u][0] = reinterpret_cast<const float4*>(mine_o + at * 8)[0];
+            v[u][1] = reinterpret_cast<const float4*>(mine_o + at * 8)[1];
+        }
+        float top = M;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) O[j] *= keep;
-                M = M_new;
-            }
+        for (int u = 0; u < AHEAD; ++u) {
+            if (i0 + u >= n) ml[u] = make_float2(-INFINITY, 0.f);        // (read again: weighs nothing)
+            top = fmaxf(top, ml[u].x);
+        }
+        const float base = top == -INFINITY ? 0.f : top, keep = exp2f(M - base);
+        M = top;
+        L *= keep;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {        // (a result past the end is zero)
-                const float f = __shfl_sync(0xffffffffu, weight, (u0 + u * SIDE + side) & 31);
-                O[0] += v[u][0].x * f; O[1] += v[u][0].y * f; O[2] += v[u][0].z * f; O[3] += v[u][0].w * f;
-                O[4] += v[u][1].x * f; O[5] += v[u][1].y * f; O[6] += v[u][1].z * f; O[7] += v[u][1].w * f;
+        for (int j = 0; j < 8; ++j) O[j] *= keep;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const float f = exp2f(ml[u].x - base);
+            if (i0 + u < n) {
+                L = fmaf(ml[u].y, f, L);
+                O[0] = fmaf(v[u][0].x, f, O[0]); O[1] = fmaf(v[u][0].y, f, O[1]); O[2] = fmaf(v[u][0].z, f, O[2]); O[3] = fmaf(v[u][0].w, f, O[3]);
+                O[4] = fmaf(v[u][1].x, f, O[4]); O[5] = fmaf(v[u][1].y, f, O[5]); O[6] = fmaf(v[u][1].z, f, O[6]); O[7] = fmaf(v[u][1].w, f, O[7]);
             }
         }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float sum = O[j];
-        for (int s = 1; s < SIDE; ++s) sum += __shfl_sync(0xffffffffu, O[j], (col + s * PER) & 31);
-        O[j] = sum;
-    }
-    if (sinks) L += exp2f(sinks[head] * LOG2E - (M == -INFINITY ? 0.f : M));
-    if (side == 0) {
-        const float inv = 1.0f / L;
-        uint4 o{pack_bf16(O[0] * inv, O[1] * inv), pack_bf16(O[2] * inv, O[3] * inv), pack_bf16(O[4] * inv, O[5] * inv), pack_bf16(O[6] * inv, O[7] * inv)};
-        bf16* to = out + (size_t)token * out_stride + (size_t)head * VD + col * 8;
-        *reinterpret_cast<uint2*>(to) = uint2{o.x, o.y};
-        *reinterpret_cast<uint2*>(to + 4) = uint2{o.z, o.w};
-    }
+    if (sinks) L += exp2f(sinks[g * rep + h] * LOG2E - (M == -INFINITY ? 0.f : M));
+    const float inv = 1.0f / L;
+    bf16* to = out + (size_t)token * out_stride + (size_t)(g * rep + h) * VD + col * 8;
+    *reinterpret_cast<uint2*>(to) = uint2{pack_bf16(O[0] * inv, O[1] * inv), pack_bf16(O[2] * inv, O[3] * inv)};
+    *reinterpret_cast<uint2*>(to + 4) = uint2{pack_bf16(O[4] * inv, O[5] * inv), pack_bf16(O[6] * inv, O[7] * inv)};
 }
 
 // --------------------------------------------------------------------------------------
@@ -800,6 +851,6 @@ WLLM_API int wllm_prefix_attention(const void* q, int q_stride, void* out, int o
     const int st = wllm_launch(prefix_kernel, dim3((unsigned)(pairs < ctas ? pairs : ctas)), THREADS, SMEM, stream, p, km, vm);
     if (st) return st;
     const int rep = nq / nkv;
-    return wllm_launch(prefix_merge_kernel, dim3(n_tokens, nkv, (rep + MERGE_WARPS - 1) / MERGE_WARPS), MERGE_WARPS * 32, 0, stream, (bf16*)out, out_stride, plan, rep, rows,
+    return wllm_launch(prefix_merge_kernel, dim3(n_tokens, nkv, (merge_units(rep) + MERGE_WARPS - 1) / MERGE_WARPS), MERGE_WARPS * 32, 0, stream, (bf16*)out, out_stride, plan, rep, rows,
                        (const float*)p.part_o, (const float*)p.part_ml, sinks);
 }

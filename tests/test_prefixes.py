@@ -1,0 +1,144 @@
+"""Prefixes and samples in the scheduler, with a stand-in for the step function: what is computed once, what waits for what, what is given back when."""
+import pytest
+
+from test_scheduler import ArgmaxSampler, FakeRunner, Request, Scheduler
+from wllm_b200.engine.request import RequestStatus
+from wllm_b200.sampling import SamplingParams
+from wllm_b200.sampling.params import sample_seed
+
+
+def make(pages=24, **kw):
+    runner = FakeRunner(pages)
+    return runner, Scheduler(runner, ArgmaxSampler(), **kw)
+
+
+def request(rid, prompt, prefix=None, max_tokens=4, **kw):
+    return Request(rid, list(prompt), SamplingParams(max_tokens=max_tokens, ignore_eos=True, **kw), prefix=prefix)
+
+
+def alone(prompt, max_tokens=4):
+    _, s = make()
+    r = request("x", prompt, max_tokens=max_tokens)
+    s.add_request(r)
+    s.run_to_completion()
+    return r.output_token_ids
+
+
+@pytest.mark.parametrize("length", [1, 3, 4, 5, 8, 11])
+@pytest.mark.parametrize("budget", [None, 3])
+@pytest.mark.parametrize("async_scheduling", [False, True])
+def test_a_prefix_is_computed_once_and_changes_no_token(length, budget, async_scheduling):
+    begin = [(5 * i) % 50 for i in range(length)]
+    runner, s = make(chunked_prefill_tokens=budget, async_scheduling=async_scheduling)
+    prefix = s.add_prefix(begin)
+    assert not prefix.ready and s.has_unfinished()
+    tails = [[7], [7, 9, 30], [1, 2, 3, 4, 5, 6]]
+    reqs = [request(i, begin + t, prefix) for i, t in enumerate(tails)]
+    for r in reqs:
+        s.add_request(r)
+    assert prefix.users == 3
+    with pytest.raises(ValueError, match="unfinished"):
+        s.drop_prefix(prefix)
+    s.run_to_completion()
+    assert prefix.ready and prefix.users == 0 and s.stats["prefill_tokens"] == length + sum(map(len, tails))
+    assert [r.output_token_ids for r in reqs] == [alone(begin + t) for t in tails]
+    assert runner.cache.free_pages() == [24 - -(-length // 4)]       # the prefix stays
+    late = request("late", begin + [9, 9], prefix)
+    s.add_request(late)
+    s.run_to_completion()
+    assert late.output_token_ids == alone(begin + [9, 9])
+    s.drop_prefix(prefix)
+    runner.cache.check()
+    assert runner.cache.free_pages() == [24] and prefix.holder.status == RequestStatus.FINISHED
+    for wrong in (lambda: s.drop_prefix(prefix), lambda: s.add_request(request("y", begin + [1], prefix))):
+        with pytest.raises(ValueError, match="dropped"):
+            wrong()
+
+
+def test_prompts_that_do_not_begin_with_their_prefix_are_refused():
+    _, s = make()
+    prefix = s.add_prefix([1, 2, 3])
+    for prompt in ([1, 2, 3], [1, 2], [1, 2, 4, 5], [9]):
+        with pytest.raises(ValueError, match="begins with"):
+            s.add_request(request("x", prompt, prefix))
+    assert prefix.users == 0
+    for bad in ([], [60], [1] * 64):
+        with pytest.raises(ValueError):
+            s.add_prefix(bad)
+    assert len(s.prefixes) == 1 and len(s.waiting) == 1
+    s.drop_prefix(prefix)
+    assert not s.has_unfinished()
+
+
+def test_prefixes_of_prefixes_and_those_made_for_a_few():
+    runner, s = make()
+    system = s.add_prefix([3, 1, 4, 1, 5])
+    document = s.add_prefix([3, 1, 4, 1, 5, 9, 2, 6, 5], prefix=system, auto=True)
+    reqs = [request(i, document.token_ids + [i], document) for i in range(3)] + [request(9, system.token_ids + [8], system)]
+    for r in reqs:
+        s.add_request(r)
+    assert system.users == 2 and document.users == 3
+    s.run_to_completion()
+    assert [r.output_token_ids for r in reqs] == [alone(r.prompt_token_ids) for r in reqs]
+    assert document.dropped and not system.dropped and system.users == 0 and s.prefixes == [system]
+    s.drop_prefix(system)
+    assert runner.cache.free_pages() == [24]
+
+
+def test_cancelled_users_give_a_prefix_back():
+    runner, s = make()
+    prefix = s.add_prefix([3, 1, 4, 1, 5], auto=True)
+    reqs = [request(i, prefix.token_ids + [i], prefix) for i in range(2)]
+    for r in reqs:
+        s.add_request(r)
+    s.step()
+    s.step()
+    assert s.cancel(0) and not prefix.dropped and s.cancel(1) and prefix.dropped
+    assert not s.cancel(("prefix", 0)) and runner.cache.free_pages() == [24] and not s.has_unfinished()
+    # before it was computed
+    prefix = s.add_prefix([3, 1, 4], auto=True)
+    s.add_request(request("a", [3, 1, 4, 1], prefix))
+    assert s.cancel("a") and prefix.dropped and not s.has_unfinished()
+
+
+@pytest.mark.parametrize("admission", ["worst_case", "optimistic"])
+def test_scarce_pages(admission):
+    """Requests are admitted by what they need beside the prefix's full pages; preempted ones are forked again."""
+    begin = list(range(18))                                           # 4 full pages of 4 and two tokens
+    runner, s = make(pages=12, admission=admission)
+    prefix = s.add_prefix(begin)
+    reqs = [request(i, begin + [i], prefix, max_tokens=9) for i in range(5)]
+    for r in reqs:
+        s.add_request(r)                                              # 7 pages each at the end, 3 of their own; 5 are the prefix's
+    most = 0
+    while s.has_unfinished():
+        s.step()
+        runner.cache.check()
+        most = max(most, len(s.live))
+    assert most >= 2 and [r.output_token_ids for r in reqs] == [alone(r.prompt_token_ids, 9) for r in reqs]
+    assert (s.stats["preemptions"] > 0) == (admission == "optimistic")
+    with pytest.raises(ValueError, match="prefixes"):
+        s.add_request(request("big", list(range(20)) + [1], max_tokens=20))     # 11 pages: more than the prefix leaves
+    assert s.largest_need() == 5
+    s.drop_prefix(prefix)
+    assert runner.cache.free_pages() == [12] and s.largest_need() == 0
+
+
+def test_slots_are_left_for_no_more_than_there_are():
+    runner = FakeRunner(24, max_requests=3)
+    s = Scheduler(runner, ArgmaxSampler())
+    prefix = s.add_prefix([1, 2, 3, 4, 5])
+    reqs = [request(i, prefix.token_ids + [i], prefix) for i in range(4)]
+    for r in reqs:
+        s.add_request(r)
+    while s.has_unfinished():
+        s.step()
+        assert len(s.live) <= 2
+    assert all(len(r.output_token_ids) == 4 for r in reqs)
+
+
+def test_samples_draw_from_seeds_of_their_own():
+    seeds = [sample_seed(7, k) for k in range(100)]
+    assert seeds[0] == 7 and len(set(seeds)) == 100 and all(0 <= x < 1 << 63 for x in seeds[1:])
+    with pytest.raises(ValueError):
+        SamplingParams(n=0)

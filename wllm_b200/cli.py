@@ -37,6 +37,7 @@ def parser() -> argparse.ArgumentParser:
     g = ap.add_argument_group("prompts (token ids)")
     g.add_argument("--prompt-ids", action="append", default=[], metavar="I,J,K", help="one prompt; may be repeated")
     g.add_argument("--prompt-lens", default=None, metavar="N,M", help="random prompts of these lengths")
+    g.add_argument("--prefix-ids", default=None, metavar="I,J,K", help="tokens that every prompt begins with: computed once")
     g.add_argument("--prompt-seed", type=int, default=0)
     s = ap.add_argument_group("sampling")
     s.add_argument("--max-tokens", type=int, default=16)
@@ -47,6 +48,7 @@ def parser() -> argparse.ArgumentParser:
     s.add_argument("--repetition-penalty", type=float, default=1.0)
     s.add_argument("--seed", type=int, default=None)
     s.add_argument("--ignore-eos", action="store_true")
+    s.add_argument("--n", type=int, default=1, help="samples of every prompt, which is computed once for all of them")
     r = ap.add_argument_group("random weights")
     r.add_argument("--write-random-model", metavar="DIR", help="write config.json and model.safetensors, then exit")
     r.add_argument("--config-json", metavar="FILE", help="configuration for --write-random-model")
@@ -86,13 +88,14 @@ def main(argv=None) -> int:
         parser().error("give --prompt-ids or --prompt-lens")
     sp = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p,
                         repetition_penalty=args.repetition_penalty, seed=args.seed, max_tokens=args.max_tokens,
-                        ignore_eos=args.ignore_eos)
+                        ignore_eos=args.ignore_eos, n=args.n)
     start = time.time()
-    outs = llm.generate(prompts, sp)
+    prefix = llm.add_prefix([int(t) for t in args.prefix_ids.split(",") if t.strip()]) if args.prefix_ids else None
+    outs = llm.generate(prompts, sp, prefix=prefix)
     elapsed = time.time() - start
     for o in outs:
         print(json.dumps({"request": o.request_id, "prompt_tokens": len(o.prompt_token_ids), "token_ids": o.token_ids,
-                          "finish_reason": o.finish_reason}))
+                          **({"sample": o.sample} if args.n > 1 else {}), "finish_reason": o.finish_reason}))
     st = llm.stats
     log.info("%d requests, %d prompt + %d generated tokens in %.2f s; %d steps, %d preemptions, pages high-water %s",
              len(outs), sum(len(o.prompt_token_ids) for o in outs), sum(len(o.token_ids) for o in outs), elapsed,

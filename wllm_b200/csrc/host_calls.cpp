@@ -454,11 +454,11 @@ PyObject* copy_pages(Args v, Py_ssize_t n) {
     return both;
 }
 
-// tables, q_lens, ctx_lens, page_size, query heads a kv head, kv heads, rows of an item, keys of a tile, align, min_keys, CTAs at once, pinned memory, costs (six)
+// tables, q_lens, ctx_lens, page_size, query heads a kv head, kv heads, rows of an item, keys of a tile, align, min_keys, CTAs at once, pinned memory, costs (six), caps (four)
 //   -> (status, the plan's array, ints used, items, rows, keys saved, most results, tiles, tokens, longest context)
 PyObject* prefix_plan(Args v, Py_ssize_t n) {
-    count(n, 13);
-    const std::vector<int> costs = numbers(v[12], "costs", 6);
+    count(n, 14);
+    const std::vector<int> costs = numbers(v[12], "costs", 6), caps = numbers(v[13], "caps", 4);
     struct View {
         Py_buffer b;
         bool held = false;
@@ -487,15 +487,14 @@ PyObject* prefix_plan(Args v, Py_ssize_t n) {
     long long tokens = 0, longest = 0;
     for (int x : q) tokens += x;
     for (int x : ctx) longest = x > longest ? x : longest;
-    long long info[8] = {0}, room = 8192 + 64 * (tokens > 0 ? tokens : 0);
-    const int caps[4] = {0, 0, 0, 0};
+    long long info[8] = {0}, room = 8192 + 64 * (tokens > 0 ? tokens : 0) + 8LL * caps[0] + 2LL * caps[1] + caps[2] + 2LL * caps[3];
     at::Tensor host;
     PyObject* status = nullptr;
     for (int go = 0; go < 2; ++go) {
         host = at::empty({room}, at::TensorOptions().dtype(at::kInt).pinned_memory(truth(v[11])));
         Py_XDECREF(status);
         status = launch(plan_fn, "wllm_prefix_plan", tables, (long long)width, (int)R, q.data(), ctx.data(), small(v[3]), small(v[4]), small(v[5]), small(v[6]), small(v[7]), small(v[8]),
-                        small(v[9]), (int)INT32_MAX, small(v[10]), costs.data(), caps, static_cast<int*>(host.data_ptr()), room, info);
+                        small(v[9]), (int)INT32_MAX, small(v[10]), costs.data(), caps.data(), static_cast<int*>(host.data_ptr()), room, info);
         if (!status || PyLong_AsLong(status) != 4) break;
         room = info[0];
     }

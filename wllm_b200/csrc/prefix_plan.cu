@@ -150,7 +150,7 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             }
         }
         auto parts_of = [&](int keys, int thin, int most) { return std::min(keys, std::max(1, (int)(((long long)keys * costs[2 * thin] + most - 1) / most))); };
-        const long long most_items = caps[0] > 0 ? caps[0] : (1 << 22);
+        const long long most_items = caps[0] > 0 ? caps[0] : (1 << 22), most_results = caps[2] > 0 ? caps[2] : (1 << 28);
         int dearest = 1;
         for (const Alike& a : alike) dearest = (int)std::min<long long>(std::max<long long>(dearest, (long long)a.keys * costs[2 * a.thin]), 1 << 30);
         double best = 0;
@@ -167,7 +167,7 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
                 top = std::max(top, (double)((a.keys + parts - 1) / parts) * costs[2 * a.thin] + costs[2 * a.thin + 1]);
             }
             const double end = (n * nkv <= ctas ? top : std::max(top, all * nkv / ctas + 0.5 * top)) + (double)results_rows * nkv * costs[5] / 1000;
-            if (n <= most_items && (most == 0 || end < best * 0.99)) {
+            if (n <= most_items && results_rows / rep <= most_results && (most == 0 || end < best * 0.99)) {
                 best = end;
                 most = bound;
             }

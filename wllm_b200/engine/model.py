@@ -124,6 +124,19 @@ class ComposedModel:
                         total += memory.nbytes()
         return total
 
+    def prefix_layouts(self, page_size: int) -> list:
+        """(group, query heads, kv heads, key size, value size) of the attention that can read pages shared by several requests once for all of them."""
+        found = []
+        for run, ref in zip(self.plan.runs, self.cache_refs):
+            todo = list(self.blocks[run.block].parts()) if ref.group is not None else []
+            while todo:
+                part = todo.pop()
+                todo.extend(part.parts() if hasattr(part, "parts") else [])
+                layout = part.prefix_layout(page_size) if hasattr(part, "prefix_layout") else None
+                if layout is not None and (ref.group, *layout) not in found:
+                    found.append((ref.group, *layout))
+        return found
+
     # -- one step ------------------------------------------------------------------
     def forward(self, ctx) -> torch.Tensor:
         residual = Residual(self.embedding(ctx.token_ids, ctx))

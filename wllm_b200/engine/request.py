@@ -11,6 +11,7 @@ class RequestStatus(Enum):
     WAITING = "waiting"          # queued (new, or preempted and waiting to be run again)
     PREFILLING = "prefilling"    # admitted; part of its known tokens is not in the cache yet
     RUNNING = "running"          # all but its newest token are in the cache: it decodes
+    HELD = "held"                # a prefix whose tokens are all in the cache, for requests to begin with
     FINISHED = "finished"
 
 
@@ -33,6 +34,8 @@ class Request:
     seen: set = field(default_factory=set)   # distinct generated ids, for the repetition penalty
     inflight: int = 0             # 1 while its newest token is sampled on the device and not yet read
     inflight_row: int = -1        # that token's row among the sampled tokens of the step before
+    prefix: object = None         # the Prefix that it begins with: its cache is forked from the prefix's
+    holds: bool = False           # it is the tokens of a prefix: computed and kept, nothing is sampled
 
     @property
     def num_tokens(self) -> int:
@@ -50,7 +53,7 @@ class Request:
 
     @property
     def worst_case_tokens(self) -> int:
-        return len(self.prompt_token_ids) + self.sampling.max_tokens
+        return len(self.prompt_token_ids) + (0 if self.holds else self.sampling.max_tokens)
 
     def append_token(self, token: int, logprob: float, max_model_len: int) -> None:
         self.output_token_ids.append(token)
@@ -66,3 +69,18 @@ class Request:
     @property
     def finished(self) -> bool:
         return self.status == RequestStatus.FINISHED
+
+
+@dataclass(eq=False)
+class Prefix:
+    """Tokens that several requests begin with: computed once, kept in the cache, forked for every request that names it.  Its holder is an entry of the scheduler's
+    queue like any request.  An `auto` prefix is given back when its last user has finished; any other when it is dropped."""
+    token_ids: list
+    holder: Request
+    auto: bool = False
+    users: int = 0                # requests that name it and have not finished
+    dropped: bool = False
+
+    @property
+    def ready(self) -> bool:
+        return self.holder.status == RequestStatus.HELD

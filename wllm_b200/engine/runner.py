@@ -25,6 +25,9 @@ from .model import ComposedModel
 from .staging import PinnedRing
 
 
+PREFIX_SCRATCH = 64 << 20      # floats that a step's results of shared prefixes may take; a step that would take more attends request by request
+
+
 @dataclass
 class StepEntry:
     cache: RequestCache
@@ -52,6 +55,8 @@ class StepContext:
         self.num_single = self.num_multi = 0     # requests with one token / with several
         self.memo: dict = {}                     # what a part worked out for this step and wants again in the next layer
         self.max_q_len = self.max_ctx = 0        # bounds that size the attention grids
+        # attention over shared pages, where it pays in this step: (group, query heads, kv heads, key size, value size) -> (plan, its array on the device)
+        self.prefix: dict = {}
 
     def buffer(self, name: str, shape: tuple, dtype: torch.dtype) -> torch.Tensor:
         return self.runner.workspace(name, shape, dtype)
@@ -74,7 +79,9 @@ class ModelRunner:
         self.h2d_bytes = 0
         self._tables: dict = {}        # cached int32 copies of block tables
         self._graphs_on = False
-        self._graphs: dict = {}        # (requests, table width) -> captured decode step
+        self._graphs: dict = {}        # (requests, table width, whether shared pages are attended to once) -> captured decode step
+        self.prefix_layouts = model.prefix_layouts(cache.page_size)
+        self.prefix_steps = 0          # steps that attended to shared pages once for all of their holders
         self.graph_launches = 0        # kernel launches replayed from graphs so far
 
     def workspace(self, name: str, shape: tuple, dtype: torch.dtype) -> torch.Tensor:
@@ -177,6 +184,32 @@ class ModelRunner:
 
         return host, offsets, [k for k, _ in sizes], (N, R, P), patches
 
+    def _prefix_plans(self, entries: list, host, offsets, shape, fixed: bool):
+        """(host array, {layout: plan}): what the step's attention reads of shared pages, behind the index arrays; nothing where no pages are shared or it would not pay.  `fixed`: for a captured
+        step, whose array lies at the same place whatever the batch holds."""
+        if not self.prefix_layouts or sum(e.cache.forked > 0 for e in entries) < 2:
+            return host, {}
+        (N, R, P), plans, parts = shape, {}, [host]
+
+        def view(name):
+            o, n = offsets[name]
+            return host[o:o + n]
+        lens, ctx_lens, total = view("req_q_len").tolist(), view("req_ctx_len").tolist(), host.shape[0]
+        for layout in self.prefix_layouts:
+            g, nq, nkv, hd, vd = layout
+            saved = sum(e.cache.forked for e in entries)          # (no more keys than that can be shared)
+            if not ops.prefix_pays(saved, nkv, hd, vd, self.model.dtype):
+                continue
+            plan = ops.prefix_plan(view(f"table{g}").reshape(R, P), lens, ctx_lens, self.cache.page_size, nq, nkv, hd, vd, self.model.dtype,
+                                   caps=ops.prefix_caps(R, nkv) if fixed else None)
+            if plan is None or not ops.prefix_pays(plan.saved_keys, nkv, hd, vd, self.model.dtype) or plan.scratch_floats > PREFIX_SCRATCH:
+                continue
+            plans[layout] = plan
+            offsets[("prefix", layout)] = (total, plan.used)
+            parts.append(plan.host.numpy())
+            total += plan.used
+        return (np.concatenate(parts), plans) if plans else (host, {})
+
     def _send(self, host, offsets, patches, device_tokens) -> None:
         """The host array to the device's index buffer; tokens that lie on the device are put in their places."""
         total = host.shape[0]
@@ -194,11 +227,16 @@ class ModelRunner:
                              dev("patch_src", len(patches)))
 
     def _build(self, entries: list, table_width: int | None = None, device_tokens=None,
-               pad_requests: int | None = None) -> StepContext:
+               pad_requests: int | None = None, plans=None) -> StepContext:
         """`pad_requests` (a decode step under a captured graph): the arrays are laid out for that many requests;
         the ones behind the real entries bring no token (q_len 0, no cache slot), so every kernel passes them
         by, and the logits of all rows are wanted (the caller keeps the real ones)."""
         host, offsets, names, (N, R, P), patches = self._host_arrays(entries, table_width, pad_requests)
+        if plans is None:
+            host, plans = self._prefix_plans(entries, host, offsets, (N, R, P), table_width is not None)
+        else:
+            host, offsets = plans[:2]
+            plans = plans[2]
         self._send(host, offsets, patches, device_tokens)
         ps, real = self.cache.page_size, len(entries)
         lens = [len(e.tokens) for e in entries]
@@ -224,6 +262,7 @@ class ModelRunner:
         ctx.req_ctx_len, ctx.req_slot, ctx.want_rows = dev("req_ctx_len"), dev("req_slot"), dev("want_rows")
         ctx.group_slots = [dev(f"slots{g}") for g in range(G)]
         ctx.group_tables = [dev(f"table{g}").view(R, P) for g in range(G)]
+        ctx.prefix = {layout: (plan, dev(("prefix", layout))) for layout, plan in plans.items()}
         return ctx
 
     def _table_copy(self, rc, group: int) -> np.ndarray:
@@ -262,6 +301,14 @@ class ModelRunner:
                 if not 0 <= w < n:
                     raise ValueError(f"request {e.cache.request_id!r}: wanted place {w} outside its {n} tokens")
 
+    def resize_cache(self, num_pages: int) -> None:
+        """Another number of cache pages in every group; live requests keep their tokens.  Captured steps, which hold the old pools' addresses, are made anew when they are next asked for."""
+        try:
+            self.cache.resize(num_pages)
+        finally:
+            self._graphs.clear()
+            self._tables.clear()
+
     # -- captured decode steps -------------------------------------------------------------
     def enable_graphs(self) -> None:
         """Replay a captured CUDA graph for steps in which every request brings one token and
@@ -285,15 +332,17 @@ class ModelRunner:
         bucket = 1                      # 1, 2, 3, 4, 6, 8, 12, 16, 24, 32, ...: a capture serves every count up to its size
         while bucket < len(entries):
             bucket = bucket * 3 // 2 if bucket & (bucket - 1) == 0 and bucket > 1 else (bucket * 4 // 3 if bucket > 2 else bucket + 1)
-        key = (bucket, width)
+        host, offsets, _, shape, patches = self._host_arrays(entries, width, bucket)
+        host, plans = self._prefix_plans(entries, host, offsets, shape, True)
+        self.prefix_steps += bool(plans)
+        key = (bucket, width, tuple(plans))
         rec = self._graphs.get(key)
         if rec is not None:
             # a replay reads the index buffer at the addresses of its capture: the arrays go there, nothing else is built
-            host, offsets, _, _, patches = self._host_arrays(entries, width, bucket)
             self._send(host, offsets, patches, device_tokens)
             rec = self._graphs.get(key)         # the send may have had to grow the buffer, which drops the captures
         if rec is None:
-            ctx = self._build(entries, table_width=width, device_tokens=device_tokens, pad_requests=bucket)
+            ctx = self._build(entries, table_width=width, device_tokens=device_tokens, pad_requests=bucket, plans=(host, offsets, plans))
             arena, saved, saved_views = {}, self._arena, self._views
             self._arena, self._views = arena, {}     # the capture's buffers are its own: eager steps do not write them
             try:
@@ -335,6 +384,7 @@ class ModelRunner:
                 ctx = None
             else:
                 ctx = self._build(entries, device_tokens=device_tokens)
+                self.prefix_steps += bool(ctx.prefix)
                 logits = self.model.forward(ctx)
         except BaseException:
             for e in entries:          # a failed step holds no pages beyond its committed tokens

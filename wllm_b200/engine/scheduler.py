@@ -41,13 +41,22 @@ Policy, with the reference's rule beside it:
               max_tokens and the model's length are known by count and waste nothing.
               A repetition penalty needs every earlier token on the host, and a shortage
               of pages is settled with nothing in flight: both read the tokens first.
+  prefixes    (no counterpart in the reference) tokens that several requests begin with are
+              computed once (`add_prefix`): they stand in the queue like a request, nothing
+              is sampled for them, and their pages and state stay.  A request that names a
+              prefix waits until it is ready and is admitted as a fork of it: it needs pages
+              for what lies behind the prefix's full pages only, and computes its other
+              tokens.  Preempted, it is forked again.  A prefix's own pages are given back
+              when it is dropped, or, if it was made for a few requests alone (`auto`), when
+              the last of them has finished.
 """
 from __future__ import annotations
 
 import random
 
 from ..cache import OutOfPages
-from .request import Request, RequestStatus
+from ..sampling.params import SamplingParams
+from .request import Prefix, Request, RequestStatus
 from .runner import StepEntry
 
 
@@ -67,6 +76,8 @@ class Scheduler:
         self.live: list = []          # admitted requests in order of admission
         self._rng = random.Random(seed)
         self.async_scheduling = async_scheduling
+        self.prefixes: list = []      # those that are not dropped
+        self._prefix_id = 0
         self._inflight = None         # (PendingSample, [(request, keep)]) of the step whose tokens are unread
         self.stats = {"steps": 0, "prefill_tokens": 0, "decode_tokens": 0, "preemptions": 0, "finished": 0,
                       "dropped_tokens": 0}
@@ -87,13 +98,66 @@ class Scheduler:
         if bad:
             raise ValueError(f"request {request.request_id!r}: token id {bad[0]} outside the vocabulary of {vocab}")
         worst = min(request.worst_case_tokens, self.max_model_len)
+        if request.prefix is not None:
+            begin = request.prefix.token_ids
+            if request.prefix.dropped or request.prefix not in self.prefixes:
+                raise ValueError(f"request {request.request_id!r}: its prefix was dropped, or is another engine's")
+            if n <= len(begin) or request.prompt_token_ids[:len(begin)] != begin:
+                raise ValueError(f"request {request.request_id!r}: a prompt that names a prefix begins with its {len(begin)} tokens and has more")
         pool = min(g.pool.num_pages for g in self.cache.groups) if self.cache.groups else 1 << 30
-        if self._pages(worst) > pool:
+        held = self._held_pages(request)
+        if self._pages(worst) + held > pool:
             raise ValueError(f"request {request.request_id!r}: {worst} tokens need {self._pages(worst)} pages, "
-                             f"the cache has {pool}; it could never finish")
+                             f"the cache has {pool}{f', {held} of them for prefixes' if held else ''}; it could never finish")
+        if request.prefix is not None:
+            request.prefix.users += 1
         request.status = RequestStatus.WAITING
         request.seed = request.sampling.seed if request.sampling.seed is not None else self._rng.getrandbits(63)
         self.waiting.append(request)
+
+    def _held_pages(self, request: Request | None = None) -> int:
+        """Pages that prefixes hold, or will, which `request` does not share: all of them, but the full pages of its own."""
+        total = 0
+        for x in self.prefixes:
+            if x.holder is request:
+                continue
+            shared = len(x.holder.prefix.token_ids) // self.cache.page_size if x.holder.prefix is not None else 0
+            total += self._pages(len(x.token_ids)) - shared
+        if request is not None and request.prefix is not None:
+            total -= len(request.prefix.token_ids) // self.cache.page_size
+        return total
+
+    def add_prefix(self, token_ids, prefix: Prefix | None = None, auto: bool = False) -> Prefix:
+        """Tokens for requests to begin with; `prefix`: one that they themselves begin with.  They are computed by the steps to come."""
+        holder = Request(("prefix", self._prefix_id), list(token_ids), SamplingParams(max_tokens=1), prefix=prefix, holds=True)
+        self.add_request(holder)
+        self._prefix_id += 1
+        made = Prefix(holder.prompt_token_ids, holder, auto)
+        self.prefixes.append(made)
+        return made
+
+    def drop_prefix(self, prefix: Prefix) -> None:
+        """Give a prefix's pages back (requests that were forked from it keep theirs)."""
+        if prefix.dropped:
+            raise ValueError("the prefix was dropped before")
+        if prefix.users:
+            raise ValueError(f"{prefix.users} unfinished requests begin with the prefix")
+        holder = prefix.holder
+        self.waiting = [r for r in self.waiting if r is not holder]
+        self.live = [r for r in self.live if r is not holder]
+        self.prefixes.remove(prefix)
+        prefix.dropped = True
+        self._release(holder)
+        holder.status, holder.finish_reason = RequestStatus.FINISHED, "dropped"
+        self._leave(holder)
+
+    def _leave(self, r: Request) -> None:
+        """A request that is over no longer keeps its prefix."""
+        prefix, r.prefix = r.prefix, None
+        if prefix is not None:
+            prefix.users -= 1
+            if prefix.auto and prefix.users == 0 and not prefix.dropped:
+                self.drop_prefix(prefix)
 
     def has_unfinished(self) -> bool:
         return bool(self.waiting or self.live or self._inflight)
@@ -101,15 +165,17 @@ class Scheduler:
     def cancel(self, request_id) -> bool:
         """Stop a request wherever it is and give back what it holds (scheduler.py:158-176)."""
         for r in self.live:
-            if r.request_id == request_id:
+            if r.request_id == request_id and not r.holds:
                 self._release(r)
                 self.live.remove(r)
                 r.status, r.finish_reason = RequestStatus.FINISHED, "cancelled"
+                self._leave(r)
                 return True
         for r in self.waiting:
-            if r.request_id == request_id:
+            if r.request_id == request_id and not r.holds:
                 self.waiting.remove(r)
                 r.status, r.finish_reason = RequestStatus.FINISHED, "cancelled"
+                self._leave(r)
                 return True
         return False
 
@@ -131,12 +197,15 @@ class Scheduler:
         return total
 
     def _may_admit(self, r: Request, taken_now: int) -> bool:
-        if len(self.live) >= self.max_num_seqs:
+        if len(self.live) >= self.max_num_seqs or self.cache.slots.num_free == 0:
             return False
+        if r.prefix is not None and not r.prefix.ready:
+            return False
+        shared = len(r.prefix.token_ids) // self.cache.page_size if r.prefix is not None else 0
         free = min(self.cache.free_pages(), default=1 << 30)
         if self.admission == "worst_case":   # the pledge covers the pages this step is about to take
-            return self._pages(min(r.worst_case_tokens, self.max_model_len)) <= free - self._pledged()
-        return self._pages(r.num_tokens) <= free - taken_now
+            return self._pages(min(r.worst_case_tokens, self.max_model_len)) - shared <= free - self._pledged()
+        return self._pages(r.num_tokens) - shared <= free - taken_now
 
     def _preempt_youngest(self) -> Request:
         victim = self.live.pop()
@@ -191,14 +260,14 @@ class Scheduler:
             if not self._may_admit(r, taken):
                 break                                       # the head of the queue blocks the rest
             self.waiting.pop(0)
-            r.cache = self.cache.open(r.request_id)
-            r.num_computed = 0
+            r.cache = self.cache.open(r.request_id) if r.prefix is None else self.cache.fork(r.prefix.holder.cache, r.request_id)
+            r.num_computed = r.cache.num_tokens
             r.status = RequestStatus.PREFILLING
             self.live.append(r)
-            c = min(budget, r.num_tokens)
+            c = min(budget, r.num_tokens - r.num_computed)
             budget -= c
-            plan.append((r, 0, c))
-            taken += self._pages(c)
+            plan.append((r, r.num_computed, c))
+            taken += self._pages(r.num_computed + c) - len(r.cache.tables[0] if r.cache.tables else ())
         return plan
 
     def _resolve(self) -> list:
@@ -219,14 +288,19 @@ class Scheduler:
         self._finish()
         return got
 
+    def largest_need(self) -> int:
+        """Pages that the largest unfinished request may come to hold, beside what prefixes do."""
+        return max((self._pages(min(r.worst_case_tokens, self.max_model_len)) + self._held_pages(r) for r in self.waiting + self.live), default=self._held_pages())
+
     def _finish(self) -> None:
         for r in [r for r in self.live if r.finished]:
             self._release(r)
             self.live.remove(r)
+            self._leave(r)
             self.stats["finished"] += 1
 
     def _entry(self, r: Request, start: int, c: int) -> StepEntry:
-        want = [c - 1] if start + c == r.num_tokens + r.inflight else []
+        want = [c - 1] if start + c == r.num_tokens + r.inflight and not r.holds else []
         if r.inflight:
             return StepEntry(r.cache, [0], want, device_row=r.inflight_row)
         return StepEntry(r.cache, r.tokens(start, start + c), want)
@@ -270,7 +344,11 @@ class Scheduler:
                 self.stats["prefill_tokens"] += c
             r.num_computed = start + c
             if r.num_computed == r.num_tokens + r.inflight:
-                sampled.append(r)
+                if r.holds:
+                    r.status = RequestStatus.HELD
+                    self.live.remove(r)
+                else:
+                    sampled.append(r)
         args = ([r.sampling for r in sampled], [len(r.output_token_ids) + r.inflight for r in sampled],
                 [r.seed for r in sampled], [r.seen for r in sampled])
         if not self.async_scheduling:

@@ -779,7 +779,9 @@ class PrefixPlan:
     """How a batch whose requests share pages is attended to (csrc/prefix_plan.cuh): made once for a step and a layout of heads, read by every layer of it."""
     __slots__ = ("key", "requests", "width", "n_tokens", "host", "used", "items", "rows", "saved_keys", "most_results", "tiles", "max_chunks", "scratch_floats", "launch", "places")
 
-    def __init__(self, key: tuple, requests: int, width: int, host: torch.Tensor, used: int, items: int, rows: int, saved: int, most: int, tiles: int, n_tokens: int, max_ctx: int):
+    def __init__(self, key: tuple, requests: int, width: int, caps, host: torch.Tensor, used: int, items: int, rows: int, saved: int, most: int, tiles: int, n_tokens: int, max_ctx: int):
+        if caps is not None:          # laid out for any plan of that size: the kernels read from it how many items there are
+            n_tokens, rows, max_ctx = caps[3], caps[2] * (key[1] // key[2]), width * key[0]
         self.key, self.requests, self.width, self.n_tokens = key, requests, width, n_tokens
         self.host = host[:used]                # int32 on the host, pinned where there is a device
         self.used, self.items, self.rows, self.saved_keys, self.most_results, self.tiles = used, items, rows, saved, most, tiles
@@ -787,8 +789,9 @@ class PrefixPlan:
         self.max_chunks = max(1, -(-max_ctx // SIMT_CHUNK))
         self.scratch_floats = nkv * rows * (vd + 2) if dtype == torch.bfloat16 else n_tokens * nq * self.max_chunks * (vd + 2)
         # what the native call takes of it
-        self.launch = (n_tokens, requests, width, used, self.scratch_floats, rows, items * nkv, int(host[6]) if used else 0, self.max_chunks, nq, nkv, hd, vd, page_size)
-        self.places = (int(host[2]), int(host[3]), items) if used else (0, 0, 0)
+        pairs = (items if caps is None else caps[0]) * nkv
+        self.launch = (n_tokens, requests, width, used, self.scratch_floats, rows, pairs, int(host[6]) if used else 0, self.max_chunks, nq, nkv, hd, vd, page_size)
+        self.places = (int(host[2]), int(host[3]), items if caps is None else -1) if used else (0, 0, 0)
 
     def to(self, device) -> torch.Tensor:
         """The plan's array on the device, as prefix_attention takes it (in the current stream's order)."""
@@ -821,21 +824,39 @@ def prefix_ok(nq: int, nkv: int, hd: int, vd: int, page_size: int, dtype: torch.
         0 < hd <= 256 and hd % 8 == 0 and 0 < vd <= 256 and vd % 8 == 0 and page_size >= 16 and page_size & (page_size - 1) == 0
 
 
+def prefix_pays(saved_keys: int, nkv: int, hd: int, vd: int, dtype: torch.dtype) -> bool:
+    """Whether a step reads shared keys once for all, from the keys (times further holders) that it then reads less often."""
+    item = 2 if dtype == torch.bfloat16 else 4
+    return saved_keys * nkv * (hd + vd) * item >= PREFIX_SAVED[item]
+
+
+PREFIX_SAVED = {2: 24 << 20, 4: 4 << 20}
+
+
+def prefix_caps(requests: int, nkv: int) -> tuple:
+    """Sizes that the plan of a captured step of that many requests is laid out for (one token each): items for two turns of every multiprocessor beside four a request."""
+    return 2 * sm_count() // nkv + 4 * requests, 6 * requests, 24 * requests + 512, requests
+
+
 def prefix_plan(tables, q_lens, ctx_lens, page_size: int, nq: int, nkv: int, hd: int, vd: int | None = None, dtype: torch.dtype = torch.bfloat16,
-                min_keys: int = PREFIX_MIN_KEYS) -> PrefixPlan:
+                min_keys: int = PREFIX_MIN_KEYS, caps: tuple | None = None) -> PrefixPlan | None:
     """The plan of a batch's attention, from what the host knows of it: `tables` [requests, pages] (int32; an array or a tensor of the CPU), the requests' new tokens and contexts
     (those included).  The batch's tokens stand request by request.  Requests that hold the same page at the same place share its keys and those in front of it; stretches of fewer than
-    `min_keys` shared keys are left to each request.  A plan holds for any pools and any queries of these tables and lengths."""
+    `min_keys` shared keys are left to each request.  A plan holds for any pools and any queries of these tables and lengths.
+    `caps` (items, tokens of items, results, tokens of the batch): the array is laid out for that many, so that a captured call serves every plan of the same caps whose array is put in the
+    same place; None comes back when the batch needs more (or has other than that many tokens at most)."""
     vd = hd if vd is None else vd
     if not prefix_ok(nq, nkv, hd, vd, page_size, dtype):
         raise KernelError(f"prefix_plan: {nq} query heads on {nkv}, sizes {hd}/{vd}, pages of {page_size}, {dtype}: up to 128 query heads a key/value head in bfloat16, 32 in float32, "
                           "head sizes in steps of 8 up to 256, pages of a power of two of at least 16 tokens")
     bf16 = dtype == torch.bfloat16
     status, *made = _host_calls().prefix_plan(tables, _numbers(q_lens), _numbers(ctx_lens), page_size, nq // nkv, nkv, prefix_rows(dtype), 128 if bf16 else SIMT_CHUNK,
-                                              1 if bf16 else SIMT_CHUNK, max(1, min_keys), sm_count() if bf16 else 2 * sm_count(), torch.cuda.is_available(), _prefix_costs(dtype, hd, vd))
+                                              1 if bf16 else SIMT_CHUNK, max(1, min_keys), sm_count() if bf16 else 2 * sm_count(), torch.cuda.is_available(), _prefix_costs(dtype, hd, vd), (0, 0, 0, 0) if caps is None else caps)
+    if status == 2 and caps is not None:
+        return None
     if status:
         raise KernelError(f"prefix_plan: {_STATUS.get(status, status)}")
-    return PrefixPlan((page_size, nq, nkv, hd, vd, dtype), tables.shape[0], tables.shape[1], *made)
+    return PrefixPlan((page_size, nq, nkv, hd, vd, dtype), tables.shape[0], tables.shape[1], caps, *made)
 
 
 def prefix_attention(q, out, k_pages, v_pages, block_table, plan: PrefixPlan, arrays: torch.Tensor, nq: int, nkv: int, hd: int, page_size: int, scale: float, scratch: torch.Tensor,

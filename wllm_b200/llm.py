@@ -8,16 +8,24 @@ load_native, KVCacheManager, Scheduler, add_request and run_to_completion
 (tests/test_gemma_architecture.py:119-124).  `LLM` wraps that assembly, with the
 reference's option names: num_blocks, block_size, dtype, chunked_prefill_tokens,
 cuda_graphs (src/wllm/cli.py:30-35).  `add_request` / `step` expose the loop itself.
+
+What several requests begin with is computed once, and attended to once a step for all of them:
+
+    system = llm.add_prefix([2, 651, 6037, ...])
+    outs = llm.generate([[108, 17], [99]], SamplingParams(max_tokens=32), prefix=system)   # prompts behind the prefix
+    outs = llm.generate([[2, 651, 6037]], SamplingParams(temperature=0.8, n=4))            # four samples of one prompt
+    llm.drop_prefix(system)
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 from .config import EngineConfig
 from .engine.build import build_model, build_runner
-from .engine.request import Request
+from .engine.request import Prefix, Request
 from .engine.scheduler import Scheduler
 from .sampling import SamplingParams
+from .sampling.params import sample_seed
 from .sampling.sampler import Sampler
 
 
@@ -29,6 +37,7 @@ class RequestOutput:
     logprobs: list
     finish_reason: str | None
     preemptions: int = 0
+    sample: int = 0               # which of its prompt's n samples it is
 
 
 class LLM:
@@ -55,12 +64,51 @@ class LLM:
         self.eos_token_id = self.model.plan.eos_token_id
         self._next_id = 0
 
-    def add_request(self, prompt_token_ids, sampling_params: SamplingParams | None = None, request_id=None) -> Request:
+    def add_prefix(self, token_ids) -> Prefix:
+        """Tokens for requests to begin with (a system prompt, a document): computed once, by the steps to come, and kept until they are dropped."""
+        return self.scheduler.add_prefix(token_ids)
+
+    def drop_prefix(self, prefix: Prefix) -> None:
+        """Give a prefix's pages back; every request that begins with it has finished."""
+        self.scheduler.drop_prefix(prefix)
+
+    def resize_cache(self, num_blocks: int) -> None:
+        """Another number of cache blocks: what is live moves to the front of the new pools.  Refused where a request that was taken on could not finish."""
+        need = self.scheduler.largest_need()
+        if need > num_blocks:
+            raise ValueError(f"{num_blocks} blocks: the requests and prefixes at hand need {need}")
+        self.runner.resize_cache(num_blocks)
+        self.engine_config.num_blocks = num_blocks
+
+    def add_request(self, prompt_token_ids, sampling_params: SamplingParams | None = None, request_id=None, prefix: Prefix | None = None):
+        """`prefix`: what the prompt begins with; `prompt_token_ids` are the tokens behind it.  The request, or with n > 1 the list of its n samples' requests, whose
+        ids are (request_id, sample)."""
         if request_id is None:
             request_id = self._next_id
             self._next_id += 1
-        req = Request(request_id, list(prompt_token_ids), sampling_params or SamplingParams(),
-                      eos_token_id=self.eos_token_id)
+        sp = sampling_params or SamplingParams()
+        prompt = (list(prefix.token_ids) if prefix is not None else []) + list(prompt_token_ids)
+        if sp.n == 1:
+            return self._add(request_id, prompt, sp, prefix)
+        begin = prefix
+        if len(prompt) > 1 + (len(prefix.token_ids) if prefix is not None else 0):
+            # the samples are forks of the prompt without its last token, which each of them runs for its own first draw
+            begin = self.scheduler.add_prefix(prompt[:-1], prefix=prefix, auto=True)
+        one = [replace(sp, n=1, seed=None if sp.seed is None else sample_seed(sp.seed, k)) for k in range(sp.n)]
+        made = []
+        try:
+            for k in range(sp.n):
+                made.append(self._add((request_id, k), prompt, one[k], begin))
+        except BaseException:
+            for r in made:
+                self.scheduler.cancel(r.request_id)
+            if begin is not prefix and not made:
+                self.scheduler.drop_prefix(begin)
+            raise
+        return made
+
+    def _add(self, request_id, prompt: list, sampling: SamplingParams, prefix) -> Request:
+        req = Request(request_id, prompt, sampling, eos_token_id=self.eos_token_id, prefix=prefix)
         self.scheduler.add_request(req)
         return req
 
@@ -72,17 +120,21 @@ class LLM:
     def has_unfinished(self) -> bool:
         return self.scheduler.has_unfinished()
 
-    def generate(self, prompts, sampling_params=None) -> list:
-        """Generate for a batch of prompts (lists of token ids); results in the order of the prompts."""
+    def generate(self, prompts, sampling_params=None, prefix: Prefix | None = None) -> list:
+        """Generate for a batch of prompts (lists of token ids); results in the order of the prompts, a prompt's n samples one behind the other.  `prefix`: what all of them
+        begin with; the prompts are the tokens behind it."""
         prompts = [list(p) for p in prompts]
         if sampling_params is None or isinstance(sampling_params, SamplingParams):
             sampling_params = [sampling_params or SamplingParams()] * len(prompts)
         if len(sampling_params) != len(prompts):
             raise ValueError("one SamplingParams for all prompts, or one per prompt")
-        reqs = [self.add_request(p, sp) for p, sp in zip(prompts, sampling_params)]
+        reqs = []
+        for p, sp in zip(prompts, sampling_params):
+            made = self.add_request(p, sp, prefix=prefix)
+            reqs += enumerate(made) if isinstance(made, list) else [(0, made)]
         self.scheduler.run_to_completion()
         return [RequestOutput(r.request_id, r.prompt_token_ids, list(r.output_token_ids), list(r.logprobs),
-                              r.finish_reason, r.preemptions) for r in reqs]
+                              r.finish_reason, r.preemptions, sample) for sample, r in reqs]
 
     @property
     def stats(self) -> dict:

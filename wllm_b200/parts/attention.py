@@ -46,7 +46,8 @@ projection (a mixer that projects two mixers' heads at once).
 One forward serves whole prompts, portions and decoded tokens alike: the step's keys
 and values go into the pages first, then every token attends through its request's
 block table.  Which kernels do that is decided here, from the step context's facts
-about the batch: 32-bit (and head sizes the tensor-core kernels are not built for)
+about the batch: where requests share enough pages (forked ones, those behind one prefix), the kernels that read a
+shared page once for all of its holders, of both types; else 32-bit (and head sizes the tensor-core kernels are not built for)
 runs the one-warp-per-row kernel, by row or by row and chunk of keys; bfloat16 sends
 requests with one token to the split-key decode kernel and the others to the tiled
 prefill kernel, which find their requests by q_len on the device.
@@ -137,6 +138,11 @@ class PagedAttention:
 
     def cache_need(self):
         return KVNeed(self.nkv, self.hd, self.window, self.vd if self.vd != self.hd else None, self.keep_first, blocks=self.blocks)
+
+    def prefix_layout(self, page_size: int):
+        """(query heads, kv heads, key size, value size) for which pages that several requests hold may be read once for all of them, or None (a window, sizes that it is not built for)."""
+        ok = not self.window and ops.prefix_ok(self.nq, self.nkv, self.hd, self.vd, page_size, self.model_dtype)
+        return (self.nq, self.nkv, self.hd, self.vd) if ok else None
 
     def param_specs(self):
         H, n = self.hidden_size, self.names
@@ -284,6 +290,13 @@ class PagedAttention:
         nq, nkv, hd, scale = self.nq, self.nkv, self.hd, self.scale
         window = -self.window if self.blocks else (self.window or 0)     # the kernels take a block size as a negative window
         ps, table = ctx.cache.page_size, ctx.group_tables[group]
+        shared = None if window else getattr(ctx, "prefix", {}).get((group, nq, nkv, hd, self.vd))
+        if shared is not None:
+            plan, arrays = shared
+            floats = (plan.scratch_floats + (1 << 20) - 1) >> 20 << 20       # (whole 4 MB, so that growing contexts seldom ask for more)
+            scratch = ctx.buffer(self.tag + "attention_prefix", (floats,), torch.float32)
+            ops.prefix_attention(q, out, k_pages, v_pages, table, plan, arrays, nq, nkv, hd, ps, scale, scratch, vd=self.vd, sinks=self.sinks, cap=self.softcap, slopes=self.slopes)
+            return
         if q.dtype != torch.bfloat16 or not ops.mma_head_dim_ok(hd) or self.general:
             # Kernels with one result, bit for bit, so the choice is one of speed alone.  Portions of prompts:
             # 32 rows of a request share every tile of keys (few tiles without a window: chunk of keys by chunk).  Few rows over long contexts (decoding): a warp per

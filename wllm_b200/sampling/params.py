@@ -7,7 +7,7 @@ draws the same tokens whatever else is in the batch and however its prompt was c
 because the draw for output place i depends on (seed, i) only.  The rest are the
 request-level fields the reference keeps on its Sequence
 (src/wllm/engine/sequence.py:25-27): max_tokens (max_new_tokens), stop_token_ids, and
-ignore_eos (ours).
+ignore_eos and n (ours).
 """
 from __future__ import annotations
 
@@ -25,6 +25,7 @@ class SamplingParams:
     max_tokens: int = 16
     stop_token_ids: tuple = ()
     ignore_eos: bool = False
+    n: int = 1                    # continuations of the prompt, which is computed once for all of them
 
     def __post_init__(self):
         if self.temperature < 0:
@@ -39,11 +40,18 @@ class SamplingParams:
             raise ValueError("repetition_penalty must be > 0 (1 = off)")
         if self.max_tokens < 1:
             raise ValueError("max_tokens must be at least 1")
+        if self.n < 1:
+            raise ValueError("n must be at least 1")
         object.__setattr__(self, "stop_token_ids", tuple(self.stop_token_ids))
 
     @property
     def greedy(self) -> bool:
         return self.temperature == 0.0
+
+
+def sample_seed(seed: int, sample: int) -> int:
+    """The seed of a seeded prompt's sample: its first sample draws as a request of its own with that seed would, the others by seeds apart from it."""
+    return (seed + 0xD1B54A32D192ED03 * sample) & ((1 << 63) - 1) if sample else seed
 
 
 _MASK = (1 << 64) - 1

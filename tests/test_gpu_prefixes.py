@@ -121,7 +121,8 @@ def test_captured_steps_of_changing_batches(tmp_path, always):
         llm.drop_prefix(prefix)
         want = plain.generate([r.prompt_token_ids for r in reqs], sp)
         assert [r.output_token_ids for r in reqs] == [o.token_ids for o in want]
-    assert any(key[2] for key in llm.runner._graphs) and any(not key[2] for key in llm.runner._graphs)
+    assert llm.runner._graphs and llm.runner._prefix_graphs
+    assert all(rec["meta"] is llm.runner._meta for g in (llm.runner._graphs, llm.runner._prefix_graphs) for rec in g.values())
 
 
 def test_the_command(tmp_path, capsys):

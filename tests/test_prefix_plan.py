@@ -39,9 +39,12 @@ def check(plan, tables, q_lens, ctx_lens, ps, rep, tile_rows, align):
                 seen[token][lo:top] += 1
             pages = range(lo // ps, -(-hi // ps))
             assert all(tables[request][p] == tables[owner[token]][p] for p in pages)     # the item's keys are the token's own
-            key = row + i * rep
-            assert key not in rows and key + rep <= plan.rows
-            rows[key] = (token, lo)
+            keys = 64 if tile_rows == 32 else 128
+            costs = ops._prefix_costs(torch.float32 if tile_rows == 32 else torch.bfloat16, 8, 8)
+            for side in range(costs[6] if count * rep <= costs[4] and hi - lo > keys else 1):
+                key = row + (side * count + i) * rep
+                assert key not in rows and key + rep <= plan.rows
+                rows[key] = (token, lo)
     assert all((s == 1).all() for s in seen)
     assert len(rows) == len(listed) and starts[0] == 0
     for t in range(n):

@@ -454,11 +454,11 @@ PyObject* copy_pages(Args v, Py_ssize_t n) {
     return both;
 }
 
-// tables, q_lens, ctx_lens, page_size, query heads a kv head, kv heads, rows of an item, keys of a tile, align, min_keys, CTAs at once, pinned memory, costs (six), caps (four)
+// tables, q_lens, ctx_lens, page_size, query heads a kv head, kv heads, rows of an item, keys of a tile, align, min_keys, CTAs at once, pinned memory, costs (seven), caps (four)
 //   -> (status, the plan's array, ints used, items, rows, keys saved, most results, tiles, tokens, longest context)
 PyObject* prefix_plan(Args v, Py_ssize_t n) {
     count(n, 14);
-    const std::vector<int> costs = numbers(v[12], "costs", 6), caps = numbers(v[13], "caps", 4);
+    const std::vector<int> costs = numbers(v[12], "costs", 7), caps = numbers(v[13], "caps", 4);
     struct View {
         Py_buffer b;
         bool held = false;

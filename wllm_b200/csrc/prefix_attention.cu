@@ -24,8 +24,10 @@
 // A warp without rows leaves the tensor core to multiply what lies there: row m of a product depends on row m of its operand alone, and such rows are stored nowhere.
 //
 // An item of up to 16 rows (a decoding request's own keys) would fill an eighth of such a tile, and its chain of waits (queries, scores, exponentials, output, each a round trip through
-// tensor memory) would be as long as a full one's.  There the eight warps multiply on mma.sync, straight from the ring: 16 keys of a tile each for the scores, an eighth of the values'
-// columns each for the output, with one barrier a tile.  8 x 8 requests on 4,000 keys, 16 heads of 256, half of whose items are such: see the table's figures below.
+// tensor memory) would be as long as a full one's.  There the warps multiply on mma.sync, straight from the ring: a warp takes its share of a tile's keys for the scores and of the values'
+// columns for the output, with one barrier a tile in between.  Such items are to run at the rate of the device's memory, 23 bytes a cycle and SM: a tile of 128 keys of 256 (128 KB, 5,600 cycles) is
+// worked off by all eight warps in 4,300.  A tile of smaller heads comes faster than one chain of latencies is gone through, so there each group takes every other tile on its own and leaves
+// a result of its own (96 requests' own 32,000 keys, heads of 128: 912 us by all warps together, 704 so; heads of 256: 449 and 434, but short items, 8 x 8 on 4,000, 113 and 124).
 //
 // Head sizes that are no multiple of 64 are widened to one in shared memory: a box copy that reaches past a row's end fills with zeros.  Boxes that hold none of an item's keys are not
 // copied; values behind its last key are cleared in shared memory before they are multiplied with their weight of zero (0 x NaN is no zero).
@@ -51,22 +53,26 @@ constexpr int STAGE = BN * (KW > VW ? KW : VW) * 2;
 constexpr int BUFS = VDP <= 128 ? 3 : 2;           // score buffers
 constexpr int THIN = 16;                           // rows of an item that runs on mma.sync
 constexpr int Q_BYTES = BM * HDP * 2;
-constexpr int SMALL = 2 * BM * 4 + BM * 4 + 2 * BM * 4 + 512;      // rows' positions, maxima that the groups hand over, sums of the second group, barriers
+constexpr int SMALL_FIXED = 2 * BM * 4 + BM * 4 + 2 * BM * 4 + 512;      // rows' positions, maxima that the groups hand over, sums of the second group, barriers
+// What the warps on a thin item's tile keep: by tile in turn weights [16][128] in bfloat16 and row maxima [16][warps]; sums [warps][16].  It lies behind the queries of 16 rows, the second group's
+// behind their second 64 columns; where there are none, both have memory of their own.
+constexpr int SIDES = KC == 1 ? 2 : 1, SIDE_WARPS = 8 / SIDES;       // tiles in work at once, warps each
+constexpr int THIN_M = 2 * THIN * BN * 2, THIN_L = THIN_M + 2 * THIN * SIDE_WARPS * 4, THIN_BYTES = THIN_L + SIDE_WARPS * THIN * 4;
+constexpr bool THIN_APART = HDP == 64;
+static_assert(THIN_BYTES <= (BM - THIN) * 128 && THIN_BYTES % 16 == 0, "behind the queries of 16 rows");
+constexpr int SMALL = SMALL_FIXED + (THIN_APART ? 2 * THIN_BYTES : 0);
 constexpr int MOST_STAGES = (227 * 1024 - Q_BYTES - SMALL) / STAGE;
 constexpr int STAGES = MOST_STAGES > 8 ? 8 : MOST_STAGES;
 static_assert(STAGES >= 2 && STAGES >= BUFS * VC, "when a tile's scores are there, what its values' stages held before has been used");
 constexpr int SMEM = Q_BYTES + STAGES * STAGE + SMALL;
-// what a thin item keeps where it has no queries (rows 16 .. 127 of their first 64 columns): weights [2][16][128] bfloat16, row maxima [2][16][8], sums [8][16]
-constexpr int THIN_P = THIN * 128, THIN_M = THIN_P + 2 * THIN * BN * 2, THIN_L = THIN_M + 2 * 8 * THIN * 4;
-static_assert(THIN_L + 8 * THIN * 4 <= BM * 128, "behind the queries of 16 rows");
 constexpr int THREADS = 128 + 256;
-// registers a thread: 168 at the launch; the groups that hold a row's 128 scores take what the other four warps leave (128 x 80 + 256 x 208 <= 384 x 168)
-constexpr int REGS_FEW = 80, REGS_MANY = 208;
+// registers a thread: 168 at the launch; the groups that hold a row's 128 scores take what the other four warps leave (128 x 56 + 256 x 224 <= 384 x 168)
+constexpr int REGS_FEW = 56, REGS_MANY = 224;
 static_assert(128 * REGS_FEW + 256 * REGS_MANY <= THREADS * 168, "a split of what the launch has");
 constexpr int S_COL = BUFS == 3 ? 128 : 256;
 constexpr float SLACK = 8.0f;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr uint32_t IDESC_S = umma_idesc(BM, BN, false, false), IDESC_PV = umma_idesc(BM, VW, false, true);
+constexpr uint32_t IDESC_S = umma_idesc(BM, BN, false, false), IDESC_PV = umma_idesc(BM, VW, false, true), IDESC_PV_ALL = umma_idesc(BM, VDP, false, true);
 enum { GAVE_UP_LOAD = 31, GAVE_UP_MMA = 32, GAVE_UP_SOFTMAX = 33, GAVE_UP_QUERIES = 34, NOT_ALIGNED = 35 };
 
 __device__ __forceinline__ float fast_exp2(float x) {       // ex2.approx: 2 ulp, exp2(-inf) = 0
@@ -208,8 +214,8 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
         const int4 a = at[0], b = at[1];
         return Item{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     };
-    // The plan was copied before the step's first kernel started: the first item is looked up while the kernel before this one may still run.  (The kernel behind this one starts when
-    // its CTAs leave: earlier, the merge's would crowd on the SMs that this launch leaves free.)
+    // The plan was copied before the step's first kernel started: the first item is looked up while the kernel before this one may still run.  (The kernel behind this one starts
+    // when its CTAs have left: let go any earlier, the merge's crowd on the SMs that this launch leaves free or is done with first; 64 on 8,192 20.6 us so, 24.4 let go at the roles' ends.)
     Item next = item_of(blockIdx.x);
     pdl_wait();
 
@@ -251,7 +257,7 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                                 tma_load_2d(dst + cb * (BN * 128) + (lane << box_shift) * 128, value ? &v_map : &k_map, full + 8 * s, c * width + cb * 64, row);
                     }
                 };
-                const int ahead = item.tokens * rep <= THIN ? 2 : BUFS;
+                const int ahead = item.tokens * rep <= THIN ? 2 : BUFS;          // (the scores of a thin item's next tile are worked out, or its other group begins, before a tile's output)
                 for (int n = 0; n < ahead && n < T && ok; ++n) load(n, false);
                 for (int n = 0; n < T && ok; ++n) {
                     load(n, true);
@@ -294,6 +300,17 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                 auto output = [&](int t, bool first) -> bool {       // O += P V
                     if (!mbar_wait(p_full + 8 * (t % BUFS), (t / BUFS) & 1)) return false;
                     const uint32_t pa = tmem + S_COL + t % BUFS * BN;
+                    if (VC == 2 && use % STAGES + 1 < STAGES) {      // both halves of the columns side by side in the ring: products of twice the width, the weights read once
+                        const int s = use % STAGES;
+                        if (!mbar_wait(full + 8 * s, (use / STAGES) & 1) || !mbar_wait(full + 8 * s + 8, ((use + 1) / STAGES) & 1)) return false;
+                        tc_fence_after();
+                        const uint32_t vb = v_lo + s * (STAGE >> 4);
+#pragma unroll
+                        for (int i = 0; i < BN / 16; ++i) mma_ts(tmem, pa + i * 8, vb + ((i * (16 * 128)) >> 4), IDESC_PV_ALL, first && i == 0 ? 0u : 1u);
+                        hand_back(empty + 8 * s);
+                        hand_back(empty + 8 * s + 8);
+                        use += 2;
+                    } else
 #pragma unroll
                     for (int c = 0; c < VC; ++c, ++use) {
                         const int s = use % STAGES;
@@ -380,19 +397,20 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
             if (!__all_sync(0xffffffffu, mbar_wait(q_full, k & 1))) ok = false;
             if (rows <= THIN) {
                 // ---- up to 16 rows: mma.sync; this thread holds parts of rows lane / 4 and lane / 4 + 8 ----
-                // A warp weighs its 16 keys of a tile relative to a maximum of its own, rounded up to a whole number: what brings its weights to the maximum of all warps is a power of
-                // two then, by which bfloat16 weights are multiplied without a rounding when the output's products read them.  So the warps meet once a tile, with the next tile's scores
-                // worked out in between.
-                const int w = warp - 4, a_row = lane & 15, a_chunk = lane >> 4;
-                static_assert((VW / 8) % (VDP / 64) == 0, "a warp's value columns lie in one stage");
-                constexpr int NT = VDP / 64, STEPS = (HD + 15) / 16;   // this warp's blocks of 8 value columns: w * NT ...; products of 16 of the head's columns
+                // A warp weighs its 32 keys of a tile relative to a maximum of its own, rounded up to a whole number: what brings its weights to the maximum of the group's warps is a power
+                // of two then, by which bfloat16 weights are multiplied without a rounding when the output's products read them.  So the warps meet once a tile.
+                // this warp's blocks of 8 value columns: w * NT ...; its keys in blocks of 16; products of 16 of the head's columns
+                constexpr int NT = VDP / 8 / SIDE_WARPS, KB = BN / SIDE_WARPS / 16, STEPS = (HD + 15) / 16;
+                static_assert((VW / 8) % NT == 0, "a warp's value columns lie in one stage");
+                const int side = SIDES == 2 ? group : 0, w = SIDES == 2 ? quarter : warp - 4, a_row = lane & 15, a_chunk = lane >> 4;
+                const int scratch = THIN_APART ? (int)(bars - base) + 512 + side * THIN_BYTES : THIN * 128 + side * (BM * 128);
                 uint32_t qf[STEPS][4];
 #pragma unroll
                 for (int i = 0; i < STEPS; ++i) {
                     const int c = i * 2 + a_chunk;
                     ldsm4(q_s + (c >> 3) * (BM * 128) + a_row * 128 + (((c ^ a_row) & 7) << 4), qf[i]);
                 }
-                float o[NT][4], sv[2][4], mw[2] = {-INFINITY, -INFINITY}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope2[2];
+                float o[NT][4], mw[2] = {-INFINITY, -INFINITY}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope2[2];
                 int last[2], pos[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -410,52 +428,76 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                 }
 #pragma unroll
                 for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-                volatile float* mx_all = reinterpret_cast<volatile float*>(smem + THIN_M);
-                volatile float* l_all = reinterpret_cast<volatile float*>(smem + THIN_L);
-                auto scores = [&]() {                            // of this warp's 16 keys of the next tile
-                    const int b_row = w * 16 + (lane & 7) + (lane >> 4) * 8, b_chunk = (lane >> 3) & 1;
-                    float even[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, odd[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-                    for (int c = 0; c < KC; ++c, ++use) {
-                        const int s = use % STAGES;
-                        if (ok && !__all_sync(0xffffffffu, mbar_wait(full + 8 * s, (use / STAGES) & 1))) ok = false;
-                        const uint32_t kb = ring + s * STAGE;
-                        // (64 columns' fragments at once: a load's latency is that of the two products behind it)
-#pragma unroll
-                        for (int i0 = 0; i0 < KW / 16; i0 += 4) {
-                            uint32_t b[4][4];
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                if (c * KW + (i0 + u) * 16 >= HD) continue;
-                                const int ka = (i0 + u) * 2 + b_chunk;
-                                ldsm4(kb + (ka >> 3) * (BN * 128) + b_row * 128 + (((ka ^ b_row) & 7) << 4), b[u]);
-                            }
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                if (c * KW + (i0 + u) * 16 >= HD) continue;
-                                mma16816(u & 1 ? odd[0] : even[0], qf[c * (KW / 16) + i0 + u], b[u][0], b[u][1]);
-                                mma16816(u & 1 ? odd[1] : even[1], qf[c * (KW / 16) + i0 + u], b[u][2], b[u][3]);
-                            }
-                        }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(empty + 8 * s);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sv[j][e] = even[j][e] + odd[j][e];
+                volatile float* mx_all = reinterpret_cast<volatile float*>(smem + scratch + THIN_M);
+                volatile float* l_all = reinterpret_cast<volatile float*>(smem + scratch + THIN_L);
+                const int begin = use;
+                // Every warp passes every stage, one by one, and hands each back, the other group's as soon as they are there: a warp that left some out could be overtaken by two rounds of
+                // a stage, which a wait cannot tell from none.
+                auto landed = [&]() { if (ok && !__all_sync(0xffffffffu, mbar_wait(full + 8 * (use % STAGES), (use / STAGES) & 1))) ok = false; };
+                auto handed = [&]() {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(empty + 8 * (use % STAGES));
+                    ++use;
+                };
+                auto there = [&](int at) {
+                    if (SIDES == 2)
+                        while (use < at) { landed(); handed(); }
+                    landed();
                 };
                 auto power = [](float d) { return d < -126.f ? 0u : (uint32_t)(127 + (int)d) << 23; };      // 2^d for a whole d <= 0, as the bits of a float
-                scores();
-                for (int n = 0; n < T; ++n) {
-                    const int key0 = lo + n * BN;
-                    const uint32_t p_s = q_s + THIN_P + (n & 1) * (THIN * BN * 2);
+                // the scores of this warp's keys of tile n; stages come as K 0, K 1, V 0, K 2, V 1, ...
+                float sv[2 * KB][4];
+                auto scores = [&](int n) {
+                    float odd[2 * KB][4];                        // (two chains of products a score: steps of 16 columns in turn)
+#pragma unroll
+                    for (int j = 0; j < 2 * KB; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sv[j][e] = odd[j][e] = 0.f;
+                    const int k_at = begin + n * KC + max(n - 1, 0) * VC;
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) {
+                        there(k_at + c);
+                        const int s = use % STAGES;
+                        const uint32_t kb = ring + s * STAGE;
+#pragma unroll
+                        for (int i0 = 0; i0 < KW / 16; i0 += 4 / KB) {       // (four fragments at once: a load's latency is that of the products behind it)
+                            uint32_t b[4 / KB][KB][4];
+#pragma unroll
+                            for (int u = 0; u < 4 / KB; ++u)
+#pragma unroll
+                                for (int h = 0; h < KB; ++h) {
+                                    if (c * KW + (i0 + u) * 16 >= HD) continue;
+                                    const int ka = (i0 + u) * 2 + ((lane >> 3) & 1), b_row = (w * KB + h) * 16 + (lane & 7) + (lane >> 4) * 8;
+                                    ldsm4(kb + (ka >> 3) * (BN * 128) + b_row * 128 + (((ka ^ b_row) & 7) << 4), b[u][h]);
+                                }
+#pragma unroll
+                            for (int u = 0; u < 4 / KB; ++u)
+#pragma unroll
+                                for (int h = 0; h < KB; ++h) {
+                                    if (c * KW + (i0 + u) * 16 >= HD) continue;
+                                    mma16816(u & 1 ? odd[2 * h] : sv[2 * h], qf[c * (KW / 16) + i0 + u], b[u][h][0], b[u][h][1]);
+                                    mma16816(u & 1 ? odd[2 * h + 1] : sv[2 * h + 1], qf[c * (KW / 16) + i0 + u], b[u][h][2], b[u][h][3]);
+                                }
+                        }
+                        handed();
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2 * KB; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sv[j][e] += odd[j][e];
+                };
+                if (SIDES == 1) scores(0);
+                for (int n = side; n < T; n += SIDES) {
+                    const int key0 = lo + n * BN, turn = (n / SIDES) & 1;
+                    const uint32_t p_s = base + scratch + turn * (THIN * BN * 2);
+                    if (SIDES == 2) scores(n);
+                    const int v_at = begin + min(T, n + 2) * KC + n * VC;
                     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < 2 * KB; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int i = e >> 1, key = key0 + w * 16 + j * 8 + (lane & 3) * 2 + (e & 1);
+                            const int i = e >> 1, key = key0 + w * KB * 16 + j * 8 + (lane & 3) * 2 + (e & 1);
                             float x = sv[j][e];
                             if (p.capl > 0.f) x = p.capl * (1.0f - __fdividef(2.0f, 1.0f + __expf(x * cap_in)));
                             else x *= p.scale2;
@@ -472,29 +514,34 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                         l[i] *= fast_exp2(mw[i] - from);
                         mw[i] = top;
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
+                        for (int j = 0; j < 2 * KB; ++j) {
                             const float e0 = fast_exp2(sv[j][2 * i] - from), e1 = fast_exp2(sv[j][2 * i + 1] - from);
                             l[i] += e0 + e1;
-                            asm volatile("st.shared.b32 [%0], %1;" ::"r"(p_s + r * (BN * 2) + (((w * 2 + j) ^ (r & 7)) << 4) + (lane & 3) * 4), "r"(pack_bf16(e0, e1)) : "memory");
+                            asm volatile("st.shared.b32 [%0], %1;" ::"r"(p_s + r * (BN * 2) + (((w * 2 * KB + j) ^ (r & 7)) << 4) + (lane & 3) * 4), "r"(pack_bf16(e0, e1)) : "memory");
                         }
-                        if ((lane & 3) == 0) mx_all[((n & 1) * THIN + r) * 8 + w] = top;
+                        if ((lane & 3) == 0) mx_all[(turn * THIN + r) * SIDE_WARPS + w] = top;
                     }
-                    if (n + 1 < T) scores();
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    if (SIDES == 1 && n + 1 < T) scores(n + 1);  // (while the others come to the barrier)
+                    if (SIDES == 1 || side == 0) asm volatile("bar.sync 2, %0;" ::"n"(SIDE_WARPS * 32) : "memory");
+                    else asm volatile("bar.sync 3, %0;" ::"n"(SIDE_WARPS * 32) : "memory");
                     // this warp's columns of the output
-                    uint32_t a[BN / 16][4], f[2][8];             // weights; what brings the warps' weights of the two rows to one reference, twice in a register
+                    uint32_t a[BN / 16][4], f[2][SIDE_WARPS];             // weights; what brings the warps' weights of the two rows to one reference, twice in a register
 #pragma unroll
                     for (int i = 0; i < BN / 16; ++i) ldsm4(p_s + a_row * (BN * 2) + (((i * 2 + a_chunk) ^ (a_row & 7)) << 4), a[i]);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float4* all = reinterpret_cast<const float4*>(smem + THIN_M) + ((n & 1) * THIN + (lane >> 2) + 8 * i) * 2;
-                        const float4 u = all[0], v = all[1];
-                        const float mj[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-                        const float top = fmaxf(max3(m[i], fmaxf(u.x, u.y), fmaxf(u.z, u.w)), max3(fmaxf(v.x, v.y), v.z, v.w)), from = top == -INFINITY ? 0.f : top;
-                        const float corr = __uint_as_float(power(m[i] - from));
+                        const float4* of_row = reinterpret_cast<const float4*>(smem + scratch + THIN_M) + (turn * THIN + (lane >> 2) + 8 * i) * (SIDE_WARPS / 4);
+                        float mj[SIDE_WARPS], top = m[i];
+#pragma unroll
+                        for (int j = 0; j < SIDE_WARPS / 4; ++j) {
+                            const float4 u = of_row[j];
+                            mj[4 * j] = u.x; mj[4 * j + 1] = u.y; mj[4 * j + 2] = u.z; mj[4 * j + 3] = u.w;
+                            top = max3(top, fmaxf(u.x, u.y), fmaxf(u.z, u.w));
+                        }
+                        const float from = top == -INFINITY ? 0.f : top, corr = __uint_as_float(power(m[i] - from));
                         m[i] = top;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) { const uint32_t x = power(mj[j] - from); f[i][j] = __byte_perm(x, x, 0x3232); }
+                        for (int j = 0; j < SIDE_WARPS; ++j) { const uint32_t x = power(mj[j] - from); f[i][j] = __byte_perm(x, x, 0x3232); }
 #pragma unroll
                         for (int j = 0; j < NT; ++j) { o[j][2 * i] *= corr; o[j][2 * i + 1] *= corr; }
                     }
@@ -502,15 +549,13 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                     for (int i = 0; i < BN / 16; ++i)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a[i][e]), *reinterpret_cast<__nv_bfloat162*>(&f[e & 1][i]));
+                            const __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a[i][e]), *reinterpret_cast<__nv_bfloat162*>(&f[e & 1][i / KB]));
                             a[i][e] = *reinterpret_cast<const uint32_t*>(&v);
                         }
-                    // (a warp's columns lie in one stage)
 #pragma unroll
-                    for (int c = 0; c < VC; ++c, ++use) {
-                        const int s = use % STAGES;
-                        if (ok && !__all_sync(0xffffffffu, mbar_wait(full + 8 * s, (use / STAGES) & 1))) ok = false;
-                        const int col0 = w * NT - c * (VW / 8);          // the first block's place in this chunk
+                    for (int c = 0; c < VC; ++c) {
+                        there(v_at + c);
+                        const int s = use % STAGES, col0 = w * NT - c * (VW / 8);      // the first block's place in this chunk
                         if (col0 >= 0 && col0 < VW / 8) {
                             const uint32_t vb = ring + s * STAGE;
                             if (key0 + BN > hi) {                // (slots behind the last key hold whatever lay there: 0 x NaN is no zero)
@@ -533,10 +578,10 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                                 for (int j = 0; j < NT; ++j) mma16816(o[j], a[i + 1], b[j][2], b[j][3]);
                             }
                         }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(empty + 8 * s);
+                        handed();
                     }
                 }
+                while (use < begin + T * (KC + VC)) { landed(); handed(); }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
@@ -547,20 +592,23 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                     if (!ok) atomicExch(p.status, GAVE_UP_SOFTMAX);
                     break;
                 }
+                if (side == 0 || T > 1) {                        // (the second group's results lie behind the first's)
+                    const int row0 = item.row + side * rows;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = (lane >> 2) + 8 * i;
-                    if (w == 0 && (lane & 3) == 0 && r < rows) {
-                        float sum = 0.f;
+                    for (int i = 0; i < 2; ++i) {
+                        const int r = (lane >> 2) + 8 * i;
+                        if (w == 0 && (lane & 3) == 0 && r < rows) {
+                            float sum = 0.f;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) sum += l_all[j * THIN + r];
-                        *reinterpret_cast<float2*>(p.part_ml + ((size_t)g * p.rows + item.row + r) * 2) = make_float2(m[i], sum);
-                    }
+                            for (int j = 0; j < SIDE_WARPS; ++j) sum += l_all[j * THIN + r];
+                            *reinterpret_cast<float2*>(p.part_ml + ((size_t)g * p.rows + row0 + r) * 2) = make_float2(m[i], sum);
+                        }
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const int col = w * NT + j;
-                        if (r < rows && col < VD / 8)
-                            *reinterpret_cast<float2*>(p.part_o + (((size_t)g * (VD / 8) + col) * p.rows + item.row + r) * 8 + (lane & 3) * 2) = make_float2(o[j][2 * i], o[j][2 * i + 1]);
+                        for (int j = 0; j < NT; ++j) {
+                            const int col = w * NT + j;
+                            if (r < rows && col < VD / 8)
+                                *reinterpret_cast<float2*>(p.part_o + (((size_t)g * (VD / 8) + col) * p.rows + row0 + r) * 8 + (lane & 3) * 2) = make_float2(o[j][2 * i], o[j][2 * i + 1]);
+                        }
                     }
                 }
                 __syncwarp();
@@ -819,6 +867,8 @@ static int pool_map(const void* ptr, long long rows, int box_rows, int head, CUt
 
 // Rows of an item at most.
 WLLM_API int wllm_prefix_attention_rows() { return BM; }
+// Results that an item of few rows leaves where it has several tiles of keys.
+WLLM_API int wllm_prefix_attention_sides() { return SIDES; }
 
 // The attention of a planned batch.  pool_pages: pages of the pools; n_tokens: rows of q and out; scratch: nkv * rows * (VD + 2) floats, rows as the plan has them (or the most that a plan of
 // this array may have); items_at, tokens_at: their places in the plan; n_items: its items, or -1: its header says; pairs: (item, kv head) pairs, or the most that there may be; ctas: SMs.  sinks, slopes: 32-bit [nq] or null; cap > 0: scores become cap tanh(score / cap).

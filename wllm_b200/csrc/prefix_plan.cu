@@ -64,7 +64,7 @@ struct Planner {
 };
 
 struct Tile { int token, tokens, key_lo, key_hi, request; bool own; };
-struct Item { int tile, key_lo, key_hi, row, cost; };
+struct Item { int tile, key_lo, key_hi, row, sides, cost; };
 
 long long padded(long long n) { return (n + 3) & ~3ll; }
 
@@ -73,7 +73,7 @@ long long padded(long long n) { return (n + 3) & ~3ll; }
 // tables [R][width] (pages that hold no key of a request are not looked at), q_len, ctx_len [R] on the host.  rep: query heads a key/value head; tile_rows: rows of an item at
 // most; key_tile: keys of a tile, whole tiles make an item's range; align: segments end at multiples of it; min_keys: no shared segment is shorter; pool_pages: one past the largest
 // page number; ctas: CTAs that run at once; costs: {a tile of keys, an item beside its tiles; the same two for items of at most `thin` rows; thin; a thousand rows of results and
-// kv heads}, in the caller's units; caps: {items, tokens, results, tokens of the batch} that the array is laid out for, zeros: what this plan needs (a captured
+// kv heads; results that a thin item of several tiles leaves}, in the caller's units; caps: {items, tokens, results, tokens of the batch} that the array is laid out for, zeros: what this plan needs (a captured
 // step's array lies at fixed places whatever the batch holds).  out [room]; info [8]: ints used, items, rows, shared keys saved (keys x further holders), most results of a
 // token, items that the batch has at the least.
 // Returns 0; 2: sizes that make no sense, or more than the caps hold; 4: `room` is too small (info[0] says what is needed); 7: a page number outside the pool.
@@ -162,7 +162,7 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             for (const Alike& a : alike) {
                 const int parts = parts_of(a.keys, a.thin, bound);
                 n += (long long)parts * a.count;
-                results_rows += parts * a.rows;
+                results_rows += parts * a.rows * (a.thin && a.keys > parts ? costs[6] : 1);
                 all += ((double)a.keys * costs[2 * a.thin] + (double)parts * costs[2 * a.thin + 1]) * a.count;
                 top = std::max(top, (double)((a.keys + parts - 1) / parts) * costs[2 * a.thin] + costs[2 * a.thin + 1]);
             }
@@ -184,9 +184,10 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             for (int s = 0; s < parts; ++s) {
                 const int from = (int)((long long)k * s / parts), to = (int)((long long)k * (s + 1) / parts);
                 for (size_t t = i; t < j; ++t) {
-                    items.push_back({(int)t, tiles[i].key_lo + from * key_tile, std::min(tiles[i].key_hi, tiles[i].key_lo + to * key_tile), (int)rows, (to - from) * costs[2 * is_thin(tiles[t])]});
-                    rows += (long long)tiles[t].tokens * rep;
-                    results += tiles[t].tokens;
+                    const int sides = is_thin(tiles[t]) && to - from > 1 ? costs[6] : 1;
+                    items.push_back({(int)t, tiles[i].key_lo + from * key_tile, std::min(tiles[i].key_hi, tiles[i].key_lo + to * key_tile), (int)rows, sides, (to - from) * costs[2 * is_thin(tiles[t])]});
+                    rows += (long long)tiles[t].tokens * rep * sides;
+                    results += tiles[t].tokens * sides;
                     if (rows > 0x7fffffff / nkv) return WLLM_BAD_SIZE;
                 }
             }
@@ -195,7 +196,7 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
         // results by token, in the order in which segments were found: ascending keys
         std::vector<int> starts(total + 1, 0), listed(results);
         for (const Item& it : items)
-            for (int t = 0; t < tiles[it.tile].tokens; ++t) ++starts[tokens[tiles[it.tile].token + t] + 1];
+            for (int t = 0; t < tiles[it.tile].tokens; ++t) starts[tokens[tiles[it.tile].token + t] + 1] += it.sides;
         int most_listed = 0;
         for (long long t = 0; t < total; ++t) {
             most_listed = std::max(most_listed, starts[t + 1]);
@@ -204,7 +205,8 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
         {
             std::vector<int> next(starts.begin(), starts.end() - 1);
             for (const Item& it : items)
-                for (int t = 0; t < tiles[it.tile].tokens; ++t) listed[next[tokens[tiles[it.tile].token + t]]++] = it.row + t * rep;
+                for (int t = 0; t < tiles[it.tile].tokens; ++t)
+                    for (int side = 0; side < it.sides; ++side) listed[next[tokens[tiles[it.tile].token + t]]++] = it.row + (side * tiles[it.tile].tokens + t) * rep;
         }
         std::stable_sort(items.begin(), items.end(), [](const Item& a, const Item& b) { return a.cost > b.cost; });
 

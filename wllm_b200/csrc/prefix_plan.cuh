@@ -5,6 +5,7 @@
 //              bound what they see (a request's own keys), first row of its results, first token of the batch if the others follow it one by one (else -1)
 //   tokens     2 each: a token of the batch, its position
 //   starts     by token of the batch (and one more): where its results are listed
+//              (an item of few rows and several tiles of keys may leave two results for a row, the second ones behind all the first)
 //   results    the first rows of a token's results, in ascending order of the keys that they stem from
 //   positions  by token of the batch
 // A row is a (token, query head of the group); a token's `rep` rows stand one behind the other.  Results of key/value head g lie `rows` further on than those of head g - 1.

@@ -79,8 +79,9 @@ class ModelRunner:
         self.h2d_bytes = 0
         self._tables: dict = {}        # cached int32 copies of block tables
         self._graphs_on = False
-        self._graphs: dict = {}        # (requests, table width, whether shared pages are attended to once) -> captured decode step
-        self.prefix_layouts = model.prefix_layouts(cache.page_size)
+        self._graphs: dict = {}        # (requests, table width) -> captured decode step
+        self._prefix_graphs: dict = {} # (requests, table width, layouts that attend to shared pages once) -> the same
+        self.prefix_layouts = model.prefix_layouts(cache.page_size) if hasattr(model, "prefix_layouts") else []
         self.prefix_steps = 0          # steps that attended to shared pages once for all of their holders
         self.graph_launches = 0        # kernel launches replayed from graphs so far
 
@@ -215,7 +216,7 @@ class ModelRunner:
         total = host.shape[0]
         if self._meta is None or self._meta.numel() < total:
             cap = max(total, 4096, 2 * (self._meta.numel() if self._meta is not None else 0))
-            self._graphs.clear()      # captured steps point into the old index buffer
+            self._drop_graphs()       # captured steps point into the old index buffer
             self._meta = torch.empty(cap, dtype=torch.int32, device=self.device)
         self._ring.send(host, self._meta)
         self.h2d_bytes = total * 4
@@ -306,8 +307,12 @@ class ModelRunner:
         try:
             self.cache.resize(num_pages)
         finally:
-            self._graphs.clear()
+            self._drop_graphs()
             self._tables.clear()
+
+    def _drop_graphs(self) -> None:
+        self._graphs.clear()
+        self._prefix_graphs.clear()
 
     # -- captured decode steps -------------------------------------------------------------
     def enable_graphs(self) -> None:
@@ -335,12 +340,12 @@ class ModelRunner:
         host, offsets, _, shape, patches = self._host_arrays(entries, width, bucket)
         host, plans = self._prefix_plans(entries, host, offsets, shape, True)
         self.prefix_steps += bool(plans)
-        key = (bucket, width, tuple(plans))
-        rec = self._graphs.get(key)
+        graphs, key = (self._prefix_graphs, (bucket, width, tuple(plans))) if plans else (self._graphs, (bucket, width))
+        rec = graphs.get(key)
         if rec is not None:
             # a replay reads the index buffer at the addresses of its capture: the arrays go there, nothing else is built
             self._send(host, offsets, patches, device_tokens)
-            rec = self._graphs.get(key)         # the send may have had to grow the buffer, which drops the captures
+            rec = graphs.get(key)               # the send may have had to grow the buffer, which drops the captures
         if rec is None:
             ctx = self._build(entries, table_width=width, device_tokens=device_tokens, pad_requests=bucket, plans=(host, offsets, plans))
             arena, saved, saved_views = {}, self._arena, self._views
@@ -362,7 +367,7 @@ class ModelRunner:
                 ops.launches = before
             finally:
                 self._arena, self._views = saved, saved_views
-            self._graphs[key] = rec
+            graphs[key] = rec
         rec["graph"].replay()
         self.graph_launches += rec["launches"]
         return rec["logits"][:len(entries)]

@@ -753,64 +753,168 @@ paged_attention_simt_chunk_kernel(const T* __restrict__ q, int q_stride, const T
 
 // --------------------------------------------------------------------------------------
 // items of a plan (prefix_plan.cuh), for batches whose requests share pages: up to 32 rows of any requests against a range of whole chunks, each chunk's results left where those of the
-// kernel above are.  The rows of all requests that hold a stretch of pages meet its keys together; a row's arithmetic is the walk's, so its bits are too.
+// kernel above are.  The rows of all requests that hold a stretch of pages meet its keys together.  A sum's terms and their order are the walk's, so its bits are too; which thread
+// adds up what is this kernel's own.  What bounds it is the FMA pipes and the reads of shared memory beside them, so a thread works out 4 rows x 2 keys of the scores (8 reads of a line
+// for 32 products, as long as these take; one key a thread was twice that) and 8 rows x 4 columns of the output (6), and two CTAs share an SM, so that one's products hide the other's waits.
+// 32 rows of 256 by 64 keys: 13.5 us of an SM as the kernel above does it, <measured> so.
 // --------------------------------------------------------------------------------------
+constexpr int PF_S = 68, PF_P = 36;            // rows of scores [32][68] and of weights [64][36] in shared memory
+
+static __host__ __device__ __forceinline__ int prefix_floats(int hd, int vd) { return TL_ROWS * (hd + 4) + CHUNK * (hd + 4 > vd ? hd + 4 : vd) + CHUNK * PF_P + TL_ROWS; }
+
 template <int NE>
 __global__ void __launch_bounds__(TL_WARPS * 32, 2)
 paged_attention_simt_prefix_kernel(const float* __restrict__ q, int q_stride, const float* __restrict__ k_pages, const float* __restrict__ v_pages, int pool_pages,
                                    const int* __restrict__ block_table, int max_pages, const int* __restrict__ plan, int nq, int nkv, int hd, int page_size, float scale, int vd,
                                    float cap, const float* __restrict__ slopes, float* __restrict__ scratch, int max_chunks) {
-    extern __shared__ __align__(16) unsigned char tl_smem[];
-    __shared__ size_t row_of[CHUNK], q_of[TL_ROWS];
-    pdl_wait();                          // (the merge's CTAs would crowd on the SMs that this launch leaves free)
-    const int rep = nq / nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, total = plan[PLAN_ITEMS] * nkv;
-    float* qs = reinterpret_cast<float*>(tl_smem);                          // [32 rows][hd]
-    float* ks = qs + TL_ROWS * hd;                                          // [32 keys][hd + 4]
-    float* vs = ks + 32 * (hd + Vec<float>::N);                             // [32 keys][vd]
+    constexpr int RT = NE, DG = 8 * NE;        // rows of the output a thread, threads along its columns (4 each)
+    extern __shared__ __align__(16) float pf_smem[];
+    __shared__ int row_of[CHUNK];              // the chunk's keys in the pools
+    __shared__ int token_of[TL_ROWS], pos_of[TL_ROWS];
+    pdl_wait();                                // (let go early, the merge's CTAs would crowd on the SMs that this launch leaves free)
+    const int rep = nq / nkv, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, total = plan[PLAN_ITEMS] * nkv, ld = hd + 4;
+    float* qs = pf_smem;                       // [32][hd + 4]
+    float* kv = qs + TL_ROWS * ld;             // keys [64][hd + 4], then values [64][vd]
+    float* sp = kv + CHUNK * (ld > vd ? ld : vd);      // scores, then weights
+    float* corr_of = sp + CHUNK * PF_P;        // [32] what the first tile's output is multiplied with
     const int* tokens = plan + plan[PLAN_AT_TOKENS];
     for (int it = blockIdx.x; it < total; it += gridDim.x) {
         const int* item = plan + plan[PLAN_AT_ITEMS] + it / nkv * PLAN_ITEM;
-        const int g = it % nkv, rows = item[ITEM_TOKENS] * rep, key_hi = item[ITEM_KEY_HI];
-        const int* mine = tokens + 2 * item[ITEM_TOKEN];
+        const int g = it % nkv, rows = item[ITEM_TOKENS] * rep, key_lo = item[ITEM_KEY_LO], key_hi = item[ITEM_KEY_HI];
         const int* table = block_table + (size_t)item[ITEM_REQUEST] * max_pages;
-        int pos_r[TL_RPW];
-        float slope_r[TL_RPW];
-#pragma unroll
-        for (int i = 0; i < TL_RPW; ++i) {
-            const int m = warp * TL_RPW + i;
-            slope_r[i] = slopes && m < rows ? slopes[g * rep + m % rep] : 0.f;
-            pos_r[i] = m < rows ? mine[2 * (m / rep) + 1] : -1;             // a row past the end takes no key
+        __syncthreads();                       // everyone is done with the item before
+        if (tid < TL_ROWS) {
+            const int* t = tokens + 2 * (item[ITEM_TOKEN] + tid / rep);
+            token_of[tid] = tid < rows ? t[0] : 0;
+            pos_of[tid] = tid < rows ? t[1] : -1;      // a row past the end takes no key
         }
-        for (int c = item[ITEM_KEY_LO] / CHUNK; c * CHUNK < key_hi; ++c) {
-            __syncthreads();                                                // everyone is done with the chunk (and the queries) before
-            if (c == item[ITEM_KEY_LO] / CHUNK && threadIdx.x >= CHUNK && threadIdx.x < CHUNK + TL_ROWS) {
-                const int m = threadIdx.x - CHUNK;
-                if (m < rows) q_of[m] = (size_t)mine[2 * (m / rep)] * q_stride + (size_t)(g * rep + m % rep) * hd;
+        __syncthreads();
+        for (int i = tid; i < TL_ROWS * (hd / 4); i += TL_WARPS * 32) {
+            const int m = i / (hd / 4), piece = i % (hd / 4);
+            cp_async_16(qs + m * ld + piece * 4, q + (m < rows ? (size_t)token_of[m] * q_stride + (size_t)(g * rep + m % rep) * hd + piece * 4 : 0), m < rows);
+        }
+        for (int c = key_lo / CHUNK; c * CHUNK < key_hi; ++c) {
+            if (tid < CHUNK) {
+                const int key = min(c * CHUNK + tid, key_hi - 1), page = min(max(table[min(key / page_size, max_pages - 1)], 0), pool_pages - 1);
+                row_of[tid] = (page * nkv + g) * page_size + key % page_size;
             }
-            if (threadIdx.x < CHUNK) {
-                const int key = min(c * CHUNK + (int)threadIdx.x, key_hi - 1), page = min(max(table[min(key / page_size, max_pages - 1)], 0), pool_pages - 1);
-                row_of[threadIdx.x] = ((size_t)page * nkv + g) * page_size + key % page_size;
+            __syncthreads();                   // (and everyone is done with the values of the chunk before)
+            for (int i = tid; i < CHUNK * (hd / 4); i += TL_WARPS * 32) {
+                const int k = i / (hd / 4), piece = i % (hd / 4);
+                cp_async_16(kv + k * ld + piece * 4, k_pages + (size_t)row_of[k] * hd + piece * 4, c * CHUNK + k < key_hi);       // keys from key_hi on are zeros
             }
+            asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
             __syncthreads();
-            const bool first = c == item[ITEM_KEY_LO] / CHUNK;
-            float m_c[TL_RPW], l_c[TL_RPW], o_c[TL_RPW][NE];
-            chunk_of_rows<float, NE>(qs, ks, vs, row_of, k_pages, v_pages, hd, vd, c, key_hi, scale, cap, pos_r, slope_r, [&]() {
-                if (first)
-                    for (int idx = threadIdx.x; idx < TL_ROWS * hd; idx += blockDim.x) {
-                        const int m = idx / hd, d = idx - m * hd;
-                        qs[idx] = m < rows ? q[q_of[m] + d] : 0.f;
-                    }
-            }, m_c, l_c, o_c);
+            {   // scores: rows r0 .. r0 + 3, keys k0 and k0 + 16
+                const int r0 = (warp & 3) * 8 + (lane >> 4) * 4, k0 = (warp >> 2) * 32 + (lane & 15);
+                float acc[4][2][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) acc[i][j][u] = 0.f;
+#pragma unroll 2
+                for (int d = 0; d < hd; d += 4) {
+                    float qv[4][4], kk[2][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) Vec<float>::load(qs + (r0 + i) * ld + d, qv[i]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) Vec<float>::load(kv + (k0 + 16 * j) * ld + d, kk[j]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) acc[i][j][u] = fmaf(qv[i][u], kk[j][u], acc[i][j][u]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) sp[(r0 + i) * PF_S + k0 + 16 * j] = (acc[i][j][0] + acc[i][j][1]) + (acc[i][j][2] + acc[i][j][3]);
+            }
+            __syncthreads();                   // the scores are there, the keys are done with
+            for (int i = tid; i < CHUNK * (vd / 4); i += TL_WARPS * 32) {
+                const int k = i / (vd / 4), piece = i % (vd / 4);
+                cp_async_16(kv + k * vd + piece * 4, v_pages + (size_t)row_of[k] * vd + piece * 4, c * CHUNK + k < key_hi);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            // weights of this warp's four rows, a lane a key, tile by tile as the walk takes them
+            float p[TL_RPW][2];
 #pragma unroll
             for (int i = 0; i < TL_RPW; ++i) {
-                const int m = warp * TL_RPW + i;
-                if (pos_r[i] < c * CHUNK || c >= max_chunks) continue;
-                float* dst = scratch + (((size_t)mine[2 * (m / rep)] * nq + g * rep + m % rep) * max_chunks + c) * (vd + 2);
-                if (lane == 0) { dst[0] = m_c[i]; dst[1] = l_c[i]; }
+                const int r = warp * TL_RPW + i, pos = pos_of[r];
+                const float slope = slopes && r < rows ? slopes[g * rep + r % rep] : 0.f;
+                float m = -INFINITY, l = 0.f, corr = 1.f;
 #pragma unroll
-                for (int e = 0; e < NE; ++e) {
-                    const int d = e * 32 + lane;
-                    if (d < vd) dst[2 + d] = o_c[i][e];
+                for (int t = 0; t < 2; ++t) {
+                    const int tile = c * CHUNK + t * 32, key = tile + lane;
+                    p[i][t] = 0.f;
+                    if (tile > pos) continue;
+                    const bool valid = key <= pos;
+                    float x = valid ? sp[r * PF_S + t * 32 + lane] * scale : -INFINITY;
+                    if (valid && cap > 0.f) x = cap * tanhf(x / cap);
+                    if (valid && slope != 0.f) x = __fsub_rn(x, __fmul_rn(slope, (float)(pos - key)));
+                    const float m_new = fmaxf(m, warp_max(x));
+                    p[i][t] = valid ? expf(x - m_new) : 0.f;
+                    corr = expf(m - m_new);
+                    l = fmaf(l, corr, warp_sum(p[i][t]));
+                    m = m_new;
+                    if (t == 0) corr = 1.f;
+                }
+                if (lane == 0) {
+                    corr_of[r] = corr;
+                    if (pos >= c * CHUNK && c < max_chunks) {
+                        float* dst = scratch + (((size_t)token_of[r] * nq + g * rep + r % rep) * max_chunks + c) * (vd + 2);
+                        dst[0] = m;
+                        dst[1] = l;
+                    }
+                }
+            }
+            __syncthreads();                   // the scores are done with
+#pragma unroll
+            for (int i = 0; i < TL_RPW; ++i)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) sp[(t * 32 + lane) * PF_P + warp * TL_RPW + i] = p[i][t];
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncthreads();                   // the values and the weights are there
+            const int col = (tid % DG) * 4, r0 = tid / DG * RT;
+            if (col < vd) {
+                float2 o[RT][2];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) o[i][0] = o[i][1] = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (t == 1) {
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) {
+                            const float f = corr_of[r0 + i];
+                            o[i][0].x *= f; o[i][0].y *= f; o[i][1].x *= f; o[i][1].y *= f;
+                        }
+                    }
+#pragma unroll 4
+                    for (int j = t * 32; j < t * 32 + 32; ++j) {
+                        const float4 v = *reinterpret_cast<const float4*>(kv + j * vd + col);
+                        float w[RT];
+#pragma unroll
+                        for (int i = 0; i < RT; i += 2) {
+                            const float2 two = *reinterpret_cast<const float2*>(sp + j * PF_P + r0 + i);
+                            w[i] = two.x; w[i + 1] = two.y;
+                        }
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) {
+                            o[i][0] = fma2(make_float2(w[i], w[i]), make_float2(v.x, v.y), o[i][0]);
+                            o[i][1] = fma2(make_float2(w[i], w[i]), make_float2(v.z, v.w), o[i][1]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    const int r = r0 + i;
+                    if (pos_of[r] < c * CHUNK || c >= max_chunks) continue;
+                    float* dst = scratch + (((size_t)token_of[r] * nq + g * rep + r % rep) * max_chunks + c) * (vd + 2) + 2 + col;
+                    *reinterpret_cast<float2*>(dst) = o[i][0];
+                    *reinterpret_cast<float2*>(dst + 2) = o[i][1];
                 }
             }
         }
@@ -944,8 +1048,10 @@ WLLM_API int wllm_paged_attention_simt_prefix(const void* q, int q_stride, void*
         pool_pages <= 0 || max_chunks < 1 || scratch == nullptr || !(cap >= 0.f) || ctas < 1)
         return WLLM_BAD_SIZE;
     if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) return WLLM_BAD_ALIGN;
-    constexpr int VN = Vec<float>::N, most = (TL_ROWS * 256 + 32 * (256 + VN) + 32 * 256) * (int)sizeof(float);
-    const size_t smem = ((size_t)TL_ROWS * hd + 32 * (hd + VN) + 32 * vd) * sizeof(float);
+    if (((uintptr_t)scratch & 7) || ((uintptr_t)q & 15) || q_stride % 4 != 0) return WLLM_BAD_ALIGN;
+    if ((long long)pool_pages * nkv * page_size > 0x7fffffffLL) return WLLM_BAD_SIZE;
+    const int most = prefix_floats(256, 256) * (int)sizeof(float);
+    const size_t smem = (size_t)prefix_floats(hd, vd) * sizeof(float);
     const int blocks = (int)(((long long)n_tokens * nq + WARPS - 1) / WARPS);
 #define GO(NE) do { \
         static bool raised = false; \

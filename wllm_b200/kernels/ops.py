@@ -812,7 +812,7 @@ def _prefix_costs(dtype: torch.dtype, hd: int, vd: int) -> tuple:
     thousand rows of results, the results of a thin item of several tiles.  bfloat16: the tensor core's products (100 cycles a step of 16 for the scores, 85 for 128 columns of the output), but no less than a group's turn with three
     buffers, or two, takes; thin items at 44 bytes a cycle and SM, but no less than their chain.  32 bits: 32 rows by 64 keys on the FMA pipes."""
     if dtype == torch.float32:
-        return 40 * (hd + vd), 6000, 40 * (hd + vd), 6000, 0, 4 * vd, 1
+        return 24 * (hd + vd), 4000, 24 * (hd + vd), 4000, 0, 4 * vd, 1
     wide, out = -(-hd // 64) * 64, -(-vd // 64) * 64
     tile = max(100 * wide // 16 + 85 * 8 * out // 128, 1500 if out <= 128 else 3000)
     return tile, 3500, max(256 * (hd + vd) // 44, 1500), 2500, 16, 3 * vd, 2 if hd <= 192 else 1

@@ -47,6 +47,8 @@
 // Used for the 32-bit path at every size, and for bfloat16 at the sizes that the
 // tensor-core kernels refuse.
 #include "common.cuh"
+#include <type_traits>
+
 #include "prefix_plan.cuh"
 
 constexpr int WARPS = 4;
@@ -589,14 +591,41 @@ __device__ __forceinline__ int chunk_pair(const int* __restrict__ req_q_len, con
     return -1;
 }
 
-// A warp's four rows over chunk `c`, whose keys' rows in the pools are `row_of`, by all warps of a CTA together; keys from key_hi on are zeros that no row sees.
-// `queries` puts the rows' queries into `qs` while the first tile is on its way (there is a barrier behind it).
-template <typename T, int NE, typename Queries>
-__device__ __forceinline__ void chunk_of_rows(const float* qs, T* ks, T* vs, const size_t* row_of, const T* __restrict__ k_pages, const T* __restrict__ v_pages, int hd, int vd, int c,
-                                              int key_hi, float scale, float cap, const int (&pos_r)[TL_RPW], const float (&slope_r)[TL_RPW], Queries queries, float (&m_c)[TL_RPW],
-                                              float (&l_c)[TL_RPW], float (&o_c)[TL_RPW][NE]) {
+template <typename T, int NE>
+__global__ void __launch_bounds__(TL_WARPS * 32, 2)
+paged_attention_simt_chunk_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
+                                  const int* __restrict__ req_q_start, const int* __restrict__ req_q_len, const int* __restrict__ req_ctx_len,
+                                  const int* __restrict__ block_table, int max_pages, int requests, int nq, int nkv, int hd, int page_size, float scale, int vd,
+                                  float cap, const float* __restrict__ slopes, float* __restrict__ scratch, int max_chunks) {
     constexpr int VN = Vec<T>::N;
-    const int lane = threadIdx.x & 31, kld = hd + VN;
+    extern __shared__ __align__(16) unsigned char tl_smem[];
+    __shared__ size_t row_of[CHUNK];               // the chunk's keys in the pools
+    pdl_begin();
+    int tile_at, c;
+    const int g = blockIdx.y, rep = nq / nkv, r = chunk_pair(req_q_len, req_ctx_len, requests, rep, max_chunks, blockIdx.x, tile_at, c);
+    if (r < 0) return;
+    const int q_len = req_q_len[r], rows = q_len * rep, m0 = tile_at * TL_ROWS;
+    const int ctx = req_ctx_len[r], q_start = req_q_start[r], pos0 = ctx - q_len;
+    const int key_hi = pos0 + (min(rows, m0 + TL_ROWS) - 1) / rep + 1;         // one past the last row's position
+    if (c * CHUNK >= key_hi) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kld = hd + VN;
+    float* qs = reinterpret_cast<float*>(tl_smem);                          // [32 rows][hd] float
+    T* ks = reinterpret_cast<T*>(qs + TL_ROWS * hd);                        // [32 keys][kld]
+    T* vs = ks + 32 * kld;                                                  // [32 keys][vd]
+    if (threadIdx.x < CHUNK) {
+        const int key = min(c * CHUNK + (int)threadIdx.x, key_hi - 1);
+        row_of[threadIdx.x] = ((size_t)block_table[(size_t)r * max_pages + key / page_size] * nkv + g) * page_size + key % page_size;
+    }
+    int pos_r[TL_RPW];
+    float slope_r[TL_RPW];
+#pragma unroll
+    for (int i = 0; i < TL_RPW; ++i) {
+        const int m = m0 + warp * TL_RPW + i;
+        slope_r[i] = slopes ? slopes[g * rep + m % rep] : 0.f;
+        pos_r[i] = m < rows ? pos0 + m / rep : -1;                          // a row past the end takes no key
+    }
+    __syncthreads();
     // 32 rows of `pieces` 16-byte pieces; keys past the last row's are zeros
     auto load = [&](int t, T* to, const T* from, int ld, int width, int to_ld) {
         const int pieces = width / VN, rows_on = (int)blockDim.x / pieces, pieces_on = (int)blockDim.x % pieces;
@@ -612,7 +641,11 @@ __device__ __forceinline__ void chunk_of_rows(const float* qs, T* ks, T* vs, con
     const int t0 = 2 * c, t1 = min(t0 + 2, (key_hi + 31) >> 5);
     load(t0, ks, k_pages, hd, hd, kld);
     load(t0, vs, v_pages, vd, vd, vd);
-    queries();
+    for (int idx = threadIdx.x; idx < TL_ROWS * hd; idx += blockDim.x) {
+        const int m = m0 + idx / hd, d = idx % hd;
+        qs[idx] = m < rows ? to_f32(q[(size_t)(q_start + m / rep) * q_stride + (size_t)(g * rep + m % rep) * hd + d]) : 0.f;
+    }
+    float m_c[TL_RPW], l_c[TL_RPW], o_c[TL_RPW][NE];
 #pragma unroll
     for (int i = 0; i < TL_RPW; ++i) {
         m_c[i] = -INFINITY; l_c[i] = 0.f;
@@ -629,7 +662,7 @@ __device__ __forceinline__ void chunk_of_rows(const float* qs, T* ks, T* vs, con
         float p[TL_RPW] = {0.f, 0.f, 0.f, 0.f};
         if (any) {
             const T* kr = ks + (size_t)lane * kld;
-            const float* qw = qs + (size_t)((int)(threadIdx.x >> 5) * TL_RPW) * hd;
+            const float* qw = qs + (size_t)(warp * TL_RPW) * hd;
             float acc[TL_RPW][4];
 #pragma unroll
             for (int i = 0; i < TL_RPW; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
@@ -693,50 +726,6 @@ __device__ __forceinline__ void chunk_of_rows(const float* qs, T* ks, T* vs, con
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-}
-
-template <typename T, int NE>
-__global__ void __launch_bounds__(TL_WARPS * 32, 2)
-paged_attention_simt_chunk_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ k_pages, const T* __restrict__ v_pages,
-                                  const int* __restrict__ req_q_start, const int* __restrict__ req_q_len, const int* __restrict__ req_ctx_len,
-                                  const int* __restrict__ block_table, int max_pages, int requests, int nq, int nkv, int hd, int page_size, float scale, int vd,
-                                  float cap, const float* __restrict__ slopes, float* __restrict__ scratch, int max_chunks) {
-    constexpr int VN = Vec<T>::N;
-    extern __shared__ __align__(16) unsigned char tl_smem[];
-    __shared__ size_t row_of[CHUNK];               // the chunk's keys in the pools
-    pdl_begin();
-    int tile_at, c;
-    const int g = blockIdx.y, rep = nq / nkv, r = chunk_pair(req_q_len, req_ctx_len, requests, rep, max_chunks, blockIdx.x, tile_at, c);
-    if (r < 0) return;
-    const int q_len = req_q_len[r], rows = q_len * rep, m0 = tile_at * TL_ROWS;
-    const int ctx = req_ctx_len[r], q_start = req_q_start[r], pos0 = ctx - q_len;
-    const int key_hi = pos0 + (min(rows, m0 + TL_ROWS) - 1) / rep + 1;         // one past the last row's position
-    if (c * CHUNK >= key_hi) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kld = hd + VN;
-    float* qs = reinterpret_cast<float*>(tl_smem);                          // [32 rows][hd] float
-    T* ks = reinterpret_cast<T*>(qs + TL_ROWS * hd);                        // [32 keys][kld]
-    T* vs = ks + 32 * kld;                                                  // [32 keys][vd]
-    if (threadIdx.x < CHUNK) {
-        const int key = min(c * CHUNK + (int)threadIdx.x, key_hi - 1);
-        row_of[threadIdx.x] = ((size_t)block_table[(size_t)r * max_pages + key / page_size] * nkv + g) * page_size + key % page_size;
-    }
-    int pos_r[TL_RPW];
-    float slope_r[TL_RPW];
-#pragma unroll
-    for (int i = 0; i < TL_RPW; ++i) {
-        const int m = m0 + warp * TL_RPW + i;
-        slope_r[i] = slopes ? slopes[g * rep + m % rep] : 0.f;
-        pos_r[i] = m < rows ? pos0 + m / rep : -1;                          // a row past the end takes no key
-    }
-    __syncthreads();
-    float m_c[TL_RPW], l_c[TL_RPW], o_c[TL_RPW][NE];
-    chunk_of_rows<T, NE>(qs, ks, vs, row_of, k_pages, v_pages, hd, vd, c, key_hi, scale, cap, pos_r, slope_r, [&]() {
-        for (int idx = threadIdx.x; idx < TL_ROWS * hd; idx += blockDim.x) {
-            const int m = m0 + idx / hd, d = idx % hd;
-            qs[idx] = m < rows ? to_f32(q[(size_t)(q_start + m / rep) * q_stride + (size_t)(g * rep + m % rep) * hd + d]) : 0.f;
-        }
-    }, m_c, l_c, o_c);
 #pragma unroll
     for (int i = 0; i < TL_RPW; ++i) {
         const int m = m0 + warp * TL_RPW + i;
@@ -754,13 +743,29 @@ paged_attention_simt_chunk_kernel(const T* __restrict__ q, int q_stride, const T
 // --------------------------------------------------------------------------------------
 // items of a plan (prefix_plan.cuh), for batches whose requests share pages: up to 32 rows of any requests against a range of whole chunks, each chunk's results left where those of the
 // kernel above are.  The rows of all requests that hold a stretch of pages meet its keys together.  A sum's terms and their order are the walk's, so its bits are too; which thread
-// adds up what is this kernel's own.  What bounds it is the FMA pipes and the reads of shared memory beside them, so a thread works out 4 rows x 2 keys of the scores (8 reads of a line
-// for 32 products, as long as these take; one key a thread was twice that) and 8 rows x 4 columns of the output (6), and two CTAs share an SM, so that one's products hide the other's waits.
-// 32 rows of 256 by 64 keys: 13.5 us of an SM as the kernel above does it, <measured> so.
+// adds up what is this kernel's own: a warp has the scores of 4 rows, a lane two keys of the 64 (6 reads of 16 bytes for 32 products), and the weights of the same rows, so that scores
+// stay in registers; of the output a thread has 8 rows x 4 columns.  What bounds a CTA is the turn from FMAs to reads of shared memory: 32 rows of 256 by 64 keys take it 4.5 us of scores,
+// 1.9 of weights, 2.9 of output (each product of 32 x 64 x 256 is 2.1 us of an SM's FMA pipes), 2.6 for the plan's numbers and the queries and 3 for what is left of the copies.  Two CTAs share
+// an SM, so that one's products hide the other's waits.  16 requests of 8 heads on 1,000 shared keys, 88 items: 15.5 us (request by request, with the kernels above, 59); with the four rows'
+// weights one behind the other, their scores by way of shared memory and a division a copy 19.0.
 // --------------------------------------------------------------------------------------
-constexpr int PF_S = 68, PF_P = 36;            // rows of scores [32][68] and of weights [64][36] in shared memory
+constexpr int PF_P = 36;                       // a key's row of weights in shared memory: 32 rows and padding
 
 static __host__ __device__ __forceinline__ int prefix_floats(int hd, int vd) { return TL_ROWS * (hd + 4) + CHUNK * (hd + 4 > vd ? hd + 4 : vd) + CHUNK * PF_P + TL_ROWS; }
+
+// The 16-byte pieces of rows of n floats that a thread of the CTA moves: row and column of one after the other, without a division each.
+struct Pieces {
+    int row, col, rows, cols, n;
+    __device__ __forceinline__ Pieces(int n_) : n(n_) {
+        const int a_row = n / 4;
+        row = threadIdx.x / a_row; col = threadIdx.x % a_row * 4;
+        rows = TL_WARPS * 32 / a_row; cols = TL_WARPS * 32 % a_row * 4;
+    }
+    __device__ __forceinline__ void next() {
+        row += rows; col += cols;
+        if (col >= n) { col -= n; ++row; }
+    }
+};
 
 template <int NE>
 __global__ void __launch_bounds__(TL_WARPS * 32, 2)
@@ -768,14 +773,17 @@ paged_attention_simt_prefix_kernel(const float* __restrict__ q, int q_stride, co
                                    const int* __restrict__ block_table, int max_pages, const int* __restrict__ plan, int nq, int nkv, int hd, int page_size, float scale, int vd,
                                    float cap, const float* __restrict__ slopes, float* __restrict__ scratch, int max_chunks) {
     constexpr int RT = NE, DG = 8 * NE;        // rows of the output a thread, threads along its columns (4 each)
+    constexpr int WV = RT % 4 ? 2 : 4;         // weights a load
+    using Wide = typename std::conditional<WV == 4, float4, float2>::type;
     extern __shared__ __align__(16) float pf_smem[];
-    __shared__ int row_of[CHUNK];              // the chunk's keys in the pools
-    __shared__ int token_of[TL_ROWS], pos_of[TL_ROWS];
+    __shared__ size_t row_of[CHUNK];           // the chunk's keys in the pools
+    __shared__ int token_of[TL_ROWS], head_of[TL_ROWS], row_at[TL_ROWS], pos_of[TL_ROWS];      // row_at: of the results, counted over tokens and heads
+    __shared__ float slope_of[TL_ROWS];
     pdl_wait();                                // (let go early, the merge's CTAs would crowd on the SMs that this launch leaves free)
     const int rep = nq / nkv, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, total = plan[PLAN_ITEMS] * nkv, ld = hd + 4;
     float* qs = pf_smem;                       // [32][hd + 4]
     float* kv = qs + TL_ROWS * ld;             // keys [64][hd + 4], then values [64][vd]
-    float* sp = kv + CHUNK * (ld > vd ? ld : vd);      // scores, then weights
+    float* sp = kv + CHUNK * (ld > vd ? ld : vd);      // weights [64][36]
     float* corr_of = sp + CHUNK * PF_P;        // [32] what the first tile's output is multiplied with
     const int* tokens = plan + plan[PLAN_AT_TOKENS];
     for (int it = blockIdx.x; it < total; it += gridDim.x) {
@@ -785,97 +793,124 @@ paged_attention_simt_prefix_kernel(const float* __restrict__ q, int q_stride, co
         __syncthreads();                       // everyone is done with the item before
         if (tid < TL_ROWS) {
             const int* t = tokens + 2 * (item[ITEM_TOKEN] + tid / rep);
+            const int head = g * rep + tid % rep;
             token_of[tid] = tid < rows ? t[0] : 0;
+            head_of[tid] = head;
+            row_at[tid] = tid < rows ? t[0] * nq + head : 0;
             pos_of[tid] = tid < rows ? t[1] : -1;      // a row past the end takes no key
+            slope_of[tid] = slopes ? slopes[head] : 0.f;
         }
         __syncthreads();
-        for (int i = tid; i < TL_ROWS * (hd / 4); i += TL_WARPS * 32) {
-            const int m = i / (hd / 4), piece = i % (hd / 4);
-            cp_async_16(qs + m * ld + piece * 4, q + (m < rows ? (size_t)token_of[m] * q_stride + (size_t)(g * rep + m % rep) * hd + piece * 4 : 0), m < rows);
+        for (Pieces at(hd); at.row < TL_ROWS; at.next()) {
+            const int m = at.row;
+            cp_async_16(qs + m * ld + at.col, q + (m < rows ? (size_t)token_of[m] * q_stride + (size_t)head_of[m] * hd + at.col : 0), m < rows);
         }
         for (int c = key_lo / CHUNK; c * CHUNK < key_hi; ++c) {
             if (tid < CHUNK) {
                 const int key = min(c * CHUNK + tid, key_hi - 1), page = min(max(table[min(key / page_size, max_pages - 1)], 0), pool_pages - 1);
-                row_of[tid] = (page * nkv + g) * page_size + key % page_size;
+                row_of[tid] = ((size_t)page * nkv + g) * page_size + key % page_size;
             }
             __syncthreads();                   // (and everyone is done with the values of the chunk before)
-            for (int i = tid; i < CHUNK * (hd / 4); i += TL_WARPS * 32) {
-                const int k = i / (hd / 4), piece = i % (hd / 4);
-                cp_async_16(kv + k * ld + piece * 4, k_pages + (size_t)row_of[k] * hd + piece * 4, c * CHUNK + k < key_hi);       // keys from key_hi on are zeros
-            }
+#pragma unroll 4
+            for (Pieces at(hd); at.row < CHUNK; at.next())
+                cp_async_16(kv + at.row * ld + at.col, k_pages + row_of[at.row] * hd + at.col, c * CHUNK + at.row < key_hi);       // keys from key_hi on are zeros
             asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
             __syncthreads();
-            {   // scores: rows r0 .. r0 + 3, keys k0 and k0 + 16
-                const int r0 = (warp & 3) * 8 + (lane >> 4) * 4, k0 = (warp >> 2) * 32 + (lane & 15);
-                float acc[4][2][4];
+            float sc[TL_RPW][2];               // scores of this warp's four rows, keys `lane` and `lane` + 32 a lane
+            {
+                float2 acc[TL_RPW][2][2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < TL_RPW; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < 2; ++j) acc[i][j][0] = acc[i][j][1] = make_float2(0.f, 0.f);
+                const float *qr = qs + warp * TL_RPW * ld, *kr = kv + lane * ld;
+                float4 qn[4], kn[2];           // asked for a turn ahead (the rows' 4 floats of padding are read behind the last)
+                auto ask = [&](int d) {
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) acc[i][j][u] = 0.f;
+                    for (int i = 0; i < 4; ++i) qn[i] = *reinterpret_cast<const float4*>(qr + i * ld + d);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) kn[j] = *reinterpret_cast<const float4*>(kr + 32 * j * ld + d);
+                };
+                ask(0);
 #pragma unroll 2
                 for (int d = 0; d < hd; d += 4) {
-                    float qv[4][4], kk[2][4];
+                    float4 qv[4], kk[2];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) Vec<float>::load(qs + (r0 + i) * ld + d, qv[i]);
+                    for (int i = 0; i < 4; ++i) qv[i] = qn[i];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) Vec<float>::load(kv + (k0 + 16 * j) * ld + d, kk[j]);
+                    for (int j = 0; j < 2; ++j) kk[j] = kn[j];
+                    ask(d + 4);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) acc[i][j][u] = fmaf(qv[i][u], kk[j][u], acc[i][j][u]);
+                        for (int j = 0; j < 2; ++j) {
+                            acc[i][j][0] = fma2(make_float2(qv[i].x, qv[i].y), make_float2(kk[j].x, kk[j].y), acc[i][j][0]);
+                            acc[i][j][1] = fma2(make_float2(qv[i].z, qv[i].w), make_float2(kk[j].z, kk[j].w), acc[i][j][1]);
+                        }
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) sp[(r0 + i) * PF_S + k0 + 16 * j] = (acc[i][j][0] + acc[i][j][1]) + (acc[i][j][2] + acc[i][j][3]);
+                    for (int j = 0; j < 2; ++j) sc[i][j] = (acc[i][j][0].x + acc[i][j][0].y) + (acc[i][j][1].x + acc[i][j][1].y);
             }
-            __syncthreads();                   // the scores are there, the keys are done with
-            for (int i = tid; i < CHUNK * (vd / 4); i += TL_WARPS * 32) {
-                const int k = i / (vd / 4), piece = i % (vd / 4);
-                cp_async_16(kv + k * vd + piece * 4, v_pages + (size_t)row_of[k] * vd + piece * 4, c * CHUNK + k < key_hi);
-            }
+            __syncthreads();                   // the keys are done with
+#pragma unroll 4
+            for (Pieces at(vd); at.row < CHUNK; at.next())
+                cp_async_16(kv + at.row * vd + at.col, v_pages + row_of[at.row] * vd + at.col, c * CHUNK + at.row < key_hi);
             asm volatile("cp.async.commit_group;" ::: "memory");
-            // weights of this warp's four rows, a lane a key, tile by tile as the walk takes them
-            float p[TL_RPW][2];
+            // weights of this warp's four rows, a lane a key, tile by tile as the walk takes them; the four go side by side (one behind the other they took three times as long)
+            float p[TL_RPW][2], m[TL_RPW], l[TL_RPW], corr[TL_RPW], slope[TL_RPW];
+            int pos[TL_RPW];
 #pragma unroll
             for (int i = 0; i < TL_RPW; ++i) {
-                const int r = warp * TL_RPW + i, pos = pos_of[r];
-                const float slope = slopes && r < rows ? slopes[g * rep + r % rep] : 0.f;
-                float m = -INFINITY, l = 0.f, corr = 1.f;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int tile = c * CHUNK + t * 32, key = tile + lane;
-                    p[i][t] = 0.f;
-                    if (tile > pos) continue;
-                    const bool valid = key <= pos;
-                    float x = valid ? sp[r * PF_S + t * 32 + lane] * scale : -INFINITY;
-                    if (valid && cap > 0.f) x = cap * tanhf(x / cap);
-                    if (valid && slope != 0.f) x = __fsub_rn(x, __fmul_rn(slope, (float)(pos - key)));
-                    const float m_new = fmaxf(m, warp_max(x));
-                    p[i][t] = valid ? expf(x - m_new) : 0.f;
-                    corr = expf(m - m_new);
-                    l = fmaf(l, corr, warp_sum(p[i][t]));
-                    m = m_new;
-                    if (t == 0) corr = 1.f;
-                }
-                if (lane == 0) {
-                    corr_of[r] = corr;
-                    if (pos >= c * CHUNK && c < max_chunks) {
-                        float* dst = scratch + (((size_t)token_of[r] * nq + g * rep + r % rep) * max_chunks + c) * (vd + 2);
-                        dst[0] = m;
-                        dst[1] = l;
-                    }
-                }
+                const int r = warp * TL_RPW + i;
+                m[i] = -INFINITY; l[i] = 0.f; corr[i] = 1.f;
+                pos[i] = pos_of[r];
+                slope[i] = slope_of[r];
             }
-            __syncthreads();                   // the scores are done with
 #pragma unroll
-            for (int i = 0; i < TL_RPW; ++i)
+            for (int t = 0; t < 2; ++t) {
+                const int tile = c * CHUNK + t * 32, key = tile + lane;
+                float x[TL_RPW], top[TL_RPW], sum[TL_RPW];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) sp[(t * 32 + lane) * PF_P + warp * TL_RPW + i] = p[i][t];
+                for (int i = 0; i < TL_RPW; ++i) {
+                    const bool valid = key <= pos[i];
+                    x[i] = sc[i][t] * scale;
+                    if (cap > 0.f) x[i] = cap * tanhf(x[i] / cap);
+                    if (slope[i] != 0.f) x[i] = __fsub_rn(x[i], __fmul_rn(slope[i], (float)(pos[i] - key)));
+                    if (!valid) x[i] = -INFINITY;
+                    top[i] = x[i];
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                    for (int i = 0; i < TL_RPW; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+#pragma unroll
+                for (int i = 0; i < TL_RPW; ++i) {
+                    top[i] = fmaxf(m[i], top[i]);
+                    p[i][t] = sum[i] = key <= pos[i] ? expf(x[i] - top[i]) : 0.f;
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                    for (int i = 0; i < TL_RPW; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+#pragma unroll
+                for (int i = 0; i < TL_RPW; ++i)
+                    if (tile <= pos[i]) {      // a row sits out the tiles behind its own position
+                        corr[i] = expf(m[i] - top[i]);
+                        l[i] = fmaf(l[i], corr[i], sum[i]);
+                        m[i] = top[i];
+                        if (t == 0) corr[i] = 1.f;
+                    }
+            }
+            if (lane < TL_RPW) {               // lane i has row i's to store
+                const int r = warp * TL_RPW + lane;
+                const float mm = lane & 2 ? (lane & 1 ? m[3] : m[2]) : lane & 1 ? m[1] : m[0], ll = lane & 2 ? (lane & 1 ? l[3] : l[2]) : lane & 1 ? l[1] : l[0];
+                corr_of[r] = lane & 2 ? (lane & 1 ? corr[3] : corr[2]) : lane & 1 ? corr[1] : corr[0];
+                if (pos_of[r] >= c * CHUNK && c < max_chunks) *reinterpret_cast<float2*>(scratch + ((size_t)row_at[r] * max_chunks + c) * (vd + 2)) = make_float2(mm, ll);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) *reinterpret_cast<float4*>(sp + (t * 32 + lane) * PF_P + warp * TL_RPW) = make_float4(p[0][t], p[1][t], p[2][t], p[3][t]);
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncthreads();                   // the values and the weights are there
             const int col = (tid % DG) * 4, r0 = tid / DG * RT;
@@ -895,12 +930,9 @@ paged_attention_simt_prefix_kernel(const float* __restrict__ q, int q_stride, co
 #pragma unroll 4
                     for (int j = t * 32; j < t * 32 + 32; ++j) {
                         const float4 v = *reinterpret_cast<const float4*>(kv + j * vd + col);
-                        float w[RT];
+                        alignas(16) float w[RT];
 #pragma unroll
-                        for (int i = 0; i < RT; i += 2) {
-                            const float2 two = *reinterpret_cast<const float2*>(sp + j * PF_P + r0 + i);
-                            w[i] = two.x; w[i + 1] = two.y;
-                        }
+                        for (int i = 0; i < RT; i += WV) *reinterpret_cast<Wide*>(w + i) = *reinterpret_cast<const Wide*>(sp + j * PF_P + r0 + i);
 #pragma unroll
                         for (int i = 0; i < RT; ++i) {
                             o[i][0] = fma2(make_float2(w[i], w[i]), make_float2(v.x, v.y), o[i][0]);
@@ -912,7 +944,7 @@ paged_attention_simt_prefix_kernel(const float* __restrict__ q, int q_stride, co
                 for (int i = 0; i < RT; ++i) {
                     const int r = r0 + i;
                     if (pos_of[r] < c * CHUNK || c >= max_chunks) continue;
-                    float* dst = scratch + (((size_t)token_of[r] * nq + g * rep + r % rep) * max_chunks + c) * (vd + 2) + 2 + col;
+                    float* dst = scratch + ((size_t)row_at[r] * max_chunks + c) * (vd + 2) + 2 + col;
                     *reinterpret_cast<float2*>(dst) = o[i][0];
                     *reinterpret_cast<float2*>(dst + 2) = o[i][1];
                 }

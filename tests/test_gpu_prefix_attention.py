@@ -9,7 +9,8 @@ pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
 
 SHAPES = [                      # (query heads, kv heads, key size, value size)
-    (8, 1, 256, 256), (16, 4, 128, 128), (6, 2, 72, 40), (7, 1, 64, 64), (4, 4, 96, 96), (128, 1, 8, 256), (5, 1, 192, 64), (16, 8, 200, 136), (2, 1, 256, 8)]
+    (8, 1, 256, 256), (16, 4, 128, 128), (6, 2, 72, 40), (7, 1, 64, 64), (4, 4, 96, 96), (128, 1, 8, 256), (5, 1, 192, 64), (16, 8, 200, 136), (2, 1, 256, 8),
+          (3, 1, 192, 256), (6, 3, 136, 200)]
 TREES = [
     (0, [(5, 1)]),
     (0, [(0, 1), (0, 1)]),

@@ -44,7 +44,9 @@
 
 constexpr int HD = HEAD_DIM, VD = VALUE_DIM;
 static_assert(HD % 8 == 0 && HD >= 8 && HD <= 256 && VD % 8 == 0 && VD >= 8 && VD <= 256, "head sizes in steps of 8 up to 256");
-constexpr int HDP = (HD + 63) / 64 * 64, VDP = (VD + 63) / 64 * 64;
+constexpr int VDP = (VD + 63) / 64 * 64;
+// (beside values of 256 columns, keys of 192 are worked off in two halves of 128: with stages of 192 columns only three would fit, and four are needed below)
+constexpr int HDP = HD > 128 && VDP == 256 ? 256 : (HD + 63) / 64 * 64;
 constexpr int BM = 128, BN = 128;
 // a stage of the ring: 128 keys of KW columns of K, or VW columns of V
 constexpr int KW = HDP == 256 ? 128 : HDP, VW = VDP == 256 ? 128 : VDP;
@@ -864,11 +866,6 @@ static int pool_map(const void* ptr, long long rows, int box_rows, int head, CUt
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? WLLM_OK : 2000 + (int)r;
 }
-
-// Rows of an item at most.
-WLLM_API int wllm_prefix_attention_rows() { return BM; }
-// Results that an item of few rows leaves where it has several tiles of keys.
-WLLM_API int wllm_prefix_attention_sides() { return SIDES; }
 
 // The attention of a planned batch.  pool_pages: pages of the pools; n_tokens: rows of q and out; scratch: nkv * rows * (VD + 2) floats, rows as the plan has them (or the most that a plan of
 // this array may have); items_at, tokens_at: their places in the plan; n_items: its items, or -1: its header says; pairs: (item, kv head) pairs, or the most that there may be; ctas: SMs.  sinks, slopes: 32-bit [nq] or null; cap > 0: scores become cap tanh(score / cap).

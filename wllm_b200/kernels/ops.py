@@ -813,9 +813,10 @@ def _prefix_costs(dtype: torch.dtype, hd: int, vd: int) -> tuple:
     buffers, or two, takes; thin items at 44 bytes a cycle and SM, but no less than their chain.  32 bits: 32 rows by 64 keys on the FMA pipes."""
     if dtype == torch.float32:
         return 24 * (hd + vd), 4000, 24 * (hd + vd), 4000, 0, 4 * vd, 1
-    wide, out = -(-hd // 64) * 64, -(-vd // 64) * 64
+    out = -(-vd // 64) * 64
+    wide = 256 if hd > 128 and out == 256 else -(-hd // 64) * 64      # as csrc/prefix_attention.cu widens them
     tile = max(100 * wide // 16 + 85 * 8 * out // 128, 1500 if out <= 128 else 3000)
-    return tile, 3500, max(256 * (hd + vd) // 44, 1500), 2500, 16, 3 * vd, 2 if hd <= 192 else 1
+    return tile, 3500, max(256 * (hd + vd) // 44, 1500), 2500, 16, 3 * vd, 2 if wide <= 192 else 1
 
 
 def prefix_ok(nq: int, nkv: int, hd: int, vd: int, page_size: int, dtype: torch.dtype) -> bool:

@@ -778,47 +778,48 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
     }
 }
 
-// The merge of a token's results: grid (tokens, kv heads, groups of warps).  A warp takes up to four neighbouring query heads, whose rows of eight columns are one line, by 32 / heads blocks
-// of eight columns, a lane each; results eight at a time, with a running maximum.  Bound by the latency of its chain of loads (starts, list, results), hence the eight in flight.
-constexpr int MERGE_WARPS = 4;
+// The merge of a token's results: grid (tokens, kv heads, groups of warps).  A warp's lanes are up to four neighbouring query heads, whose rows of eight columns are one line, by `split` results,
+// by blocks of eight columns: lane i of those that share a row's block takes results i, i + split, ..., eight at a time, with a running maximum, and what they have is added up by shuffles.  (No
+// shared memory: that would keep the next launch, which wants all of an SM's, from getting ready meanwhile.)  Bound by the latency of its chain of loads (starts, list, results), hence the
+// eight in flight, and the more lanes a row the fewer rows there are (8 heads of 256 by one lane, and so: 2 tokens of 65 results 11.7 and 5.8 us, 64 of 19 6.0 and 4.9).
+constexpr int MERGE_WARPS = 4, MERGE_SPLIT = 8;
 __host__ __device__ __forceinline__ int merge_heads(int rep) { return rep >= 4 ? 4 : rep >= 2 ? 2 : 1; }
-__host__ __device__ __forceinline__ int merge_units(int rep) {
-    const int heads = merge_heads(rep), blocks = 32 / heads;
+__host__ __device__ __forceinline__ int merge_units(int rep, int split) {
+    const int heads = merge_heads(rep), blocks = 32 / (heads * split);
     return (rep + heads - 1) / heads * ((VD / 8 + blocks - 1) / blocks);
 }
 __global__ void __launch_bounds__(MERGE_WARPS * 32)
 prefix_merge_kernel(bf16* __restrict__ out, int out_stride, const int* __restrict__ plan, int rep, long long rows, const float* __restrict__ part_o, const float* __restrict__ part_ml,
-                    const float* __restrict__ sinks) {
-    pdl_begin();
+                    const float* __restrict__ sinks, int split) {
+    pdl_wait();
     const int token = blockIdx.x, g = blockIdx.y, unit = (int)blockIdx.z * MERGE_WARPS + (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (unit >= merge_units(rep)) return;
-    const int heads = merge_heads(rep), groups = (rep + heads - 1) / heads;
-    const int h = unit % groups * heads + lane % heads, col = unit / groups * (32 / heads) + lane / heads;
-    if (h >= rep || col >= VD / 8) return;
+    if (unit >= merge_units(rep, split)) return;
+    const int heads = merge_heads(rep), groups = (rep + heads - 1) / heads, part = lane / heads % split;
+    const int h = unit % groups * heads + lane % heads, col = unit / groups * (32 / (heads * split)) + lane / (heads * split);
+    const bool live = h < rep && col < VD / 8;
     const int* starts = plan + plan[PLAN_AT_STARTS];
     const int first = starts[token], n = starts[token + 1] - first;
-    if (n <= 0) return;
     const int* list = plan + plan[PLAN_AT_RESULTS] + first;
     const float* mine_o = part_o + ((size_t)g * (VD / 8) + col) * rows * 8;
     const float2* mine_ml = reinterpret_cast<const float2*>(part_ml) + (size_t)g * rows;
     float M = -INFINITY, L = 0.f, O[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     constexpr int AHEAD = 8;
-    for (int i0 = 0; i0 < n; i0 += AHEAD) {
+    for (int i0 = part; live && i0 < n; i0 += AHEAD * split) {
         float4 v[AHEAD][2];
         float2 ml[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const size_t at = (size_t)list[min(i0 + u, n - 1)] + h;
-            ml[u] = mine_ml[at];
-            v[u][0] = reinterpret_cast<const float4*>(mine_o + at * 8)[0];
-            v[u][1] = reinterpret_cast<const float4*>(mine_o + at * 8)[1];
+            ml[u] = make_float2(-INFINITY, 0.f);
+            if (i0 + u * split < n) {
+                const size_t at = (size_t)list[i0 + u * split] + h;
+                ml[u] = mine_ml[at];
+                v[u][0] = reinterpret_cast<const float4*>(mine_o + at * 8)[0];
+                v[u][1] = reinterpret_cast<const float4*>(mine_o + at * 8)[1];
+            }
         }
         float top = M;
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            if (i0 + u >= n) ml[u] = make_float2(-INFINITY, 0.f);        // (read again: weighs nothing)
-            top = fmaxf(top, ml[u].x);
-        }
+        for (int u = 0; u < AHEAD; ++u) top = fmaxf(top, ml[u].x);
         const float base = top == -INFINITY ? 0.f : top, keep = exp2f(M - base);
         M = top;
         L *= keep;
@@ -827,13 +828,26 @@ prefix_merge_kernel(bf16* __restrict__ out, int out_stride, const int* __restric
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const float f = exp2f(ml[u].x - base);
-            if (i0 + u < n) {
+            if (i0 + u * split < n) {
                 L = fmaf(ml[u].y, f, L);
                 O[0] = fmaf(v[u][0].x, f, O[0]); O[1] = fmaf(v[u][0].y, f, O[1]); O[2] = fmaf(v[u][0].z, f, O[2]); O[3] = fmaf(v[u][0].w, f, O[3]);
                 O[4] = fmaf(v[u][1].x, f, O[4]); O[5] = fmaf(v[u][1].y, f, O[5]); O[6] = fmaf(v[u][1].z, f, O[6]); O[7] = fmaf(v[u][1].w, f, O[7]);
             }
         }
     }
+    pdl_launch_dependents();       // (at the start it cost 96 requests' layer 3 us: the next launch's CTAs came to lie unevenly beside this one's)
+    for (int o = heads; o < heads * split; o *= 2) {
+        const float other = __shfl_xor_sync(0xffffffffu, M, o), top = fmaxf(M, other), base = top == -INFINITY ? 0.f : top, keep = exp2f(M - base);
+        M = top;
+        L *= keep;
+        L += __shfl_xor_sync(0xffffffffu, L, o);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            O[j] *= keep;
+            O[j] += __shfl_xor_sync(0xffffffffu, O[j], o);
+        }
+    }
+    if (!live || n <= 0 || part > 0) return;
     if (sinks) L += exp2f(sinks[g * rep + h] * LOG2E - (M == -INFINITY ? 0.f : M));
     const float inv = 1.0f / L;
     bf16* to = out + (size_t)token * out_stride + (size_t)(g * rep + h) * VD + col * 8;
@@ -898,6 +912,9 @@ WLLM_API int wllm_prefix_attention(const void* q, int q_stride, void* out, int o
     const int st = wllm_launch(prefix_kernel, dim3((unsigned)(pairs < ctas ? pairs : ctas)), THREADS, SMEM, stream, p, km, vm);
     if (st) return st;
     const int rep = nq / nkv;
-    return wllm_launch(prefix_merge_kernel, dim3(n_tokens, nkv, (merge_units(rep) + MERGE_WARPS - 1) / MERGE_WARPS), MERGE_WARPS * 32, 0, stream, (bf16*)out, out_stride, plan, rep, rows,
-                       (const float*)p.part_o, (const float*)p.part_ml, sinks);
+    // lanes that share a row's block: as many as keep the device's SMs at 16 warps each
+    int split = 1;
+    while (split < MERGE_SPLIT && (long long)n_tokens * nkv * merge_units(rep, 2 * split) <= 16LL * ctas) split *= 2;
+    return wllm_launch(prefix_merge_kernel, dim3(n_tokens, nkv, (merge_units(rep, split) + MERGE_WARPS - 1) / MERGE_WARPS), MERGE_WARPS * 32, 0, stream, (bf16*)out, out_stride, plan, rep, rows,
+                       (const float*)p.part_o, (const float*)p.part_ml, sinks, split);
 }

@@ -825,13 +825,17 @@ def prefix_ok(nq: int, nkv: int, hd: int, vd: int, page_size: int, dtype: torch.
         0 < hd <= 256 and hd % 8 == 0 and 0 < vd <= 256 and vd % 8 == 0 and page_size >= 16 and page_size & (page_size - 1) == 0
 
 
+# Bytes of keys and values that a step then reads less often.  bfloat16: the engine's other attention reads the same keys again from the L2 cache, and what is saved has to pay for results in
+# parts and their merge (us a layer, it and prefix_attention: 16 heads on 4 of 128, 4 requests on 1,024 keys, 6 MB: 6.2 and 8.2; 16 on 512, 15 MB: 10.6 and 9.4; 16 heads of 256 on 16, 2 on 1,024,
+# 16 MB: 10.3 and 10.7; 32 on 8 of 128, 4 on 2,048, 24 MB: 12.0 and 9.6; 8 heads of 256 on one, 64 on 512, 31 MB: 14.9 and 12.4; 2 on 8,192, 8 MB: 9.5 and 11.6; 16 on 8,192, 120 MB: 21 and 15).
+# 32 bits: 8 heads of 256 on one, 2 on 128, 256 KB: 22.9 and 16.1; 16 on 256, 7.5 MB: 46 and 17.
+PREFIX_SAVED = {2: 24 << 20, 4: 1 << 18}
+
+
 def prefix_pays(saved_keys: int, nkv: int, hd: int, vd: int, dtype: torch.dtype) -> bool:
     """Whether a step reads shared keys once for all, from the keys (times further holders) that it then reads less often."""
     item = 2 if dtype == torch.bfloat16 else 4
     return saved_keys * nkv * (hd + vd) * item >= PREFIX_SAVED[item]
-
-
-PREFIX_SAVED = {2: 24 << 20, 4: 4 << 20}
 
 
 def prefix_caps(requests: int, nkv: int) -> tuple:

@@ -125,6 +125,18 @@ def test_captured_steps_of_changing_batches(tmp_path, always):
     assert all(rec["meta"] is llm.runner._meta for g in (llm.runner._graphs, llm.runner._prefix_graphs) for rec in g.values())
 
 
+def test_samples_without_room_for_their_prompt_beside_them(tmp_path):
+    """Three pages hold a request to its end, but not the prompt that its samples would share beside one of them; nor are there slots for all prompts of a batch."""
+    folder = folders(tmp_path)["A"]()
+    kw = dict(dtype="float32", block_size=16, max_num_seqs=3)
+    sp = SamplingParams(max_tokens=8, ignore_eos=True, temperature=0.8, seed=5, n=3)
+    for blocks, lengths in ((3, (40,)), (40, (20, 33, 17, 40))):
+        llm, roomy = LLM(folder, num_blocks=blocks, **kw), LLM(folder, dtype="float32", block_size=16, num_blocks=80)
+        prompts = [tokens(n, llm.model.plan.vocab_size, n) for n in lengths]
+        assert [o.token_ids for o in llm.generate(prompts, sp)] == [o.token_ids for o in roomy.generate(prompts, sp)]
+        assert llm.runner.cache.free_pages() == [blocks] * len(llm.runner.cache.groups) and not llm.scheduler.prefixes
+
+
 def test_the_command(tmp_path, capsys):
     import json
 

@@ -137,6 +137,39 @@ def test_slots_are_left_for_no_more_than_there_are():
     assert all(len(r.output_token_ids) == 4 for r in reqs)
 
 
+def test_prefixes_leave_what_was_taken_on_its_pages_and_a_slot():
+    """A request that was taken on can finish whatever prefixes come after it."""
+    runner, s = make(pages=8)
+    big = request("big", range(20), max_tokens=9)                     # 8 pages at the end
+    s.add_request(big)
+    for auto in (False, True):
+        with pytest.raises(ValueError, match="pages"):
+            s.add_prefix([1, 2, 3], auto=auto)
+    s.step()
+    with pytest.raises(ValueError, match="pages"):
+        s.add_prefix([1])
+    assert not s.prefixes
+    s.run_to_completion()
+    assert big.output_token_ids == alone(list(range(20)), 9)
+    prefix = s.add_prefix(range(10))                                  # 3 pages, two of them full
+    s.add_request(request("a", list(range(10)) + [1], prefix, max_tokens=16))      # 7 pages, 5 beside the prefix's
+    with pytest.raises(ValueError, match="pages"):
+        s.add_prefix([5])
+    nested = s.prefix_refusal(12, prefix)
+    assert nested and "pages" in nested
+    s.run_to_completion()
+    assert s.prefix_refusal(12, prefix) is None and s.prefix_refusal(4, None, 16) is None and "pages" in s.prefix_refusal(4, None, 25)
+    runner = FakeRunner(24, max_requests=3)
+    s = Scheduler(runner, ArgmaxSampler())
+    kept = [s.add_prefix([i, 2, 3]) for i in range(2)]
+    with pytest.raises(ValueError, match="none would be left"):
+        s.add_prefix([9])
+    r = request("r", kept[0].token_ids + [4], kept[0])
+    s.add_request(r)
+    s.run_to_completion()
+    assert r.output_token_ids == alone(r.prompt_token_ids)
+
+
 def test_samples_draw_from_seeds_of_their_own():
     seeds = [sample_seed(7, k) for k in range(100)]
     assert seeds[0] == 7 and len(set(seeds)) == 100 and all(0 <= x < 1 << 63 for x in seeds[1:])

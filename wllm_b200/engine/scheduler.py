@@ -127,9 +127,24 @@ class Scheduler:
             total -= len(request.prefix.token_ids) // self.cache.page_size
         return total
 
+    def prefix_refusal(self, num_tokens: int, prefix: Prefix | None = None, worst_tokens: int = 0) -> str | None:
+        """Why a prefix of that many tokens cannot be kept beside what was taken on, or None: with its pages held, some unfinished request, or one of `worst_tokens` that is to begin with
+        it, could never finish."""
+        if len(self.prefixes) + 1 >= self.cache.slots.num_slots:
+            return f"{len(self.prefixes)} prefixes and {self.cache.slots.num_slots} requests at most: none would be left"
+        ps = self.cache.page_size
+        own = self._pages(num_tokens) - (len(prefix.token_ids) // ps if prefix is not None else 0)
+        need = max(self.largest_need(), self._held_pages() + self._pages(min(worst_tokens, self.max_model_len)) - num_tokens // ps) + own
+        pool = min(g.pool.num_pages for g in self.cache.groups) if self.cache.groups else 1 << 30
+        return f"with a prefix of {num_tokens} tokens the unfinished requests need {need} pages, the cache has {pool}" if need > pool else None
+
     def add_prefix(self, token_ids, prefix: Prefix | None = None, auto: bool = False) -> Prefix:
         """Tokens for requests to begin with; `prefix`: one that they themselves begin with.  They are computed by the steps to come."""
-        holder = Request(("prefix", self._prefix_id), list(token_ids), SamplingParams(max_tokens=1), prefix=prefix, holds=True)
+        token_ids = list(token_ids)
+        refusal = self.prefix_refusal(len(token_ids), prefix)
+        if refusal:
+            raise ValueError(refusal)
+        holder = Request(("prefix", self._prefix_id), token_ids, SamplingParams(max_tokens=1), prefix=prefix, holds=True)
         self.add_request(holder)
         self._prefix_id += 1
         made = Prefix(holder.prompt_token_ids, holder, auto)

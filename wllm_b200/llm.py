@@ -91,8 +91,8 @@ class LLM:
         if sp.n == 1:
             return self._add(request_id, prompt, sp, prefix)
         begin = prefix
-        if len(prompt) > 1 + (len(prefix.token_ids) if prefix is not None else 0):
-            # the samples are forks of the prompt without its last token, which each of them runs for its own first draw
+        if len(prompt) > 1 + (len(prefix.token_ids) if prefix is not None else 0) and not self.scheduler.prefix_refusal(len(prompt) - 1, prefix, len(prompt) + sp.max_tokens):
+            # the samples are forks of the prompt without its last token, which each of them runs for its own first draw; a prompt that cannot be kept beside them is computed by each
             begin = self.scheduler.add_prefix(prompt[:-1], prefix=prefix, auto=True)
         one = [replace(sp, n=1, seed=None if sp.seed is None else sample_seed(sp.seed, k)) for k in range(sp.n)]
         made = []

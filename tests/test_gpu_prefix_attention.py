@@ -153,6 +153,47 @@ def test_in_a_graph_on_a_stream_and_twice_at_once(dtype):
     assert torch.equal(outs[0].cpu(), want[0])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_captured_call_for_plans_of_several_batches(dtype):
+    """A call laid out for twelve tokens replayed for batches of twelve, five and one: the rows behind the last token stay as they were."""
+    from wllm_b200.kernels import ops
+    caps, width = (64, 96, 400, 12), 24
+    batches = [Batch(tree, 8, 2, 64, 64, 16, seed=i, dtype=dtype) for i, tree in enumerate([(256, [(5, 1)] * 12), (0, [(128, [(9, 1)] * 3), (70, 1), (0, 1)]), (0, [(33, 1)])])]
+    made = []
+    for b in batches:
+        table = torch.full((b.R, width), -1, dtype=torch.int32)
+        table[:, :b.table.shape[1]] = torch.as_tensor(b.table)
+        made.append((ops.prefix_plan(torch.cat([table, torch.full((12 - b.R, width), -1, dtype=torch.int32)]), b.q_lens + [0] * (12 - b.R), b.ctx_lens + [0] * (12 - b.R), 16, 8, 2, 64, 64,
+                                     dtype, caps=caps), table))
+    pages = max(b.k.shape[0] for b in batches)
+    q, out, k, v = (torch.zeros(*s, dtype=dtype, device=DEV) for s in ((12, 512), (12, 512), (pages, 2, 16, 64), (pages, 2, 16, 64)))
+    table = torch.zeros(12, width, dtype=torch.int32, device=DEV)
+    plan = made[0][0]
+    arrays, scratch = torch.zeros(plan.used, dtype=torch.int32, device=DEV), torch.full((plan.scratch_floats,), float("nan"), device=DEV)
+
+    def put(i):
+        b, (p, t) = batches[i], made[i]
+        assert p.used == plan.used and p.launch == plan.launch and p.places == plan.places
+        arrays.copy_(p.host)
+        table[:b.R] = t.to(DEV)
+        q[:b.n], k[:b.k.shape[0]], v[:b.v.shape[0]] = (x.to(DEV) for x in (b.q, b.k, b.v))
+        out.fill_(7.0)
+        scratch.fill_(float("nan"))
+    put(0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.prefix_attention(q, out, k, v, table, plan, arrays, 8, 2, 64, 16, 64 ** -0.5, scratch)
+    for i in (0, 1, 2, 0):
+        put(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        b = batches[i]
+        assert bool((out[b.n:] == 7.0).all())
+        # bfloat16: a weight's and the output's rounding, as above; 32 bits: as in test_float32_against_64_bits, sums of 64 products and of 300 keys
+        bound = 2.0 ** -8 * (1.0625 * magnitude(b, "plain") + b.exact(64 ** -0.5).abs()) if dtype == BF16 else 4e-4 * magnitude(b, "plain")
+        assert bool(((out[:b.n].cpu().double() - b.exact(64 ** -0.5)).abs() <= bound).all()), i
+
+
 def test_pools_past_32_bits():
     """Keys that lie more than 2^32 bytes into the pools, at places above 2^31 elements."""
     b = Batch((256, [(70, 1), (5, 2)]), 8, 1, 256, 256, 64, dtype=BF16)

@@ -115,9 +115,30 @@ def test_refusals():
     ops.prefix_plan(**good)
     for wrong in (dict(q_lens=[1]), dict(q_lens=[-1, 2]), dict(q_lens=[71, 2]), dict(ctx_lens=[129, 71]), dict(tables=np.array([[3, -1], [3, 9]], dtype=np.int32)),
                   dict(tables=table.astype(np.int64)), dict(tables=table[0]), dict(nq=5), dict(nq=512), dict(hd=12), dict(hd=264), dict(vd=0), dict(page_size=8), dict(page_size=48),
-                  dict(dtype=torch.float16), dict(dtype=torch.float32, nq=128), dict(ctx_lens=[0, 71]), dict(q_lens=[1.0, 2.0])):
+                  dict(caps=(0, 8, 8, 8)), dict(caps=(8, 8, 8, -1)), dict(caps=(8, 8, 8)), dict(dtype=torch.float16), dict(dtype=torch.float32, nq=128), dict(ctx_lens=[0, 71]), dict(q_lens=[1.0, 2.0])):
         with pytest.raises(ops.KernelError):
             ops.prefix_plan(**{**good, **wrong})
+
+
+def test_a_long_chain_of_branchings():
+    """Every request leaves the others one page after the last: the plan follows some hundred of them and is right for all."""
+    n = 400
+    table = np.array([[j if j < r else 1000 + r * n + j for j in range(n)] for r in range(n)], dtype=np.int32)
+    ctx = [16 * (r + 1) + 1 if r + 1 < n else 16 * n for r in range(n)]
+    plan = ops.prefix_plan(table, [1] * n, ctx, 16, 1, 1, 8, min_keys=1)
+    assert plan.saved_keys > 0
+    check(plan, table.tolist(), [1] * n, ctx, 16, 1, 128, 1)
+
+
+def test_a_plan_laid_out_for_more_than_the_batch_has():
+    b = Batch((512, [(3, 1), (0, 1), (40, 1)]), 4, 1, 8, 8, 64)
+    for dtype in (torch.bfloat16, torch.float32):
+        plan = ops.prefix_plan(b.table, b.q_lens, b.ctx_lens, 64, 4, 1, 8, 8, dtype, caps=(64, 64, 128, 9))
+        items, tokens, starts, listed, _ = parts(plan)
+        h = plan.host.numpy()
+        assert plan.n_tokens == 9 and h[h[4]:h[4] + 10].tolist() == starts.tolist() + [starts[-1]] * 6 and h[h[6]:h[6] + 9].tolist() == [c - 1 for c in b.ctx_lens] + [-1] * 6
+        for caps in ((1, 64, 128, 9), (64, 1, 128, 9), (64, 64, 1, 9), (64, 64, 128, 2)):
+            assert ops.prefix_plan(b.table, b.q_lens, b.ctx_lens, 64, 4, 1, 8, 8, dtype, caps=caps) is None
 
 
 @pytest.mark.parametrize("seed", range(8))

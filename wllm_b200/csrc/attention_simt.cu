@@ -268,6 +268,7 @@ paged_attention_simt_merge_kernel(T* __restrict__ out, int out_stride, const int
     if (item >= n_tokens * nq) return;
     const int token = item / nq, head = item % nq;
     const int pos = positions[token];
+    if (pos < 0) return;               // (a planned batch: a row behind the last token)
     const int slots = min(max_chunks, row_chunk_count(row_keys(pos, window, keep)));
     float m = -INFINITY, l = 0.f, o[NE];
 #pragma unroll

@@ -29,8 +29,9 @@ struct Planner {
 
     int page(int r, int i) const { return tables[r * width + i]; }
 
-    // `set`: requests that agree on all pages in front of `from`; their keys in front of `key` belong to segments
-    void walk(const std::vector<int>& set, int from, int key) {
+    // `set`: requests that agree on all pages in front of `from`; their keys in front of `key` belong to segments.  Beyond DEEPEST branchings requests go on alone (the stack is the caller's).
+    static constexpr int DEEPEST = 256;
+    void walk(const std::vector<int>& set, int from, int key, int depth) {
         std::vector<int> next;
         for (int r : set)
             if (share[r] > from) next.push_back(r);
@@ -56,7 +57,7 @@ struct Planner {
                     members.insert(members.end(), group.begin(), group.end());
                     for (int r : group) cover[r] = hi;
                 } else hi = key;
-                walk(group, p, hi);
+                if (depth < DEEPEST) walk(group, p, hi, depth + 1);
             }
             i = j;
         }
@@ -96,7 +97,7 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             all.push_back(r);
         }
         start[R] = (int)total;
-        p.walk(all, 0, 0);
+        p.walk(all, 0, 0, 0);
         long long saved = 0;
         for (const Segment& s : p.segments) saved += (long long)(s.count - 1) * (s.key_hi - s.key_lo);
         for (int r : all) {
@@ -222,6 +223,7 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
         if (used > 0x7fffffff) return WLLM_BAD_SIZE;
         if (used > room) return OUT_TOO_SMALL;
         std::fill(out, out + used, 0);
+        std::fill(out + at_positions + total, out + at_positions + cap[3], -1);      // rows behind the last token: passed by
         out[PLAN_ITEMS] = (int)need[0]; out[PLAN_TOKENS] = (int)total; out[PLAN_AT_ITEMS] = (int)at_items; out[PLAN_AT_TOKENS] = (int)at_tokens;
         out[PLAN_AT_STARTS] = (int)at_starts; out[PLAN_AT_RESULTS] = (int)at_results; out[PLAN_AT_POSITIONS] = (int)at_positions; out[PLAN_ROWS] = (int)rows;
         for (size_t i = 0; i < items.size(); ++i) {

@@ -854,6 +854,8 @@ def prefix_plan(tables, q_lens, ctx_lens, page_size: int, nq: int, nkv: int, hd:
     if not prefix_ok(nq, nkv, hd, vd, page_size, dtype):
         raise KernelError(f"prefix_plan: {nq} query heads on {nkv}, sizes {hd}/{vd}, pages of {page_size}, {dtype}: up to 128 query heads a key/value head in bfloat16, 32 in float32, "
                           "head sizes in steps of 8 up to 256, pages of a power of two of at least 16 tokens")
+    if caps is not None and (len(caps) != 4 or min(caps) < 1):
+        raise KernelError(f"prefix_plan: caps (items, tokens of items, results, tokens of the batch) of at least one, not {caps}")
     bf16 = dtype == torch.bfloat16
     status, *made = _host_calls().prefix_plan(tables, _numbers(q_lens), _numbers(ctx_lens), page_size, nq // nkv, nkv, prefix_rows(dtype), 128 if bf16 else SIMT_CHUNK,
                                               1 if bf16 else SIMT_CHUNK, max(1, min_keys), sm_count() if bf16 else 2 * sm_count(), torch.cuda.is_available(), _prefix_costs(dtype, hd, vd), (0, 0, 0, 0) if caps is None else caps)

@@ -13,6 +13,7 @@ def always(monkeypatch):
     """Shared pages are attended to once however few they are."""
     from wllm_b200.kernels import ops
     monkeypatch.setattr(ops, "PREFIX_SAVED", {2: 1, 4: 1})
+    monkeypatch.setattr(ops, "PREFIX_PORTION", (1, 0.0))
     plan = ops.prefix_plan
     monkeypatch.setattr(ops, "prefix_plan", lambda *a, **k: plan(*a, **{**k, "min_keys": 1}))
 

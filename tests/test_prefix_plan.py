@@ -120,6 +120,14 @@ def test_refusals():
             ops.prefix_plan(**{**good, **wrong})
 
 
+def test_when_sharing_pays():
+    pays = lambda saved, dtype=torch.bfloat16, nkv=1, **kw: ops.prefix_pays(saved, nkv, 256, 256, dtype, **kw)  # noqa: E731
+    assert pays(24 << 10) and not pays((24 << 10) - 1) and pays(128, torch.float32) and not pays(127, torch.float32)
+    assert pays(3 * 512, holders=4, tokens=1.5) and not pays(3 * 512 - 1, holders=4, tokens=1.5)
+    assert not pays(3 * 512, nkv=16, holders=4, tokens=100) and pays(3 * 1120, nkv=16, holders=4, tokens=100)
+    assert not pays(0, holders=1, tokens=2) and not pays(0)
+
+
 def test_a_long_chain_of_branchings():
     """Every request leaves the others one page after the last: the plan follows some hundred of them and is right for all."""
     n = 400

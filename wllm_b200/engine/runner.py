@@ -188,7 +188,8 @@ class ModelRunner:
     def _prefix_plans(self, entries: list, host, offsets, shape, fixed: bool):
         """(host array, {layout: plan}): what the step's attention reads of shared pages, behind the index arrays; nothing where no pages are shared or it would not pay.  `fixed`: for a captured
         step, whose array lies at the same place whatever the batch holds."""
-        if not self.prefix_layouts or sum(e.cache.forked > 0 for e in entries) < 2:
+        holders = sum(e.cache.forked > 0 for e in entries)
+        if not self.prefix_layouts or holders < 2:
             return host, {}
         (N, R, P), plans, parts = shape, {}, [host]
 
@@ -196,14 +197,15 @@ class ModelRunner:
             o, n = offsets[name]
             return host[o:o + n]
         lens, ctx_lens, total = view("req_q_len").tolist(), view("req_ctx_len").tolist(), host.shape[0]
+        tokens = sum(lens) / len(entries)
         for layout in self.prefix_layouts:
             g, nq, nkv, hd, vd = layout
             saved = sum(e.cache.forked for e in entries)          # (no more keys than that can be shared)
-            if not ops.prefix_pays(saved, nkv, hd, vd, self.model.dtype):
+            if not ops.prefix_pays(saved, nkv, hd, vd, self.model.dtype, holders, tokens):
                 continue
             plan = ops.prefix_plan(view(f"table{g}").reshape(R, P), lens, ctx_lens, self.cache.page_size, nq, nkv, hd, vd, self.model.dtype,
                                    caps=ops.prefix_caps(R, nkv) if fixed else None)
-            if plan is None or not ops.prefix_pays(plan.saved_keys, nkv, hd, vd, self.model.dtype) or plan.scratch_floats > PREFIX_SCRATCH:
+            if plan is None or not ops.prefix_pays(plan.saved_keys, nkv, hd, vd, self.model.dtype, holders, tokens) or plan.scratch_floats > PREFIX_SCRATCH:
                 continue
             plans[layout] = plan
             offsets[("prefix", layout)] = (total, plan.used)

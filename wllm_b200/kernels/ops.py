@@ -832,9 +832,17 @@ def prefix_ok(nq: int, nkv: int, hd: int, vd: int, page_size: int, dtype: torch.
 PREFIX_SAVED = {2: 24 << 20, 4: 1 << 18}
 
 
-def prefix_pays(saved_keys: int, nkv: int, hd: int, vd: int, dtype: torch.dtype) -> bool:
-    """Whether a step reads shared keys once for all, from the keys (times further holders) that it then reads less often."""
+# Steps with portions of several tokens in bfloat16: shared keys a holder, at the least, and at the least so many times the mean portion's tokens and kv heads.  There the other attention is a chain over
+# each portion's keys, until the portions alone fill the device (us, it and prefix_attention: 8 heads of 256 on one, 2 portions of 9 on 256 keys 11.7 and 11.1, on 1,000 25.1 and 12.4, 20 of 100 on 512
+# 21.7 and 23.8, on 3,000 51 and 47; 16 on 16, 2 of 30 on 256 11.8 and 13.4, on 512 15.9 and 12.8, 6 of 100 on 512 20.7 and 27.9, on 3,000 63 and 46; 16 on 4 of 128, 20 of 9 on 512 26.2 and 11.1).
+PREFIX_PORTION = (512, 0.7)
+
+
+def prefix_pays(saved_keys: int, nkv: int, hd: int, vd: int, dtype: torch.dtype, holders: int = 2, tokens: float = 1.0) -> bool:
+    """Whether a step reads shared keys once for all, from the keys (times further holders) that it then reads less often, the requests that hold some, and the mean of the requests' new tokens."""
     item = 2 if dtype == torch.bfloat16 else 4
+    if item == 2 and tokens > 1:
+        return saved_keys >= (holders - 1) * max(PREFIX_PORTION[0], PREFIX_PORTION[1] * tokens * nkv) > 0
     return saved_keys * nkv * (hd + vd) * item >= PREFIX_SAVED[item]
 
 

@@ -816,7 +816,7 @@ def _prefix_costs(dtype: torch.dtype, hd: int, vd: int) -> tuple:
     out = -(-vd // 64) * 64
     wide = 256 if hd > 128 and out == 256 else -(-hd // 64) * 64      # as csrc/prefix_attention.cu widens them
     tile = max(100 * wide // 16 + 85 * 8 * out // 128, 1500 if out <= 128 else 3000)
-    return tile, 3500, max(256 * (hd + vd) // 44, 1500), 2500, 16, 3 * vd, 2 if wide <= 192 else 1
+    return tile, 3500, max(256 * (hd + vd) // 44, 1500), 2500, 16, 5 * vd, 2 if wide <= 192 else 1
 
 
 def prefix_ok(nq: int, nkv: int, hd: int, vd: int, page_size: int, dtype: torch.dtype) -> bool:

@@ -783,7 +783,7 @@ class PrefixPlan:
         if caps is not None:          # laid out for any plan of that size: the kernels read from it how many items there are
             n_tokens, rows, max_ctx = caps[3], caps[2] * (key[1] // key[2]), width * key[0]
         self.key, self.requests, self.width, self.n_tokens = key, requests, width, n_tokens
-        self.host = host[:used]                # int32 on the host, pinned where there is a device
+        self.host = host[:used]                # int32 on the host (more than 64 KB of it pinned, where there is a device)
         self.used, self.items, self.rows, self.saved_keys, self.most_results, self.tiles = used, items, rows, saved, most, tiles
         page_size, nq, nkv, hd, vd, dtype = key
         self.max_chunks = max(1, -(-max_ctx // SIMT_CHUNK))

@@ -17,6 +17,8 @@
 #include <algorithm>
 #include <vector>
 
+#include "prefix_plan.cuh"
+
 namespace {
 
 struct Failed {};                      // a Python error is set
@@ -456,7 +458,7 @@ PyObject* copy_pages(Args v, Py_ssize_t n) {
 }
 
 // tables, q_lens, ctx_lens, page_size, query heads a kv head, kv heads, rows of an item, keys of a tile, align, min_keys, CTAs at once, pinned memory, costs (seven), caps (four)
-//   -> (status, the plan's array, ints used, items, rows, keys saved, most results, tiles, tokens, longest context)
+//   -> (status, the plan's array, ints used, items, rows, keys saved, most results, tiles, tokens, longest context, the places of items, tokens and positions in the array)
 PyObject* prefix_plan(Args v, Py_ssize_t n) {
     count(n, 14);
     const std::vector<int> costs = numbers(v[12], "costs", 7), caps = numbers(v[13], "caps", 4);
@@ -505,7 +507,8 @@ PyObject* prefix_plan(Args v, Py_ssize_t n) {
     const bool sound = PyLong_AsLong(status) == 0;
     at::Tensor host = at::empty({sound ? (int64_t)info[0] : 0}, at::TensorOptions().dtype(at::kInt).pinned_memory(truth(v[11]) && info[0] > (64 << 10) / 4));
     if (sound) std::copy(made.begin(), made.begin() + info[0], static_cast<int*>(host.data_ptr()));
-    return Py_BuildValue("(NNLLLLLLLL)", status, THPVariable_Wrap(host), info[0], info[1], info[2], info[3], info[4], info[5], tokens, longest);
+    const int *head = made.data(), at_items = sound ? head[PLAN_AT_ITEMS] : 0, at_tokens = sound ? head[PLAN_AT_TOKENS] : 0, at_positions = sound ? head[PLAN_AT_POSITIONS] : 0;
+    return Py_BuildValue("(NNLLLLLLLLiii)", status, THPVariable_Wrap(host), info[0], info[1], info[2], info[3], info[4], info[5], tokens, longest, at_items, at_tokens, at_positions);
 }
 
 // q, out, k_pages, v_pages, block_table, arrays, scratch, status, sinks, slopes, tokens, requests, width, ints of the plan, floats of scratch, rows, pairs, place of the positions,

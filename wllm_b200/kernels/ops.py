@@ -779,19 +779,20 @@ class PrefixPlan:
     """How a batch whose requests share pages is attended to (csrc/prefix_plan.cuh): made once for a step and a layout of heads, read by every layer of it."""
     __slots__ = ("key", "requests", "width", "n_tokens", "host", "used", "items", "rows", "saved_keys", "most_results", "tiles", "max_chunks", "scratch_floats", "launch", "places")
 
-    def __init__(self, key: tuple, requests: int, width: int, caps, host: torch.Tensor, used: int, items: int, rows: int, saved: int, most: int, tiles: int, n_tokens: int, max_ctx: int):
+    def __init__(self, key: tuple, requests: int, width: int, caps, host: torch.Tensor, used: int, items: int, rows: int, saved: int, most: int, tiles: int, n_tokens: int, max_ctx: int,
+                 at_items: int, at_tokens: int, at_positions: int):
         if caps is not None:          # laid out for any plan of that size: the kernels read from it how many items there are
             n_tokens, rows, max_ctx = caps[3], caps[2] * (key[1] // key[2]), width * key[0]
         self.key, self.requests, self.width, self.n_tokens = key, requests, width, n_tokens
-        self.host = host[:used]                # int32 on the host (more than 64 KB of it pinned, where there is a device)
+        self.host = host                       # int32 on the host (more than 64 KB of it pinned, where there is a device)
         self.used, self.items, self.rows, self.saved_keys, self.most_results, self.tiles = used, items, rows, saved, most, tiles
         page_size, nq, nkv, hd, vd, dtype = key
         self.max_chunks = max(1, -(-max_ctx // SIMT_CHUNK))
         self.scratch_floats = nkv * rows * (vd + 2) if dtype == torch.bfloat16 else n_tokens * nq * self.max_chunks * (vd + 2)
         # what the native call takes of it
         pairs = (items if caps is None else caps[0]) * nkv
-        self.launch = (n_tokens, requests, width, used, self.scratch_floats, rows, pairs, int(host[6]) if used else 0, self.max_chunks, nq, nkv, hd, vd, page_size)
-        self.places = (int(host[2]), int(host[3]), items if caps is None else -1) if used else (0, 0, 0)
+        self.launch = (n_tokens, requests, width, used, self.scratch_floats, rows, pairs, at_positions, self.max_chunks, nq, nkv, hd, vd, page_size)
+        self.places = (at_items, at_tokens, items if caps is None else -1)
 
     def to(self, device) -> torch.Tensor:
         """The plan's array on the device, as prefix_attention takes it (in the current stream's order)."""
@@ -804,6 +805,11 @@ PREFIX_MIN_KEYS = 128
 def prefix_rows(dtype: torch.dtype) -> int:
     """Rows (token, query head of the group) of an item of a plan, at most."""
     return 128 if dtype == torch.bfloat16 else 32
+
+
+@functools.lru_cache(maxsize=None)
+def _pinning() -> bool:
+    return torch.cuda.is_available()
 
 
 @functools.lru_cache(maxsize=None)
@@ -866,7 +872,7 @@ def prefix_plan(tables, q_lens, ctx_lens, page_size: int, nq: int, nkv: int, hd:
         raise KernelError(f"prefix_plan: caps (items, tokens of items, results, tokens of the batch) of at least one, not {caps}")
     bf16 = dtype == torch.bfloat16
     status, *made = _host_calls().prefix_plan(tables, _numbers(q_lens), _numbers(ctx_lens), page_size, nq // nkv, nkv, prefix_rows(dtype), 128 if bf16 else SIMT_CHUNK,
-                                              1 if bf16 else SIMT_CHUNK, max(1, min_keys), sm_count() if bf16 else 2 * sm_count(), torch.cuda.is_available(), _prefix_costs(dtype, hd, vd), (0, 0, 0, 0) if caps is None else caps)
+                                              1 if bf16 else SIMT_CHUNK, max(1, min_keys), sm_count() if bf16 else 2 * sm_count(), _pinning(), _prefix_costs(dtype, hd, vd), (0, 0, 0, 0) if caps is None else caps)
     if status == 2 and caps is not None:
         return None
     if status:

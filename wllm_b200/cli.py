@@ -9,6 +9,7 @@ Engine options carry the reference's names and meanings (src/wllm/cli.py:21-56):
 server; servers are outside this engine, so the command generates instead, and the
 sampling options of the reference's requests (temperature, top_k, top_p, min_p,
 repetition_penalty, seed, max_tokens; src/wllm/api/schemas.py:30-47) become flags.
+--prefix-ids (tokens that every prompt begins with) and --n (samples of a prompt) have no counterpart there.
 """
 from __future__ import annotations
 

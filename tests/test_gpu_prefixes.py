@@ -138,6 +138,40 @@ def test_samples_without_room_for_their_prompt_beside_them(tmp_path):
         assert llm.runner.cache.free_pages() == [blocks] * len(llm.runner.cache.groups) and not llm.scheduler.prefixes
 
 
+@pytest.mark.parametrize("name,asynchronous", [("A", False), ("A", True), ("gudarax", False), ("zafilix", False)])
+def test_another_size_of_the_cache_and_new_requests_between_steps(tmp_path, always, name, asynchronous):
+    """The cache grows and shrinks while requests decode and a prefix is half computed; requests come, are cancelled and begin with prefixes between steps."""
+    folder = folders(tmp_path)[name]()
+    kw = dict(dtype="float32", block_size=16, chunked_prefill_tokens=24)
+    llm, plain = LLM(folder, num_blocks=40, cuda_graphs=True, async_scheduling=asynchronous, poison_pages=True, **kw), LLM(folder, num_blocks=96, **kw)
+    vocab = llm.model.plan.vocab_size
+    sp = SamplingParams(max_tokens=14, ignore_eos=True)
+    first = [llm.add_request(tokens(20 + 9 * i, vocab, i), sp) for i in range(2)]
+    for _ in range(5):
+        llm.step()
+    prefix = llm.add_prefix(tokens(50, vocab, 7))
+    behind = [llm.add_request(tokens(1 + 6 * i, vocab, 20 + i), sp, prefix=prefix) for i in range(3)]
+    gone = llm.add_request(tokens(9, vocab, 40), sp, prefix=prefix)
+    llm.step()
+    llm.resize_cache(64)
+    for _ in range(6):
+        llm.step()
+    assert llm.scheduler.cancel(gone.request_id)
+    llm.resize_cache(36)
+    llm.step()
+    late = llm.add_request(tokens(4, vocab, 30), SamplingParams(max_tokens=14, ignore_eos=True, n=2, seed=3, temperature=0.7), prefix=prefix)
+    llm.step()
+    llm.resize_cache(50)
+    llm.scheduler.run_to_completion()
+    llm.runner.cache.check()
+    for r in first + behind:
+        assert r.output_token_ids == plain.generate([r.prompt_token_ids], sp)[0].token_ids
+    want = plain.generate([late[0].prompt_token_ids], SamplingParams(max_tokens=14, ignore_eos=True, n=2, seed=3, temperature=0.7))
+    assert [r.output_token_ids for r in late] == [o.token_ids for o in want]
+    llm.drop_prefix(prefix)
+    assert llm.runner.cache.free_pages() == [50] * len(llm.runner.cache.groups) and not llm.scheduler.prefixes
+
+
 def test_the_command(tmp_path, capsys):
     import json
 

@@ -35,8 +35,6 @@
 #include "tc_common.cuh"
 #include "prefix_plan.cuh"
 
-#include <mutex>
-#include <unordered_map>
 
 #if !defined(HEAD_DIM) || !defined(VALUE_DIM)
 #error "compile with -DHEAD_DIM=<key head size> -DVALUE_DIM=<value head size>"

@@ -35,7 +35,6 @@
 #include "tc_common.cuh"
 #include "prefix_plan.cuh"
 
-
 #if !defined(HEAD_DIM) || !defined(VALUE_DIM)
 #error "compile with -DHEAD_DIM=<key head size> -DVALUE_DIM=<value head size>"
 #endif

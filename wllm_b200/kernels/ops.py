@@ -883,8 +883,9 @@ def prefix_plan(tables, q_lens, ctx_lens, page_size: int, nq: int, nkv: int, hd:
 def prefix_attention(q, out, k_pages, v_pages, block_table, plan: PrefixPlan, arrays: torch.Tensor, nq: int, nkv: int, hd: int, page_size: int, scale: float, scratch: torch.Tensor,
                      vd: int | None = None, sinks: torch.Tensor | None = None, cap: float = 0.0, slopes: torch.Tensor | None = None) -> None:
     """Attention of a planned batch (csrc/prefix_attention.cu; 32-bit: csrc/attention_simt.cu, bit for bit what the other 32-bit kernels give): q [tokens, nq * hd] (row stride free),
-    out [tokens, nq * vd], pages [pages, nkv, page_size, hd | vd], `block_table` [requests, pages] the tables of the plan on the device, `arrays` = plan.to(device), `scratch` float32 of at
-    least plan.scratch_floats, which the call alone uses while it runs.  Every earlier key is seen (no window).  `sinks`, `cap`, `slopes`: as for attention_mma_decode."""
+    out [tokens, nq * vd], pages [pages, nkv, page_size, hd | vd], `block_table` [requests, pages] the tables of the plan on the device, `arrays` = plan.to(device) (or its numbers copied
+    from the host into an array of their own: they are looked at before the kernel in front has ended, so no kernel may be what writes them), `scratch` float32 of at least plan.scratch_floats, which the
+    call alone uses while it runs.  A new value that is no number reaches all new tokens of its own request.  Every earlier key is seen (no window).  `sinks`, `cap`, `slopes`: as for attention_mma_decode."""
     if plan.key != (page_size, nq, nkv, hd, hd if vd is None else vd, q.dtype):
         raise KernelError(f"prefix_attention: a plan for (page size, heads, kv heads, sizes, type) {plan.key}, not {(page_size, nq, nkv, hd, hd if vd is None else vd, q.dtype)}")
     if plan.n_tokens == 0:

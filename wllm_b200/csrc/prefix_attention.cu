@@ -581,11 +581,13 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                     }
                 }
                 while (use < begin + T * (KC + VC)) { landed(); handed(); }
+                // (The second group without a tile leaves no result: its sums are read by nobody, and a warp that stored them here could overtake the one that still reads the item before's,
+                // which only a tile's barrier holds back.)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
                     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-                    if ((lane & 3) == 0) l_all[w * THIN + (lane >> 2) + 8 * i] = l[i] * __uint_as_float(power(mw[i] - (m[i] == -INFINITY ? 0.f : m[i])));
+                    if ((lane & 3) == 0 && (side == 0 || T > 1)) l_all[w * THIN + (lane >> 2) + 8 * i] = l[i] * __uint_as_float(power(mw[i] - (m[i] == -INFINITY ? 0.f : m[i])));
                 }
                 if (!all_of_groups(ok)) {
                     if (!ok) atomicExch(p.status, GAVE_UP_SOFTMAX);

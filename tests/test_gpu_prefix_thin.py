@@ -35,3 +35,14 @@ def test_items_of_one_tile_behind_longer_ones(nq, nkv, hd, vd):
     b = Batch((256, [(n, 1) for n in lengths(600 // nkv, hd + vd)]), nq, nkv, hd, vd, 16, seed=hd, dtype=BF16)
     plan = check(b, 6)
     assert plan.items * nkv > 3 * 148 and plan.saved_keys > 0
+
+
+@pytest.mark.parametrize("nq,nkv,hd,vd", [(8, 1, 128, 256), (16, 2, 128, 128), (4, 1, 64, 64), (8, 1, 256, 256)])
+def test_long_runs_of_thin_items_with_wide_ones_between(nq, nkv, hd, vd):
+    """Thin items go on without the thread that issues the tensor core's products, wide ones wait for it: runs of the one kind between the others, eight items and more a multiprocessor."""
+    g = torch.Generator().manual_seed(hd)
+    draw = lambda n: int(torch.randint(0, n, (1,), generator=g))  # noqa: E731
+    groups = [(128 * (1 + i % 4), [(draw(700 if i % 3 else 60), 1) for _ in range(32 if i % 5 else 3)]) for i in range(48)]
+    b = Batch((0, groups), nq, nkv, hd, vd, 64, seed=vd, dtype=BF16)
+    plan = check(b, 6, min_keys=1)
+    assert plan.items * nkv > 8 * 148 and plan.saved_keys > 0

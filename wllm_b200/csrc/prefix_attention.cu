@@ -193,7 +193,7 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
         for (int s = 0; s < STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 8); }
         for (int b = 0; b < BUFS; ++b) { mbar_init(s_full + 8 * b, 1); mbar_init(p_full + 8 * b, 4); mbar_init(pv_done + 8 * b, 1); }
         mbar_init(q_full, 2); mbar_init(q_empty, 8);
-        mbar_init(begun, 8); mbar_init(o_free, 8);
+        mbar_init(begun, 9); mbar_init(o_free, 8);
         for (int i = 0; i < 8; ++i) mbar_init(m_ready + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -327,17 +327,19 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                     const Item item = next;
                     next = item_of(pair_at(k + 1));
                     const int T = (item.hi - item.lo + BN - 1) / BN;
+                    // A wait cannot tell two rounds of a barrier from none.  Thin items go on without this thread, so it has its part in `begun`: the next item's queries come when it has seen this one's.
                     if (!mbar_wait(q_full, k & 1)) { ok = false; break; }
+                    mbar_arrive(begun);
                     if (item.tokens * rep <= THIN) {
                         use += T * (KC + VC);
-                        if (k > 0 && !mbar_wait(o_free, (k - 1) & 1)) ok = false;
                         continue;
                     }
                     tc_fence_after();
                     // K 0, K 1, (K 2,) V 0, K 2 (3), V 1, ...
                     for (int n = 0; n < BUFS && n < T && ok; ++n) ok = scores(tile + n);
                     if (T <= BUFS) hand_back(q_empty);
-                    // the first product with the values waits until the groups have read the outputs of the item before
+                    // The first product with the values waits until the groups have read the outputs of the item before (they began that item when they were through with those before it, and
+                    // cannot end this one without the product: the round waited for is the last or the next).
                     if (ok && k > 0) ok = mbar_wait(o_free, (k - 1) & 1);
                     tc_fence_after();
                     for (int n = 0; n < T && ok; ++n) {

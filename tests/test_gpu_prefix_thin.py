@@ -46,3 +46,11 @@ def test_long_runs_of_thin_items_with_wide_ones_between(nq, nkv, hd, vd):
     b = Batch((0, groups), nq, nkv, hd, vd, 64, seed=vd, dtype=BF16)
     plan = check(b, 6, min_keys=1)
     assert plan.items * nkv > 8 * 148 and plan.saved_keys > 0
+
+
+@pytest.mark.parametrize("nq,nkv,hd,vd", [(8, 1, 128, 256), (16, 4, 128, 128), (4, 1, 64, 64), (8, 1, 256, 256)])
+@pytest.mark.parametrize("ps", [16, 128])
+def test_values_cleared_behind_the_last_key_leave_the_next_tile_alone(nq, nkv, hd, vd, ps):
+    """Tiles that hold a few keys, their other rows cleared in a stage of the ring that the next item's full tiles are brought to."""
+    own = [(1 + i % 120) if i % 2 else 127 + 128 * (i % 3) for i in range(400 // nkv)]
+    check(Batch((0, [(n, 1) for n in own]), nq, nkv, hd, vd, ps, seed=ps, dtype=BF16), 6)

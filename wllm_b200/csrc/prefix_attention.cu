@@ -565,6 +565,7 @@ prefix_kernel(const __grid_constant__ Prefix p, const __grid_constant__ CUtensor
                                     for (int j = 0; j < NT; ++j)
                                         asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + ((col0 + j) >> 3) * (BN * 128) + r * 128 + ((((col0 + j) ^ r) & 7) << 4)), "r"(0u)
                                                      : "memory");
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // (the stage's next tile comes by TMA: not before these)
                                 __syncwarp();
                             }
 #pragma unroll

@@ -175,3 +175,47 @@ def test_samples_draw_from_seeds_of_their_own():
     assert seeds[0] == 7 and len(set(seeds)) == 100 and all(0 <= x < 1 << 63 for x in seeds[1:])
     with pytest.raises(ValueError):
         SamplingParams(n=0)
+
+
+def test_ids_that_callers_choose_meet_no_prefix():
+    """Samples are named (id of the prompt, sample): also those of a prompt called "prefix" are nobody else."""
+    runner, s = make()
+    prefix = s.add_prefix([1, 2, 3, 4, 5], auto=True)
+    reqs = [request(("prefix", k), prefix.token_ids + [7], prefix) for k in range(2)]
+    for r in reqs:
+        s.add_request(r)
+    s.run_to_completion()
+    assert [r.output_token_ids for r in reqs] == [alone(r.prompt_token_ids) for r in reqs]
+    assert prefix.dropped and runner.cache.free_pages() == [24]
+
+
+@pytest.mark.parametrize("name", ["fork", "open"])
+def test_a_request_whose_cache_cannot_be_made_stays_in_the_queue(monkeypatch, name):
+    runner, s = make()
+    prefix = s.add_prefix([1, 2, 3, 4, 5], auto=True)
+    r = request("r", prefix.token_ids + [7], prefix)
+    s.add_request(r)
+    s.step()
+    if name == "open":
+        s.add_request(request("first", [9], max_tokens=1))
+    wrong, right = s.waiting[-1 if name == "open" else 0], getattr(runner.cache, name)
+    s.waiting = [wrong] + [x for x in s.waiting if x is not wrong]
+
+    def fail(*args, **kw):
+        raise MemoryError("no copy")
+    monkeypatch.setattr(runner.cache, name, fail)
+    with pytest.raises(MemoryError):
+        s.step()
+    assert s.waiting[0] is wrong and wrong not in s.live and wrong.cache is None and prefix.users == 1
+    monkeypatch.setattr(runner.cache, name, right)
+    s.run_to_completion()
+    assert r.output_token_ids == alone(r.prompt_token_ids) and prefix.dropped and runner.cache.free_pages() == [24]
+
+
+def test_one_id_twice_is_run_one_behind_the_other():
+    runner, s = make()
+    pair = [request("same", [4, 9], max_tokens=3), request("same", [8], max_tokens=2)]
+    for r in pair:
+        s.add_request(r)
+    s.run_to_completion()
+    assert [r.output_token_ids for r in pair] == [alone([4, 9], 3), alone([8], 2)] and runner.cache.free_pages() == [24]

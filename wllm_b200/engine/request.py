@@ -71,6 +71,16 @@ class Request:
         return self.status == RequestStatus.FINISHED
 
 
+class PrefixId:
+    """The request id of a prefix's holder: like no id that a caller may choose."""
+
+    def __init__(self, number: int):
+        self.number = number
+
+    def __repr__(self) -> str:
+        return f"prefix {self.number}"
+
+
 @dataclass(eq=False)
 class Prefix:
     """Tokens that several requests begin with: computed once, kept in the cache, forked for every request that names it.  Its holder is an entry of the scheduler's

@@ -56,7 +56,7 @@ import random
 
 from ..cache import OutOfPages
 from ..sampling.params import SamplingParams
-from .request import Prefix, Request, RequestStatus
+from .request import Prefix, PrefixId, Request, RequestStatus
 from .runner import StepEntry
 
 
@@ -144,7 +144,7 @@ class Scheduler:
         refusal = self.prefix_refusal(len(token_ids), prefix)
         if refusal:
             raise ValueError(refusal)
-        holder = Request(("prefix", self._prefix_id), token_ids, SamplingParams(max_tokens=1), prefix=prefix, holds=True)
+        holder = Request(PrefixId(self._prefix_id), token_ids, SamplingParams(max_tokens=1), prefix=prefix, holds=True)
         self.add_request(holder)
         self._prefix_id += 1
         made = Prefix(holder.prompt_token_ids, holder, auto)
@@ -214,6 +214,8 @@ class Scheduler:
     def _may_admit(self, r: Request, taken_now: int) -> bool:
         if len(self.live) >= self.max_num_seqs or self.cache.slots.num_free == 0:
             return False
+        if r.request_id in self.cache.live:      # another request of that id has to be over first
+            return False
         if r.prefix is not None and not r.prefix.ready:
             return False
         shared = len(r.prefix.token_ids) // self.cache.page_size if r.prefix is not None else 0
@@ -274,8 +276,9 @@ class Scheduler:
             r = self.waiting[0]
             if not self._may_admit(r, taken):
                 break                                       # the head of the queue blocks the rest
-            self.waiting.pop(0)
+            # (in the queue until it has a cache: nothing is lost when there is an error)
             r.cache = self.cache.open(r.request_id) if r.prefix is None else self.cache.fork(r.prefix.holder.cache, r.request_id)
+            self.waiting.pop(0)
             r.num_computed = r.cache.num_tokens
             r.status = RequestStatus.PREFILLING
             self.live.append(r)

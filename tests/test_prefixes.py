@@ -219,3 +219,35 @@ def test_one_id_twice_is_run_one_behind_the_other():
         s.add_request(r)
     s.run_to_completion()
     assert [r.output_token_ids for r in pair] == [alone([4, 9], 3), alone([8], 2)] and runner.cache.free_pages() == [24]
+
+
+@pytest.mark.parametrize("admission", ["worst_case", "optimistic"])
+@pytest.mark.parametrize("async_scheduling", [False, True])
+def test_what_was_made_for_a_few_refuses_nothing_behind_them(admission, async_scheduling):
+    """A request that would not fit beside the prompt of the samples in front of it fits when they are over, as it does when it is added first."""
+    runner, s = make(pages=12, admission=admission, async_scheduling=async_scheduling)
+    for turn in range(2):
+        begin = [(7 * i + turn) % 50 for i in range(22)]              # 6 pages
+        prefix = s.add_prefix(begin, auto=True)
+        few = [request(("few", k), begin + [k], prefix, max_tokens=5) for k in range(3)]
+        big = request("big", [(3 * i) % 50 for i in range(30)], max_tokens=14)      # 11 pages
+        small = request("small", [5], max_tokens=3)
+        for r in few + [big, small]:
+            s.add_request(r)
+        with pytest.raises(ValueError, match="pages"):                # what it would need beside what is kept now
+            s.add_prefix([1] * 8)
+        while s.has_unfinished():
+            s.step()
+            runner.cache.check()
+        assert [r.output_token_ids for r in few + [big, small]] == [alone(r.prompt_token_ids, r.sampling.max_tokens) for r in few + [big, small]]
+        assert prefix.dropped and runner.cache.free_pages() == [12]
+    kept = s.add_prefix([1] * 8)                                      # one that is kept counts, and so does a request's own
+    with pytest.raises(ValueError, match="for prefixes"):
+        s.add_request(request("big", range(30), max_tokens=14))
+    nested = s.add_prefix([1] * 30, prefix=kept, auto=True)
+    with pytest.raises(ValueError, match="for prefixes"):
+        s.add_request(request("own", [1] * 31, nested, max_tokens=14))          # 12 pages, 7 of them the prefix's, which has one more
+    own = request("own", [1] * 31, nested, max_tokens=10)
+    s.add_request(own)
+    s.run_to_completion()
+    assert own.output_token_ids == alone([1] * 31, 10) and nested.dropped

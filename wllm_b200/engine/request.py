@@ -36,6 +36,7 @@ class Request:
     inflight_row: int = -1        # that token's row among the sampled tokens of the step before
     prefix: object = None         # the Prefix that it begins with: its cache is forked from the prefix's
     holds: bool = False           # it is the tokens of a prefix: computed and kept, nothing is sampled
+    order: int = -1               # its place among all that were added
 
     @property
     def num_tokens(self) -> int:

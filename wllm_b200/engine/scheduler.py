@@ -77,7 +77,7 @@ class Scheduler:
         self._rng = random.Random(seed)
         self.async_scheduling = async_scheduling
         self.prefixes: list = []      # those that are not dropped
-        self._prefix_id = 0
+        self._prefix_id = self._added = 0
         self._inflight = None         # (PendingSample, [(request, keep)]) of the step whose tokens are unread
         self.stats = {"steps": 0, "prefill_tokens": 0, "decode_tokens": 0, "preemptions": 0, "finished": 0,
                       "dropped_tokens": 0}
@@ -105,21 +105,27 @@ class Scheduler:
             if n <= len(begin) or request.prompt_token_ids[:len(begin)] != begin:
                 raise ValueError(f"request {request.request_id!r}: a prompt that names a prefix begins with its {len(begin)} tokens and has more")
         pool = min(g.pool.num_pages for g in self.cache.groups) if self.cache.groups else 1 << 30
+        request.order = self._added
         held = self._held_pages(request)
         if self._pages(worst) + held > pool:
             raise ValueError(f"request {request.request_id!r}: {worst} tokens need {self._pages(worst)} pages, "
                              f"the cache has {pool}{f', {held} of them for prefixes' if held else ''}; it could never finish")
         if request.prefix is not None:
             request.prefix.users += 1
+        self._added += 1
         request.status = RequestStatus.WAITING
         request.seed = request.sampling.seed if request.sampling.seed is not None else self._rng.getrandbits(63)
         self.waiting.append(request)
 
     def _held_pages(self, request: Request | None = None) -> int:
-        """Pages that prefixes hold, or will, which `request` does not share: all of them, but the full pages of its own."""
-        total = 0
+        """Pages that prefixes hold, or will, when `request` has run so far that it is the only one left, and which it does not share: not the full pages of its own, nor what was made for a
+        few requests in front of it (they are live in front of it or over)."""
+        total, mine, x = 0, [], request.prefix if request is not None else None
+        while x is not None:                     # its prefix, what that begins with, ...
+            mine.append(x)
+            x = x.holder.prefix
         for x in self.prefixes:
-            if x.holder is request:
+            if x.holder is request or (request is not None and x.auto and x.holder.order < request.order and x not in mine):
                 continue
             shared = len(x.holder.prefix.token_ids) // self.cache.page_size if x.holder.prefix is not None else 0
             total += self._pages(len(x.token_ids)) - shared

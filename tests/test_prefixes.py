@@ -251,3 +251,100 @@ def test_what_was_made_for_a_few_refuses_nothing_behind_them(admission, async_sc
     s.add_request(own)
     s.run_to_completion()
     assert own.output_token_ids == alone([1] * 31, 10) and nested.dropped
+
+
+def samples_of(s, i, prompt, n, max_tokens):
+    """n samples of a prompt, as the engine adds them: forks of all but its last token."""
+    prefix = s.add_prefix(prompt[:-1], auto=True)
+    reqs = [request((i, k), prompt, prefix, max_tokens=max_tokens) for k in range(n)]
+    for r in reqs:
+        s.add_request(r)
+    return reqs
+
+
+@pytest.mark.parametrize("budget", [None, 320])
+def test_prompts_with_samples_are_taken_on_together(budget):
+    """Sixteen prompts of four samples: their tokens in the first step, the samples from the second on; a request behind them runs in the first."""
+    runner = FakeRunner(600, max_requests=100)
+    s = Scheduler(runner, ArgmaxSampler(), chunked_prefill_tokens=budget)
+    reqs = [r for i in range(16) for r in samples_of(s, i, [(i + 3 * j) % 50 for j in range(20)], 4, 8)]
+    late = request("late", [9, 8, 7], max_tokens=8)
+    s.add_request(late)
+    s.step()
+    assert s.stats["prefill_tokens"] == 16 * 19 + 3 and len(late.output_token_ids) == 1
+    s.run_to_completion()
+    assert s.stats["steps"] == 9
+    assert all(r.output_token_ids == alone(r.prompt_token_ids, 8) for r in reqs + [late])
+    # whoever can run is taken in the order of the queue
+    first = [[rid for rid, _, _ in b] for b in runner.batches[1:2]][0]
+    assert first == ["late"] + [(i, k) for i in range(16) for k in range(4)]
+
+
+def test_who_waits_for_its_prefix_is_passed_only_by_those_that_fit_beside_it():
+    runner, s = make(pages=16, chunked_prefill_tokens=8)
+    few = samples_of(s, "few", [(7 * i) % 50 for i in range(30)], 2, 4)       # 29 tokens: 8 pages, for four steps
+    big = request("big", [(3 * i) % 50 for i in range(30)], max_tokens=6)     # 9 pages: not beside those
+    small = request("small", [5], max_tokens=3)
+    for r in (big, small):
+        s.add_request(r)
+    s.step()
+    assert [rid for rid, _, _ in runner.batches[0]] == [s.prefixes[0].holder.request_id] and not big.passed
+    s.run_to_completion()
+    assert all(r.output_token_ids == alone(r.prompt_token_ids, r.sampling.max_tokens) for r in few + [big, small])
+    runner, s = make(pages=24, chunked_prefill_tokens=8)
+    few = samples_of(s, "few", [(7 * i) % 50 for i in range(24)], 2, 4)
+    small = request("small", [5], max_tokens=9)
+    s.add_request(small)
+    for _ in range(3):
+        s.step()
+    assert small.passed and len(small.output_token_ids) > 0 and not few[0].output_token_ids
+    s.run_to_completion()
+    assert all(r.output_token_ids == alone(r.prompt_token_ids, r.sampling.max_tokens) for r in few + [small])
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_any_mixture_comes_to_an_end(seed):
+    """Prefixes that are kept, dropped or made for a few, requests with and without, cancelled ones, scarce pages and slots: everything that was taken on finishes with its own tokens."""
+    import random
+    rng = random.Random(seed)
+    pages, slots = rng.randint(6, 30), rng.choice([3, 5, 8, 20])
+    runner = FakeRunner(pages, max_requests=slots)
+    s = Scheduler(runner, ArgmaxSampler(), chunked_prefill_tokens=rng.choice([None, 5, 16]), admission=rng.choice(["worst_case", "optimistic"]), async_scheduling=rng.random() < 0.5)
+    reqs, kept, refused = [], [], 0
+    for turn in range(60):
+        for _ in range(rng.choice([0, 0, 1, 3])):
+            begin = rng.choice(kept) if kept and rng.random() < 0.4 else None
+            prompt = (begin.token_ids if begin else []) + [rng.randrange(50) for _ in range(rng.randint(1, 24))]
+            most, what = rng.randint(1, 12), rng.random()
+            try:
+                if what < 0.3 and len(prompt) - (len(begin.token_ids) if begin else 0) > 1 and not s.prefix_refusal(len(prompt) - 1, begin, len(prompt) + most):
+                    auto, made = s.add_prefix(prompt[:-1], prefix=begin, auto=True), []
+                    for k in range(rng.randint(1, 4)):
+                        made.append(request((turn, len(reqs) + k), prompt, auto, max_tokens=most))
+                        s.add_request(made[-1])
+                    reqs += made
+                elif what < 0.45:
+                    kept.append(s.add_prefix(prompt, prefix=begin))
+                else:
+                    r = request((turn, len(reqs)), prompt, begin, max_tokens=most)
+                    s.add_request(r)
+                    reqs.append(r)
+            except ValueError:
+                refused += 1
+        for p in [p for p in kept if p.users == 0 and rng.random() < 0.1]:
+            s.drop_prefix(p)
+            kept.remove(p)
+        if reqs and rng.random() < 0.1:
+            s.cancel(rng.choice(reqs).request_id)
+        if s.has_unfinished():
+            s.step()
+            runner.cache.check()
+    s.run_to_completion(max_steps=4000)
+    assert not s.has_unfinished() and all(r.finished for r in reqs)
+    for r in reqs:
+        if r.finish_reason != "cancelled":
+            assert r.output_token_ids == alone(r.prompt_token_ids, r.sampling.max_tokens), r.request_id
+    while any(not p.dropped for p in kept):
+        for p in [p for p in kept if not p.dropped and p.users == 0]:
+            s.drop_prefix(p)
+    assert runner.cache.free_pages() == [pages] and runner.cache.slots.num_free == slots and not s.prefixes

@@ -37,6 +37,7 @@ class Request:
     prefix: object = None         # the Prefix that it begins with: its cache is forked from the prefix's
     holds: bool = False           # it is the tokens of a prefix: computed and kept, nothing is sampled
     order: int = -1               # its place among all that were added
+    passed: bool = False          # admitted in front of some that wait for their prefix
 
     @property
     def num_tokens(self) -> int:

@@ -46,7 +46,8 @@ Policy, with the reference's rule beside it:
               is sampled for them, and their pages and state stay.  A request that names a
               prefix waits until it is ready and is admitted as a fork of it: it needs pages
               for what lies behind the prefix's full pages only, and computes its other
-              tokens.  Preempted, it is forked again.  A prefix's own pages are given back
+              tokens.  While its prefix is being computed, those behind it in the queue may
+              pass it, if they could finish beside all prefixes.  Preempted, it is forked again.  A prefix's own pages are given back
               when it is dropped, or, if it was made for a few requests alone (`auto`), when
               the last of them has finished.
 """
@@ -117,15 +118,16 @@ class Scheduler:
         request.seed = request.sampling.seed if request.sampling.seed is not None else self._rng.getrandbits(63)
         self.waiting.append(request)
 
-    def _held_pages(self, request: Request | None = None) -> int:
+    def _held_pages(self, request: Request | None = None, passing: bool = False) -> int:
         """Pages that prefixes hold, or will, when `request` has run so far that it is the only one left, and which it does not share: not the full pages of its own, nor what was made for a
-        few requests in front of it (they are live in front of it or over)."""
+        few requests in front of it (they are live in front of it or over, unless it has passed them)."""
+        passing = passing or request is None or request.passed
         total, mine, x = 0, [], request.prefix if request is not None else None
         while x is not None:                     # its prefix, what that begins with, ...
             mine.append(x)
             x = x.holder.prefix
         for x in self.prefixes:
-            if x.holder is request or (request is not None and x.auto and x.holder.order < request.order and x not in mine):
+            if x.holder is request or (not passing and x.auto and x.holder.order < request.order and x not in mine):
                 continue
             shared = len(x.holder.prefix.token_ids) // self.cache.page_size if x.holder.prefix is not None else 0
             total += self._pages(len(x.token_ids)) - shared
@@ -230,6 +232,11 @@ class Scheduler:
             return self._pages(min(r.worst_case_tokens, self.max_model_len)) - shared <= free - self._pledged()
         return self._pages(r.num_tokens) - shared <= free - taken_now
 
+    def _may_pass(self, r: Request) -> bool:
+        """Whether a request may be admitted in front of some that wait for their prefix: it could finish beside all prefixes, theirs too."""
+        pool = min((g.pool.num_pages for g in self.cache.groups), default=1 << 30)
+        return self._pages(min(r.worst_case_tokens, self.max_model_len)) + self._held_pages(r, passing=True) <= pool
+
     def _preempt_youngest(self) -> Request:
         victim = self.live.pop()
         self._release(victim)
@@ -278,13 +285,20 @@ class Scheduler:
             plan.append((r, r.num_computed, c))
         for r, _, c in plan:
             taken += max(self.cache.pages_needed([(r.cache, c)]), default=0)     # of the group that needs most
-        while self.waiting and budget > 0:
-            r = self.waiting[0]
+        at = 0                                              # requests in front of it wait for a prefix that is being computed
+        while at < len(self.waiting) and budget > 0:
+            r = self.waiting[at]
+            if r.prefix is not None and r.prefix.holder.status == RequestStatus.PREFILLING:
+                at += 1
+                continue
+            if at > 0 and not self._may_pass(r):
+                break
             if not self._may_admit(r, taken):
-                break                                       # the head of the queue blocks the rest
+                break                                       # who has no room blocks the rest
             # (in the queue until it has a cache: nothing is lost when there is an error)
             r.cache = self.cache.open(r.request_id) if r.prefix is None else self.cache.fork(r.prefix.holder.cache, r.request_id)
-            self.waiting.pop(0)
+            self.waiting.pop(at)
+            r.passed = r.passed or at > 0
             r.num_computed = r.cache.num_tokens
             r.status = RequestStatus.PREFILLING
             self.live.append(r)

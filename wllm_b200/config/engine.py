@@ -33,7 +33,7 @@ class EngineConfig:
     chunked_prefill_tokens: int | None = None   # token budget of one step; None = whole prompts
     prefill_row_quantum: int | None = None     # rows of a tile of the products of a step of many rows (scheduler: 'rows');
                                                # None: 256 under bfloat16 (pairs of CTAs), off under float32
-    max_num_seqs: int = 256              # requests that may be live at once (table rows, state slots)
+    max_num_seqs: int = 256              # requests that may be live at once (of a model with per-request state: they and kept prefixes)
     max_model_len: int | None = None     # None: the model's max_position_embeddings
     cuda_graphs: bool = False            # replay captured graphs for decode-only steps
     device: str = "cuda:0"

@@ -65,7 +65,8 @@ class LLM:
         self._next_id = 0
 
     def add_prefix(self, token_ids) -> Prefix:
-        """Tokens for requests to begin with (a system prompt, a document): computed once, by the steps to come, and kept until they are dropped."""
+        """Tokens for requests to begin with (a system prompt, a document): computed once, by the steps to come, and kept until they are dropped.  It takes pages, and in a model with state of every
+        request the place of one of `max_num_seqs`, of which one is left; what could not be kept beside the requests at hand is refused."""
         return self.scheduler.add_prefix(token_ids)
 
     def drop_prefix(self, prefix: Prefix) -> None:

@@ -164,3 +164,15 @@ def test_random_trees(seed):
         plan = ops.prefix_plan(b.table, b.q_lens, b.ctx_lens, ps, nkv * rep, nkv, 8, 8, dtype, min_keys=rng.choice([1, 64, 128]))
         bf16 = dtype == torch.bfloat16
         check(plan, b.table.tolist(), b.q_lens, b.ctx_lens, ps, rep, ops.prefix_rows(dtype), 1 if bf16 else 64)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,vd,shared", [(8, 1, 256, 256, True), (6, 2, 48, 48, True), (16, 4, 128, 64, False), (4, 2, 72, 72, False), (6, 2, 72, 40, False), (4, 2, 20, 20, False)])
+def test_bfloat16_layers_with_32_bit_weights_are_not_planned(nq, nkv, hd, vd, shared):
+    """Layers whose other kernels weigh values in 32 bits (values of a size of their own, head sizes that are no multiple of 16) keep them whoever shares pages beside a request."""
+    from wllm_b200.parts import MIXERS, spec
+    make = lambda dtype, **kw: MIXERS.build(spec("attention", num_heads=nq, num_kv_heads=nkv, head_dim=hd, value_dim=vd, position=spec("rope", theta=1e4, head_dim=hd), q_proj="q",  # noqa: E731
+                                                 k_proj="k", v_proj="v", o_proj="o", **kw), hidden_size=64, model_dtype=dtype)
+    held = [nq, nkv, -(-hd // 8) * 8, -(-vd // 8) * 8]
+    assert make(torch.bfloat16).prefix_layout(16) == (tuple(held) if shared else None)
+    assert make(torch.float32).prefix_layout(16) == tuple(held)
+    assert make(torch.float32, window=8).prefix_layout(16) is None and make(torch.bfloat16).prefix_layout(24) is None

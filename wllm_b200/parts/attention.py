@@ -140,9 +140,14 @@ class PagedAttention:
         return KVNeed(self.nkv, self.hd, self.window, self.vd if self.vd != self.hd else None, self.keep_first, blocks=self.blocks)
 
     def prefix_layout(self, page_size: int):
-        """(query heads, kv heads, key size, value size) for which pages that several requests hold may be read once for all of them, or None (a window, sizes that it is not built for)."""
-        ok = not self.window and ops.prefix_ok(self.nq, self.nkv, self.hd, self.vd, page_size, self.model_dtype)
+        """(query heads, kv heads, key size, value size) for which pages that several requests hold may be read once for all of them, or None: a window, sizes that it is not built for, and in
+        bfloat16 the sizes whose other kernels keep the weights of the values in 32 bits, as this one does not (a step goes by a plan as a whole, so a request would lose them by what is beside it)."""
+        ok = not self.window and ops.prefix_ok(self.nq, self.nkv, self.hd, self.vd, page_size, self.model_dtype) and not self._rounds_apart()
         return (self.nq, self.nkv, self.hd, self.vd) if ok else None
+
+    def _rounds_apart(self) -> bool:
+        """bfloat16 layers on the kernels without tensor cores."""
+        return self.model_dtype == torch.bfloat16 and (self.general or not ops.mma_head_dim_ok(self.hd))
 
     def param_specs(self):
         H, n = self.hidden_size, self.names

@@ -176,3 +176,51 @@ def test_bfloat16_layers_with_32_bit_weights_are_not_planned(nq, nkv, hd, vd, sh
     assert make(torch.bfloat16).prefix_layout(16) == (tuple(held) if shared else None)
     assert make(torch.float32).prefix_layout(16) == tuple(held)
     assert make(torch.float32, window=8).prefix_layout(16) is None and make(torch.bfloat16).prefix_layout(24) is None
+
+
+def step(sharers, others, fresh=0):
+    """(tables, new tokens, contexts, who shares): (count, new tokens, shared keys), (count, context), a whole prompt of its own; pages of 64."""
+    (count, new, shared), (more, ctx) = sharers, others
+    reqs = [(new, shared + 20 + new + 7 * i, shared) for i in range(count)] + [(1, ctx + 13 * (i % 29), 0) for i in range(more)] + ([(fresh, fresh, 0)] if fresh else [])
+    free = iter(range(shared // 64, 10 ** 6))
+    table = np.full((len(reqs), -(-max(c for _, c, _ in reqs) // 64)), -1, dtype=np.int32)
+    for r, (_, c, s) in enumerate(reqs):
+        mine = list(range(s // 64)) + [next(free) for _ in range(-(-c // 64) - s // 64)]
+        table[r, :len(mine)] = mine
+    return table, [n for n, _, _ in reqs], [c for _, c, _ in reqs], [s > 0 for _, _, s in reqs]
+
+
+F32, B16 = torch.float32, torch.bfloat16
+# steps that were timed both ways, with the faster one: (heads, kv heads, size, type), sharers, others, a fresh prompt
+TIMED = [((8, 1, 256, B16), (2, 16, 576), (0, 0), 2048, False), ((8, 1, 256, B16), (2, 1, 576), (62, 3000), 2048, False), ((16, 16, 256, B16), (2, 1, 576), (62, 3000), 2048, False),
+         ((16, 16, 256, B16), (16, 1, 1024), (62, 3000), 0, False), ((16, 16, 256, B16), (16, 1, 8192), (62, 3000), 0, True), ((8, 1, 256, B16), (16, 16, 1024), (16, 1000), 2048, True),
+         ((8, 1, 256, B16), (2, 1, 576), (0, 0), 256, True), ((16, 4, 128, B16), (2, 1, 576), (62, 3000), 2048, True), ((16, 16, 256, F32), (2, 1, 256), (62, 3000), 0, False),
+         ((16, 16, 256, F32), (16, 1, 1024), (62, 500), 0, False), ((16, 16, 256, F32), (16, 1, 1024), (0, 0), 0, True), ((16, 16, 256, F32), (4, 1, 8192), (62, 500), 0, True),
+         ((8, 1, 256, F32), (2, 1, 256), (62, 3000), 0, True), ((32, 8, 64, F32), (2, 1, 256), (16, 3000), 0, False), ((16, 16, 256, F32), (16, 1, 1024), (62, 500), 512, True)]
+
+
+@pytest.mark.parametrize("layout,sharers,others,fresh,faster", TIMED)
+def test_a_step_goes_by_its_plan_where_all_of_it_is_the_faster(layout, sharers, others, fresh, faster):
+    """Also by way of the runner, whose decision stands for everything that is in the step."""
+    from types import SimpleNamespace
+
+    from wllm_b200.engine.runner import ModelRunner
+    nq, nkv, size, dtype = layout
+    table, q_lens, ctx_lens, holds = step(sharers, others, fresh)
+    plan = ops.prefix_plan(table, q_lens, ctx_lens, 64, nq, nkv, size, size, dtype)
+    assert ops.prefix_beside(plan, q_lens, ctx_lens, holds) == faster
+    runner = object.__new__(ModelRunner)
+    runner.prefix_layouts, runner.cache, runner.model = [(0, nq, nkv, size, size)], SimpleNamespace(page_size=64), SimpleNamespace(dtype=dtype)
+    host = np.concatenate([np.array(q_lens, dtype=np.int32), np.array(ctx_lens, dtype=np.int32), table.reshape(-1)])
+    R, P = table.shape
+    offsets = {"req_q_len": (0, R), "req_ctx_len": (R, R), "table0": (2 * R, R * P)}
+    entries = [SimpleNamespace(cache=SimpleNamespace(forked=c - n if h else 0)) for n, c, h in zip(q_lens, ctx_lens, holds)]
+    pays = ops.prefix_pays(plan.saved_keys, nkv, size, size, dtype, sum(holds), sum(q_lens) / R)
+    assert bool(runner._prefix_plans(entries, host, offsets, (sum(q_lens), R, P), False)[1]) == (faster and pays)
+
+
+def test_steps_of_sharers_alone_and_small_ones_go_by_their_plan():
+    for nq, nkv, size, dtype in ((8, 1, 256, B16), (16, 16, 256, B16), (4, 2, 32, F32), (2, 2, 64, F32), (8, 1, 256, F32)):
+        for sharers in ((4, 1, 64), (3, 20, 128)):
+            table, q_lens, ctx_lens, holds = step(sharers, (0, 0))
+            assert ops.prefix_beside(ops.prefix_plan(table, q_lens, ctx_lens, 64, nq, nkv, size, size, dtype, min_keys=1), q_lens, ctx_lens, holds)

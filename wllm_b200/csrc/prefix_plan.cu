@@ -75,8 +75,8 @@ long long padded(long long n) { return (n + 3) & ~3ll; }
 // most; key_tile: keys of a tile, whole tiles make an item's range; align: segments end at multiples of it; min_keys: no shared segment is shorter; pool_pages: one past the largest
 // page number; ctas: CTAs that run at once; costs: {a tile of keys, an item beside its tiles; the same two for items of at most `thin` rows; thin; a thousand rows of results and
 // kv heads; results that a thin item of several tiles leaves}, in the caller's units; caps: {items, tokens, results, tokens of the batch} that the array is laid out for, zeros: what this plan needs (a captured
-// step's array lies at fixed places whatever the batch holds).  out [room]; info [8]: ints used, items, rows, shared keys saved (keys x further holders), most results of a
-// token, items that the batch has at the least.
+// step's array lies at fixed places whatever the batch holds).  out [room]; info [9]: ints used, items, rows, shared keys saved (keys x further holders), most results of a
+// token, tiles of rows, tokens of items, results, tiles of rows by tiles of keys.
 // Returns 0; 2: sizes that make no sense, or more than the caps hold; 4: `room` is too small (info[0] says what is needed); 7: a page number outside the pool.
 WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const int* q_len, const int* ctx_len, int page_size, int rep, int nkv, int tile_rows, int key_tile, int align,
                               int min_keys, int pool_pages, int ctas, const int* costs, const int* caps, int* out, long long room, long long* info) {
@@ -251,6 +251,8 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
         const long long at_items = PLAN_HEADER, at_tokens = at_items + padded(cap[0] * PLAN_ITEM), at_starts = at_tokens + padded(cap[1] * 2), at_results = at_starts + padded(cap[3] + 1),
                         at_positions = at_results + padded(cap[2]), used = at_positions + padded(cap[3]);
         info[0] = used; info[1] = need[0]; info[2] = rows; info[3] = saved; info[4] = most_listed; info[5] = (long long)tiles.size(); info[6] = need[1]; info[7] = results;
+        info[8] = 0;
+        for (const Alike& a : alike) info[8] += (long long)a.keys * a.count;
         if (used > 0x7fffffff) return WLLM_BAD_SIZE;
         if (used > room) return OUT_TOO_SMALL;
         std::fill(out, out + used, 0);

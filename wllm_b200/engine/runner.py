@@ -186,7 +186,7 @@ class ModelRunner:
         return host, offsets, [k for k, _ in sizes], (N, R, P), patches
 
     def _prefix_plans(self, entries: list, host, offsets, shape, fixed: bool):
-        """(host array, {layout: plan}): what the step's attention reads of shared pages, behind the index arrays; nothing where no pages are shared or it would not pay.  `fixed`: for a captured
+        """(host array, {layout: plan}): what the step's attention reads of shared pages, behind the index arrays; nothing where no pages are shared or the step would be no faster.  `fixed`: for a captured
         step, whose array lies at the same place whatever the batch holds."""
         holders = sum(e.cache.forked > 0 for e in entries)
         if not self.prefix_layouts or holders < 2:
@@ -206,6 +206,8 @@ class ModelRunner:
             plan = ops.prefix_plan(view(f"table{g}").reshape(R, P), lens, ctx_lens, self.cache.page_size, nq, nkv, hd, vd, self.model.dtype,
                                    caps=ops.prefix_caps(R, nkv) if fixed else None)
             if plan is None or not ops.prefix_pays(plan.saved_keys, nkv, hd, vd, self.model.dtype, holders, tokens) or plan.scratch_floats > PREFIX_SCRATCH:
+                continue
+            if not ops.prefix_beside(plan, view("req_q_len")[:len(entries)], view("req_ctx_len")[:len(entries)], [e.cache.forked > 0 for e in entries], P * self.cache.page_size if fixed else None):
                 continue
             plans[layout] = plan
             offsets[("prefix", layout)] = (total, plan.used)

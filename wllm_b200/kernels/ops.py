@@ -777,15 +777,16 @@ def _numbers(values) -> list:
 
 class PrefixPlan:
     """How a batch whose requests share pages is attended to (csrc/prefix_plan.cuh): made once for a step and a layout of heads, read by every layer of it."""
-    __slots__ = ("key", "requests", "width", "n_tokens", "host", "used", "items", "rows", "saved_keys", "most_results", "tiles", "max_chunks", "scratch_floats", "launch", "places")
+    __slots__ = ("key", "requests", "width", "n_tokens", "host", "used", "items", "rows", "saved_keys", "most_results", "tiles", "key_tiles", "max_chunks", "scratch_floats", "launch", "places")
 
-    def __init__(self, key: tuple, requests: int, width: int, caps, host: torch.Tensor, used: int, items: int, rows: int, saved: int, most: int, tiles: int, n_tokens: int, max_ctx: int,
+    def __init__(self, key: tuple, requests: int, width: int, caps, host: torch.Tensor, used: int, items: int, rows: int, saved: int, most: int, tiles: int, key_tiles: int, n_tokens: int, max_ctx: int,
                  at_items: int, at_tokens: int, at_positions: int):
         if caps is not None:          # laid out for any plan of that size: the kernels read from it how many items there are
             n_tokens, rows, max_ctx = caps[3], caps[2] * (key[1] // key[2]), width * key[0]
         self.key, self.requests, self.width, self.n_tokens = key, requests, width, n_tokens
         self.host = host                       # int32 on the host (more than 64 KB of it pinned, where there is a device)
         self.used, self.items, self.rows, self.saved_keys, self.most_results, self.tiles = used, items, rows, saved, most, tiles
+        self.key_tiles = key_tiles             # tiles of rows by the tiles of keys (128 in bfloat16, 64 in 32 bits) that each of them meets
         page_size, nq, nkv, hd, vd, dtype = key
         self.max_chunks = max(1, -(-max_ctx // SIMT_CHUNK))
         self.scratch_floats = nkv * rows * (vd + 2) if dtype == torch.bfloat16 else n_tokens * nq * self.max_chunks * (vd + 2)
@@ -850,6 +851,40 @@ def prefix_pays(saved_keys: int, nkv: int, hd: int, vd: int, dtype: torch.dtype,
     if item == 2 and tokens > 1:
         return saved_keys >= (holders - 1) * max(PREFIX_PORTION[0], PREFIX_PORTION[1] * tokens * nkv) > 0
     return saved_keys * nkv * (hd + vd) * item >= PREFIX_SAVED[item]
+
+
+def simt_by_chunks_of_rows(rows: int, chunks: int) -> bool:
+    """Whether single tokens' attention without tensor cores goes by (row, chunk of keys), into scratch, rather than a warp per row."""
+    return chunks > 1 and rows <= 4096 and rows * chunks <= 65536
+
+
+def prefix_beside(plan: PrefixPlan, q_lens, ctx_lens, holds, max_ctx: int | None = None) -> bool:
+    """Whether a step as a whole is the faster by its plan, which takes also the requests that share nothing.  Arrays by request: new tokens, contexts, whether it holds shared pages; `max_ctx`: the bound
+    on contexts that the other attention is launched with.  An estimate in us of a layer on either side, over steps of 2 to 32 requests on 256 to 8,192 shared keys beside 0 to 200 others of 500 to 3,000:
+    32 bits, single tokens.  A plan's item costs 32 rows whatever it has, the other attention goes row by row: 0.37 ns a row and key of heads of 256, twice that where it has no scratch for chunks, and no
+      less than its longest row; a plan 1.25 ns a kv head and key of an item.  So plans win where query heads share keys, and lose beside many requests of few rows a kv head (us, the other attention
+      and the plan: 2 on 256 beside 62 on 3,000, 8 heads of 256 on one 555 and 264, 16 on 16 1,104 and 3,271, 32 on 8 of 64 beside 16 170 and 202; 16 on 1,024 alone, 16 on 16 107 and 70).
+      Portions of several tokens go 32 rows at a time either way, and plans were never the slower ones.
+    bfloat16 heads of 256.  The other attention has portions on pairs of CTAs, at twice the plan's rate, and reads keys at 5 % more: 1.4 us a million (token, key, head)s of portions that share
+      nothing, 10 us a GB of keys; a plan saves the step's second kernel, 0.1 us a MB read less and 1.5 us a sharing portion (us, the other attention and the plan: 8 heads on one, 2 portions of 16 on 576
+      beside a fresh one of 2,048 37 and 48, 16 on 1,024 beside it and 16 others 81 and 54; 16 on 16, 16 on 1,024 beside 62 on 3,000 466 and 495).  Other heads' plans were 2 % slower at the most."""
+    page_size, nq, nkv, hd, vd, dtype = plan.key
+    if dtype == torch.bfloat16 and hd != 256:
+        return True
+    q_lens, ctx_lens, holds = (np.asarray(x) for x in (q_lens, ctx_lens, holds))
+    if dtype == torch.float32:
+        if q_lens.max() > 1:
+            return True
+        longest, size = int(ctx_lens.max()), (hd + vd) / 512
+        other = 0.37e-3 * size * nq * float(ctx_lens.sum())
+        if not simt_by_chunks_of_rows(nq * len(q_lens), simt_chunks(longest if max_ctx is None else max_ctx, 0)):
+            other = max(2 * other, (0.15 + 0.17 * size) * longest)
+        return (0.2 + 1.05 * size) * 1e-3 * nkv * SIMT_CHUNK * plan.key_tiles <= other + 6
+    several, apart = q_lens > 1, ~holds.astype(bool)
+    keys = q_lens.astype(np.float64) * (ctx_lens - q_lens / 2)
+    lost = 1.4e-6 * nq * keys[apart & several].sum() + 10e-9 * nkv * (hd + vd) * 2 * float(ctx_lens[apart].sum())
+    won = 4 + 0.1e-6 * plan.saved_keys * nkv * (hd + vd) * 2 + 1.5 * float((several & ~apart).sum())
+    return bool(won >= lost)
 
 
 def prefix_caps(requests: int, nkv: int) -> tuple:

@@ -331,7 +331,7 @@ class PagedAttention:
                 return
             rows, chunks = q.shape[0] * nq, ops.simt_chunks(ctx.max_ctx, window, self.keep_first)
             scratch = None
-            if chunks > 1 and rows <= 4096 and rows * chunks <= 65536:
+            if ops.simt_by_chunks_of_rows(rows, chunks):
                 scratch = ctx.buffer(self.tag + "attention_chunks", (rows * chunks * (self.vd + 2),), torch.float32)
             ops.paged_attention_simt(q, out, k_pages, v_pages, ctx.token_req, ctx.positions, table, nq, nkv, hd, ps,
                                      window, scale, scratch, chunks, **extra)

@@ -224,3 +224,12 @@ def test_steps_of_sharers_alone_and_small_ones_go_by_their_plan():
         for sharers in ((4, 1, 64), (3, 20, 128)):
             table, q_lens, ctx_lens, holds = step(sharers, (0, 0))
             assert ops.prefix_beside(ops.prefix_plan(table, q_lens, ctx_lens, 64, nq, nkv, size, size, dtype, min_keys=1), q_lens, ctx_lens, holds)
+
+
+def test_pages_past_the_pools_are_refused():
+    table = np.array([[3, 1, 9, -7], [3, 1, 2, 99]], dtype=np.int32)       # (99 holds no key)
+    plan = ops.prefix_plan(table, [1, 1], [48, 40], 16, 2, 1, 64, min_keys=1)
+    assert plan.top_page == 9 and ops.prefix_plan(table, [1, 1], [16, 33], 16, 2, 1, 64).top_page == 3 and ops.prefix_plan(table, [0, 0], [0, 0], 16, 2, 1, 64).top_page == -1
+    q, pages = torch.zeros(2, 128, dtype=torch.bfloat16), torch.zeros(9, 1, 16, 64, dtype=torch.bfloat16)
+    with pytest.raises(ops.KernelError, match="page 9 of a pool of 9"):
+        ops.prefix_attention(q, q, pages, pages, torch.from_numpy(table), plan, plan.host, 2, 1, 64, 16, 0.1, torch.zeros(plan.scratch_floats))

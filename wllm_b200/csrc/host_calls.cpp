@@ -458,7 +458,7 @@ PyObject* copy_pages(Args v, Py_ssize_t n) {
 }
 
 // tables, q_lens, ctx_lens, page_size, query heads a kv head, kv heads, rows of an item, keys of a tile, align, min_keys, CTAs at once, pinned memory, costs (seven), caps (four)
-//   -> (status, the plan's array, ints used, items, rows, keys saved, most results, tiles of rows, those by tiles of keys, tokens, longest context, the places of items, tokens and positions in the array)
+//   -> (status, the plan's array, ints used, items, rows, keys saved, most results, tiles of rows, those by tiles of keys, largest page, tokens, longest context, the places of items, tokens and positions in the array)
 PyObject* prefix_plan(Args v, Py_ssize_t n) {
     count(n, 14);
     const std::vector<int> costs = numbers(v[12], "costs", 7), caps = numbers(v[13], "caps", 4);
@@ -490,7 +490,7 @@ PyObject* prefix_plan(Args v, Py_ssize_t n) {
     long long tokens = 0, longest = 0;
     for (int x : q) tokens += x;
     for (int x : ctx) longest = x > longest ? x : longest;
-    long long info[9] = {0}, room = 8192 + 64 * (tokens > 0 ? tokens : 0) + 8LL * caps[0] + 2LL * caps[1] + caps[2] + 2LL * caps[3];
+    long long info[10] = {0}, room = 8192 + 64 * (tokens > 0 ? tokens : 0) + 8LL * caps[0] + 2LL * caps[1] + caps[2] + 2LL * caps[3];
     static thread_local std::vector<int> made;
     PyObject* status = nullptr;
     for (int go = 0; go < 2; ++go) {
@@ -508,7 +508,7 @@ PyObject* prefix_plan(Args v, Py_ssize_t n) {
     at::Tensor host = at::empty({sound ? (int64_t)info[0] : 0}, at::TensorOptions().dtype(at::kInt).pinned_memory(truth(v[11]) && info[0] > (64 << 10) / 4));
     if (sound) std::copy(made.begin(), made.begin() + info[0], static_cast<int*>(host.data_ptr()));
     const int *head = made.data(), at_items = sound ? head[PLAN_AT_ITEMS] : 0, at_tokens = sound ? head[PLAN_AT_TOKENS] : 0, at_positions = sound ? head[PLAN_AT_POSITIONS] : 0;
-    return Py_BuildValue("(NNLLLLLLLLLiii)", status, THPVariable_Wrap(host), info[0], info[1], info[2], info[3], info[4], info[5], info[8], tokens, longest, at_items, at_tokens, at_positions);
+    return Py_BuildValue("(NNLLLLLLLLLLiii)", status, THPVariable_Wrap(host), info[0], info[1], info[2], info[3], info[4], info[5], info[8], info[9], tokens, longest, at_items, at_tokens, at_positions);
 }
 
 // q, out, k_pages, v_pages, block_table, arrays, scratch, status, sinks, slopes, tokens, requests, width, ints of the plan, floats of scratch, rows, pairs, place of the positions,

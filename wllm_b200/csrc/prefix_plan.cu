@@ -75,8 +75,8 @@ long long padded(long long n) { return (n + 3) & ~3ll; }
 // most; key_tile: keys of a tile, whole tiles make an item's range; align: segments end at multiples of it; min_keys: no shared segment is shorter; pool_pages: one past the largest
 // page number; ctas: CTAs that run at once; costs: {a tile of keys, an item beside its tiles; the same two for items of at most `thin` rows; thin; a thousand rows of results and
 // kv heads; results that a thin item of several tiles leaves}, in the caller's units; caps: {items, tokens, results, tokens of the batch} that the array is laid out for, zeros: what this plan needs (a captured
-// step's array lies at fixed places whatever the batch holds).  out [room]; info [9]: ints used, items, rows, shared keys saved (keys x further holders), most results of a
-// token, tiles of rows, tokens of items, results, tiles of rows by tiles of keys.
+// step's array lies at fixed places whatever the batch holds).  out [room]; info [10]: ints used, items, rows, shared keys saved (keys x further holders), most results of a
+// token, tiles of rows, tokens of items, results, tiles of rows by tiles of keys, the largest page number (-1: none).
 // Returns 0; 2: sizes that make no sense, or more than the caps hold; 4: `room` is too small (info[0] says what is needed); 7: a page number outside the pool.
 WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const int* q_len, const int* ctx_len, int page_size, int rep, int nkv, int tile_rows, int key_tile, int align,
                               int min_keys, int pool_pages, int ctas, const int* costs, const int* caps, int* out, long long room, long long* info) {
@@ -104,12 +104,14 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
             p.segments.push_back({(int)p.members.size(), 1, p.cover[r], ctx_len[r], true});
             p.members.push_back(r);
         }
+        long long last_page = -1;
         for (const Segment& s : p.segments) {             // (shared pages are looked at once)
             const int* held = tables + p.members[s.first] * width;
             const int end = (int)((s.key_hi + (long long)page_size - 1) / page_size);
             unsigned top = 0;                             // (a number below zero is a large one)
             for (int i = s.key_lo / page_size; i < end; ++i) top = std::max(top, (unsigned)held[i]);
             if (top >= (unsigned)pool_pages) return PAGES_OUT_OF_RANGE;
+            if (s.key_hi > s.key_lo) last_page = std::max<long long>(last_page, top);
         }
         // tiles of rows: whole tokens of a segment's requests, one behind the other
         const int per_tile = tile_rows / rep;
@@ -253,6 +255,7 @@ WLLM_API int wllm_prefix_plan(const int* tables, long long width, int R, const i
         info[0] = used; info[1] = need[0]; info[2] = rows; info[3] = saved; info[4] = most_listed; info[5] = (long long)tiles.size(); info[6] = need[1]; info[7] = results;
         info[8] = 0;
         for (const Alike& a : alike) info[8] += (long long)a.keys * a.count;
+        info[9] = last_page;
         if (used > 0x7fffffff) return WLLM_BAD_SIZE;
         if (used > room) return OUT_TOO_SMALL;
         std::fill(out, out + used, 0);

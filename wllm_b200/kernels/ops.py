@@ -777,9 +777,9 @@ def _numbers(values) -> list:
 
 class PrefixPlan:
     """How a batch whose requests share pages is attended to (csrc/prefix_plan.cuh): made once for a step and a layout of heads, read by every layer of it."""
-    __slots__ = ("key", "requests", "width", "n_tokens", "host", "used", "items", "rows", "saved_keys", "most_results", "tiles", "key_tiles", "max_chunks", "scratch_floats", "launch", "places")
+    __slots__ = ("key", "requests", "width", "n_tokens", "host", "used", "items", "rows", "saved_keys", "most_results", "tiles", "key_tiles", "top_page", "max_chunks", "scratch_floats", "launch", "places")
 
-    def __init__(self, key: tuple, requests: int, width: int, caps, host: torch.Tensor, used: int, items: int, rows: int, saved: int, most: int, tiles: int, key_tiles: int, n_tokens: int, max_ctx: int,
+    def __init__(self, key: tuple, requests: int, width: int, caps, host: torch.Tensor, used: int, items: int, rows: int, saved: int, most: int, tiles: int, key_tiles: int, top_page: int, n_tokens: int, max_ctx: int,
                  at_items: int, at_tokens: int, at_positions: int):
         if caps is not None:          # laid out for any plan of that size: the kernels read from it how many items there are
             n_tokens, rows, max_ctx = caps[3], caps[2] * (key[1] // key[2]), width * key[0]
@@ -787,6 +787,7 @@ class PrefixPlan:
         self.host = host                       # int32 on the host (more than 64 KB of it pinned, where there is a device)
         self.used, self.items, self.rows, self.saved_keys, self.most_results, self.tiles = used, items, rows, saved, most, tiles
         self.key_tiles = key_tiles             # tiles of rows by the tiles of keys (128 in bfloat16, 64 in 32 bits) that each of them meets
+        self.top_page = top_page               # the largest page number in it
         page_size, nq, nkv, hd, vd, dtype = key
         self.max_chunks = max(1, -(-max_ctx // SIMT_CHUNK))
         self.scratch_floats = nkv * rows * (vd + 2) if dtype == torch.bfloat16 else n_tokens * nq * self.max_chunks * (vd + 2)
@@ -918,13 +919,15 @@ def prefix_plan(tables, q_lens, ctx_lens, page_size: int, nq: int, nkv: int, hd:
 def prefix_attention(q, out, k_pages, v_pages, block_table, plan: PrefixPlan, arrays: torch.Tensor, nq: int, nkv: int, hd: int, page_size: int, scale: float, scratch: torch.Tensor,
                      vd: int | None = None, sinks: torch.Tensor | None = None, cap: float = 0.0, slopes: torch.Tensor | None = None) -> None:
     """Attention of a planned batch (csrc/prefix_attention.cu; 32-bit: csrc/attention_simt.cu, bit for bit what the other 32-bit kernels give): q [tokens, nq * hd] (row stride free),
-    out [tokens, nq * vd], pages [pages, nkv, page_size, hd | vd], `block_table` [requests, pages] the tables of the plan on the device, `arrays` = plan.to(device) (or its numbers copied
+    out [tokens, nq * vd], pages [pages, nkv, page_size, hd | vd], `block_table` [requests, pages] the tables of the plan on the device (whose pages lie in the pools), `arrays` = plan.to(device) (or its numbers copied
     from the host into an array of their own: they are looked at before the kernel in front has ended, so no kernel may be what writes them), `scratch` float32 of at least plan.scratch_floats, which the
     call alone uses while it runs.  A new value that is no number reaches all new tokens of its own request.  Every earlier key is seen (no window).  `sinks`, `cap`, `slopes`: as for attention_mma_decode."""
     if plan.key != (page_size, nq, nkv, hd, hd if vd is None else vd, q.dtype):
         raise KernelError(f"prefix_attention: a plan for (page size, heads, kv heads, sizes, type) {plan.key}, not {(page_size, nq, nkv, hd, hd if vd is None else vd, q.dtype)}")
     if plan.n_tokens == 0:
         return
+    if plan.top_page >= k_pages.shape[0]:
+        raise KernelError(f"prefix_attention: the plan's tables name page {plan.top_page} of a pool of {k_pages.shape[0]}")
     status = _host_calls().prefix_attention(q, out, k_pages, v_pages, block_table, arrays, scratch, _device_status(q.device), sinks, slopes, *plan.launch, scale, cap, sm_count(), *plan.places)
     if status:
         _check(status, f"prefix_attention(head_dim={hd}/{vd}, heads={nq}/{nkv})")

@@ -353,16 +353,19 @@ def test_any_mixture_comes_to_an_end(seed):
 @pytest.mark.parametrize("states,most", [((), 4), (("state",), 3)])
 def test_prefixes_cost_requests_of_models_without_state_no_place(states, most):
     """Four samples of a prompt run at once where four requests do, beside the prompt; one request at a time may have a prefix."""
-    from types import SimpleNamespace
+    import torch
 
-    from wllm_b200.engine.build import request_slots
-    model = SimpleNamespace(state_specs=list(states))
-    runner = FakeRunner(40, max_requests=request_slots(model, 4))
-    s = Scheduler(runner, ArgmaxSampler(), max_num_seqs=4)
-    reqs, live = samples_of(s, 0, list(range(10)), 4, 6), 0
+    from wllm_b200.cache import CacheGroupSpec, CacheManager, StateSpec
+
+    def scheduler(requests):
+        runner = FakeRunner(40)
+        runner.cache = CacheManager([CacheGroupSpec("all", 1, 1, 8)], 4, 40, requests, [StateSpec(n, (3,), torch.float32) for n in states], prefix_slots=requests)
+        assert runner.cache.slots.num_free == requests
+        return Scheduler(runner, ArgmaxSampler(), max_num_seqs=requests)
+    s, live = scheduler(4), 0
+    reqs = samples_of(s, 0, list(range(10)), 4, 6)
     while s.has_unfinished():
         s.step()
         live = max(live, len(s.live))
-    assert live == most and all(r.output_token_ids == alone(r.prompt_token_ids, 6) for r in reqs)
-    s = Scheduler(FakeRunner(40, max_requests=request_slots(model, 1)), ArgmaxSampler(), max_num_seqs=1)
-    assert (s.prefix_refusal(5) is None) == (not states)
+    assert live == most and all(r.output_token_ids == alone(r.prompt_token_ids, 6) for r in reqs) and s.cache.slots.num_free == 4
+    assert (scheduler(1).prefix_refusal(5) is None) == (not states)

@@ -156,12 +156,14 @@ class CacheGroup:
 
 
 class StateSlots:
-    """Rows of fixed-size per-request state: tensor `name` has shape [num_slots, *shape]."""
+    """Rows of fixed-size per-request state: tensor `name` has shape [num_slots, *shape].  `spare`: more slots beside those of the requests, for prefixes that are kept; there
+    are none where a slot is memory."""
 
-    def __init__(self, num_slots: int, specs: list, device):
+    def __init__(self, num_slots: int, specs: list, device, spare: int = 0):
         self.num_slots, self.specs = num_slots, list(specs)
-        self._free = list(range(num_slots - 1, -1, -1))
-        self._held = [False] * num_slots
+        self.total = num_slots + (0 if self.specs else spare)
+        self._free = list(range(self.total - 1, -1, -1))
+        self._held = [False] * self.total
         self.tensors = {}
         if device is not None:
             for s in specs:
@@ -169,7 +171,8 @@ class StateSlots:
 
     @property
     def num_free(self) -> int:
-        return len(self._free)
+        """Requests that may still take one."""
+        return min(self.num_slots, len(self._free))
 
     def take(self, zero: bool = True) -> int:
         if not self._free:
@@ -193,15 +196,15 @@ class StateSlots:
 
 class CacheManager:
     def __init__(self, groups: list, page_size: int, num_pages: int, max_requests: int, states: list = (),
-                 dtype=torch.bfloat16, device=None, poison: bool = False):
-        """`poison` (a debugging aid; the tests switch it on): pools start as NaN instead of zeros and every
+                 dtype=torch.bfloat16, device=None, poison: bool = False, prefix_slots: int = 0):
+        """`prefix_slots`: slots beside those of `max_requests` requests, for prefixes (none if there is per-request state, where they take the requests').  `poison` (a debugging aid; the tests switch it on): pools start as NaN instead of zeros and every
         page is filled with NaN again when it is given back, so a kernel that reads a slot that was never
         written, or a page that its request no longer holds, shows at once in the logits."""
         if page_size < 1:
             raise ValueError("page_size must be positive")
         self.page_size = page_size
         self.groups = [CacheGroup(g, num_pages, page_size, dtype, device, poison) for g in groups]
-        self.slots = StateSlots(max_requests, list(states), device)
+        self.slots = StateSlots(max_requests, list(states), device, prefix_slots)
         self.live: dict = {}
         self.dtype, self.device = dtype, device
         self.pages_high_water = [0] * len(self.groups)

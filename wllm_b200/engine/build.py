@@ -39,17 +39,11 @@ def build_model(folder: str | None, dtype, device, config=None, random_seed: int
     return model
 
 
-def request_slots(model: ComposedModel, max_num_seqs: int) -> int:
-    """Slots of a cache for that many requests at once.  A prefix that is kept has one too: where a slot is a number alone there are as many again for prefixes; where it is memory
-    (state of every request), prefixes take them from the requests."""
-    return max_num_seqs if model.state_specs else 2 * max_num_seqs
-
-
 def build_runner(model: ComposedModel, engine: EngineConfig, num_pages: int | None = None,
                  poison_pages: bool = False) -> ModelRunner:
     device = require_cuda(engine.device)
     cache = CacheManager(model.group_specs, page_size=engine.block_size,
                          num_pages=num_pages if num_pages is not None else engine.num_blocks,
-                         max_requests=request_slots(model, engine.max_num_seqs), states=model.state_specs, dtype=model.dtype, device=device,
+                         max_requests=engine.max_num_seqs, prefix_slots=engine.max_num_seqs, states=model.state_specs, dtype=model.dtype, device=device,
                          poison=poison_pages)
     return ModelRunner(model, cache, device)

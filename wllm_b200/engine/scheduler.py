@@ -138,8 +138,8 @@ class Scheduler:
     def prefix_refusal(self, num_tokens: int, prefix: Prefix | None = None, worst_tokens: int = 0) -> str | None:
         """Why a prefix of that many tokens cannot be kept beside what was taken on, or None: with its pages held, some unfinished request, or one of `worst_tokens` that is to begin with
         it, could never finish."""
-        if len(self.prefixes) + 1 >= self.cache.slots.num_slots:
-            return f"{len(self.prefixes)} prefixes and {self.cache.slots.num_slots} requests at most: none would be left"
+        if len(self.prefixes) + 1 >= self.cache.slots.total:
+            return f"{len(self.prefixes)} prefixes, and {self.cache.slots.total} of them and requests at most: none would be left"
         ps = self.cache.page_size
         own = self._pages(num_tokens) - (len(prefix.token_ids) // ps if prefix is not None else 0)
         need = max(self.largest_need(), self._held_pages() + self._pages(min(worst_tokens, self.max_model_len)) - num_tokens // ps) + own

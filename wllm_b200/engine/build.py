@@ -5,6 +5,7 @@ import torch
 
 from ..cache import CacheManager
 from ..config import EngineConfig, config_from_folder, resolve_architecture
+from ..kernels import ops
 from ..kernels.build import KernelBuildError
 from ..weights import fill_random, load_weights
 from .model import ComposedModel
@@ -46,4 +47,7 @@ def build_runner(model: ComposedModel, engine: EngineConfig, num_pages: int | No
                          num_pages=num_pages if num_pages is not None else engine.num_blocks,
                          max_requests=engine.max_num_seqs, prefix_slots=engine.max_num_seqs, states=model.state_specs, dtype=model.dtype, device=device,
                          poison=poison_pages)
-    return ModelRunner(model, cache, device)
+    runner = ModelRunner(model, cache, device)
+    for _, _, _, hd, vd in runner.prefix_layouts:
+        ops.prefix_prepare(hd, vd, model.dtype)
+    return runner

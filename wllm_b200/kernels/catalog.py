@@ -32,8 +32,8 @@ FAMILIES = {
     # tensor-core attention is built per head size; others are built when a model first asks
     "attention_mma": [{"HEAD_DIM": 256}, {"HEAD_DIM": 32}, {"HEAD_DIM": 48}],
     "attention_decode_static": [{"HEAD_DIM": 256}],
-    # and so is attention over shared prefixes, per key and value head size
-    "prefix_attention": [{"HEAD_DIM": 256, "VALUE_DIM": 256}, {"HEAD_DIM": 128, "VALUE_DIM": 128}],
+    # and so is attention over shared prefixes, per key and value head size (others when a model that may use it is loaded)
+    "prefix_attention": [{"HEAD_DIM": d, "VALUE_DIM": d} for d in (256, 128, 32, 48)],
     # attention over latent rows on the tensor cores is built per row and value size, when a model first asks
     "latent_attention_mma": [],
 }

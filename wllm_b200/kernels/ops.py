@@ -888,6 +888,13 @@ def prefix_beside(plan: PrefixPlan, q_lens, ctx_lens, holds, max_ctx: int | None
     return bool(won >= lost)
 
 
+def prefix_prepare(hd: int, vd: int, dtype: torch.dtype) -> None:
+    """Builds and loads what prefix_attention takes for heads of these sizes, so that no step waits for a compiler."""
+    if dtype == torch.bfloat16:
+        _host_calls()
+        _bind((hd, vd))
+
+
 def prefix_caps(requests: int, nkv: int) -> tuple:
     """Sizes that the plan of a captured step of that many requests is laid out for (one token each): items for two turns of every multiprocessor beside four a request."""
     return 2 * sm_count() // nkv + 4 * requests, 6 * requests, 24 * requests + 512, requests

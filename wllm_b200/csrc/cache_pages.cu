@@ -9,6 +9,7 @@
 // one contiguous run (a page of one layer, or one head's slots of it where not all of them are copied) with 16-byte loads, all of a thread's in flight before the
 // first is stored.  Moves happen in no order: no destination may be named twice or be a source of the same pool, which the entry point checks.
 #include "common.cuh"
+#include "cache_pages.cuh"
 
 #include <new>
 #include <vector>
@@ -59,14 +60,6 @@ copy_pages_kernel(const __grid_constant__ PageMoves<MOVES> p, int piece) {
 }
 
 enum { PAGES_OUT_OF_RANGE = 7, PAGES_TWICE = 8, POOLS_OVERLAP = 9 };
-
-// One pool and its moves, as the caller gives them
-struct PagePoolMoves {
-    const void* src;
-    void* dst;
-    long long outer, src_pages, dst_pages, heads, slots, row_bytes, moves;
-    const int *src_list, *dst_list, *slot_list;      // slot_list null: whole pages
-};
 
 static bool apart(const void* a, long long na, const void* b, long long nb) {
     return (const char*)a + na <= (const char*)b || (const char*)b + nb <= (const char*)a;

@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <vector>
 
+#include "cache_pages.cuh"
 #include "prefix_plan.cuh"
 
 namespace {
@@ -151,12 +152,6 @@ typedef int (*PrefixFn)(const void*, int, void*, int, const void*, const void*, 
                         int, int, int, float*, long long, long long, int, int*, void*);
 typedef int (*PrefixSimtFn)(const void*, int, void*, int, const void*, const void*, int, const int*, int, int, int, int, int, int, int, float, float, const float*, const float*,
                             const int*, const int*, float*, int, long long, int, void*);
-struct PagePoolMoves {                 // as csrc/cache_pages.cu has it
-    const void* src;
-    void* dst;
-    long long outer, src_pages, dst_pages, heads, slots, row_bytes, moves;
-    const int *src_list, *dst_list, *slot_list;
-};
 typedef int (*CopyPagesFn)(const PagePoolMoves*, int, int, int*, void*);
 
 GemmFn gemm_fn;

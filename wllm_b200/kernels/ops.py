@@ -818,7 +818,9 @@ def _pinning() -> bool:
 def _prefix_costs(dtype: torch.dtype, hd: int, vd: int) -> tuple:
     """What a plan weighs, in cycles: a tile of keys and an item beside its tiles, for items of many rows and for those of at most 16, which run on other instructions; those 16; a
     thousand rows of results, the results of a thin item of several tiles.  bfloat16: the tensor core's products (100 cycles a step of 16 for the scores, 85 for 128 columns of the output), but no less than a group's turn with three
-    buffers, or two, takes; thin items at 44 bytes a cycle and SM, but no less than their chain.  32 bits: 32 rows by 64 keys on the FMA pipes."""
+    buffers, or two, takes; a thin item's tile 44 bytes a cycle, but no less than its chain.  The weights are fitted to the times of whole plans, not to a tile's own: a thin tile takes longer where all SMs read at
+    once (memory gives each 23 bytes a cycle), but weighed so it would leave longer ranges and an end with fewer SMs at work (15 batches: 4.5 % longer, 8 x 8 on 4,000 tokens 127 us a layer for 103; every weight a third less or
+    more 0.5 % shorter to 3 % longer).  32 bits: 32 rows by 64 keys on the FMA pipes."""
     if dtype == torch.float32:
         return 24 * (hd + vd), 4000, 24 * (hd + vd), 4000, 0, 4 * vd, 1
     out = -(-vd // 64) * 64

@@ -233,3 +233,26 @@ def test_pages_past_the_pools_are_refused():
     q, pages = torch.zeros(2, 128, dtype=torch.bfloat16), torch.zeros(9, 1, 16, 64, dtype=torch.bfloat16)
     with pytest.raises(ops.KernelError, match="page 9 of a pool of 9"):
         ops.prefix_attention(q, q, pages, pages, torch.from_numpy(table), plan, plan.host, 2, 1, 64, 16, 0.1, torch.zeros(plan.scratch_floats))
+
+
+def test_no_plan_is_made_where_the_best_one_would_not_do(monkeypatch):
+    """What a plan can save at most is known without it."""
+    for layout, sharers, others, fresh, faster in TIMED:
+        nq, nkv, size, dtype = layout
+        table, q_lens, ctx_lens, holds = step(sharers, others, fresh)
+        plan = ops.prefix_plan(table, q_lens, ctx_lens, 64, nq, nkv, size, size, dtype, min_keys=1)
+        forked = [c - n if h else 0 for n, c, h in zip(q_lens, ctx_lens, holds)]
+        bound = ops.PrefixBound(plan.key, ctx_lens, forked)
+        assert bound.saved_keys >= plan.saved_keys and bound.key_tiles <= plan.key_tiles
+        assert ops.prefix_beside(bound, q_lens, ctx_lens, holds) or not faster
+    from types import SimpleNamespace
+
+    from wllm_b200.engine.runner import ModelRunner
+    runner = object.__new__(ModelRunner)
+    runner.prefix_layouts, runner.cache, runner.model = [(0, 16, 16, 256, 256)], SimpleNamespace(page_size=64), SimpleNamespace(dtype=F32)
+    table, q_lens, ctx_lens, holds = step((2, 1, 256), (62, 3000))
+    host = np.concatenate([np.array(q_lens, dtype=np.int32), np.array(ctx_lens, dtype=np.int32), table.reshape(-1)])
+    R, P = table.shape
+    monkeypatch.setattr(ops, "prefix_plan", lambda *a, **k: pytest.fail("a plan was made"))
+    entries = [SimpleNamespace(cache=SimpleNamespace(forked=256 if h else 0)) for h in holds]
+    assert not runner._prefix_plans(entries, host, {"req_q_len": (0, R), "req_ctx_len": (R, R), "table0": (2 * R, R * P)}, (R, R, P), False)[1]

@@ -197,17 +197,15 @@ class ModelRunner:
             o, n = offsets[name]
             return host[o:o + n]
         lens, ctx_lens, total = view("req_q_len").tolist(), view("req_ctx_len").tolist(), host.shape[0]
-        tokens = sum(lens) / len(entries)
+        tokens, forked, ps = sum(lens) / len(entries), [e.cache.forked for e in entries], self.cache.page_size
+        step = (view("req_q_len")[:len(entries)], view("req_ctx_len")[:len(entries)], [f > 0 for f in forked], P * ps if fixed else None)
         for layout in self.prefix_layouts:
             g, nq, nkv, hd, vd = layout
-            saved = sum(e.cache.forked for e in entries)          # (no more keys than that can be shared)
-            if not ops.prefix_pays(saved, nkv, hd, vd, self.model.dtype, holders, tokens):
+            pays = lambda keys: ops.prefix_pays(keys, nkv, hd, vd, self.model.dtype, holders, tokens)  # noqa: E731
+            if not pays(sum(forked)) or not ops.prefix_beside(ops.PrefixBound((ps, nq, nkv, hd, vd, self.model.dtype), step[1], forked), *step):
                 continue
-            plan = ops.prefix_plan(view(f"table{g}").reshape(R, P), lens, ctx_lens, self.cache.page_size, nq, nkv, hd, vd, self.model.dtype,
-                                   caps=ops.prefix_caps(R, nkv) if fixed else None)
-            if plan is None or not ops.prefix_pays(plan.saved_keys, nkv, hd, vd, self.model.dtype, holders, tokens) or plan.scratch_floats > PREFIX_SCRATCH:
-                continue
-            if not ops.prefix_beside(plan, view("req_q_len")[:len(entries)], view("req_ctx_len")[:len(entries)], [e.cache.forked > 0 for e in entries], P * self.cache.page_size if fixed else None):
+            plan = ops.prefix_plan(view(f"table{g}").reshape(R, P), lens, ctx_lens, ps, nq, nkv, hd, vd, self.model.dtype, caps=ops.prefix_caps(R, nkv) if fixed else None)
+            if plan is None or not pays(plan.saved_keys) or plan.scratch_floats > PREFIX_SCRATCH or not ops.prefix_beside(plan, *step):
                 continue
             plans[layout] = plan
             offsets[("prefix", layout)] = (total, plan.used)

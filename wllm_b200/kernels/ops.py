@@ -861,8 +861,17 @@ def simt_by_chunks_of_rows(rows: int, chunks: int) -> bool:
     return chunks > 1 and rows <= 4096 and rows * chunks <= 65536
 
 
-def prefix_beside(plan: PrefixPlan, q_lens, ctx_lens, holds, max_ctx: int | None = None) -> bool:
-    """Whether a step as a whole is the faster by its plan, which takes also the requests that share nothing.  Arrays by request: new tokens, contexts, whether it holds shared pages; `max_ctx`: the bound
+class PrefixBound:
+    """What a plan can save and has to read at best, known without making it: `forked`, the tokens below which each request may share pages."""
+    __slots__ = ("key", "saved_keys", "key_tiles")
+
+    def __init__(self, key: tuple, ctx_lens, forked):
+        self.key, self.saved_keys = key, sum(forked) - max(forked)
+        self.key_tiles = int((np.asarray(ctx_lens) - np.asarray(forked)).sum()) // (128 if key[5] == torch.bfloat16 else SIMT_CHUNK)
+
+
+def prefix_beside(plan, q_lens, ctx_lens, holds, max_ctx: int | None = None) -> bool:
+    """Whether a step as a whole is the faster by its plan (or may be by one within a PrefixBound), which takes also the requests that share nothing.  Arrays by request: new tokens, contexts, whether it holds shared pages; `max_ctx`: the bound
     on contexts that the other attention is launched with.  An estimate in us of a layer on either side, over steps of 2 to 32 requests on 256 to 8,192 shared keys beside 0 to 200 others of 500 to 3,000:
     32 bits, single tokens.  A plan's item costs 32 rows whatever it has, the other attention goes row by row: 0.37 ns a row and key of heads of 256, twice that where it has no scratch for chunks, and no
       less than its longest row; a plan 1.25 ns a kv head and key of an item.  So plans win where query heads share keys, and lose beside many requests of few rows a kv head (us, the other attention
@@ -872,7 +881,7 @@ def prefix_beside(plan: PrefixPlan, q_lens, ctx_lens, holds, max_ctx: int | None
       nothing, 10 us a GB of keys; a plan saves the step's second kernel, 0.1 us a MB read less and 1.5 us a sharing portion (us, the other attention and the plan: 8 heads on one, 2 portions of 16 on 576
       beside a fresh one of 2,048 37 and 48, 16 on 1,024 beside it and 16 others 81 and 54; 16 on 16, 16 on 1,024 beside 62 on 3,000 466 and 495).  Other heads' plans were 2 % slower at the most."""
     page_size, nq, nkv, hd, vd, dtype = plan.key
-    if dtype == torch.bfloat16 and hd != 256:
+    if dtype == torch.bfloat16 and (hd != 256 or all(holds)):
         return True
     q_lens, ctx_lens, holds = (np.asarray(x) for x in (q_lens, ctx_lens, holds))
     if dtype == torch.float32:

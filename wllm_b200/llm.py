@@ -74,7 +74,8 @@ class LLM:
         self.scheduler.drop_prefix(prefix)
 
     def resize_cache(self, num_blocks: int) -> None:
-        """Another number of cache blocks: what is live moves to the front of the new pools.  Refused where a request that was taken on could not finish."""
+        """Another number of cache blocks: what is live moves to the front of the new pools.  Refused where a request that was taken on could not finish (ValueError), or what is
+        live now holds more (OutOfPages); everything is as it was then."""
         need = self.scheduler.largest_need()
         if need > num_blocks:
             raise ValueError(f"{num_blocks} blocks: the requests and prefixes at hand need {need}")

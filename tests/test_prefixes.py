@@ -369,3 +369,27 @@ def test_prefixes_cost_requests_of_models_without_state_no_place(states, most):
         live = max(live, len(s.live))
     assert live == most and all(r.output_token_ids == alone(r.prompt_token_ids, 6) for r in reqs) and s.cache.slots.num_free == 4
     assert (scheduler(1).prefix_refusal(5) is None) == (not states)
+
+
+def test_adding_many_prompts_with_samples_is_no_work_of_its_own():
+    """What the requests in the queue need beside each other's prompts is added up once a prompt, not prompt by prompt for every request: 64 and 128 prompts, in lines that the interpreter runs."""
+    import sys
+
+    def steps(prompts):
+        s, count = Scheduler(FakeRunner(20000, max_requests=2000), ArgmaxSampler()), 0
+
+        def trace(frame, event, arg):
+            nonlocal count
+            count += event == "line"
+            return trace
+        for i in range(prompts):
+            if i == prompts - 1:
+                sys.settrace(trace)
+            try:
+                assert not s.prefix_refusal(9, None, 14)
+                samples_of(s, i, [(i + j) % 50 for j in range(10)], 4, 4)
+            finally:
+                sys.settrace(None)
+        return count
+    few, many = steps(64), steps(128)
+    assert many < 3 * few                                             # (proportional to the queue; by every pair of a request and a prompt it would be four times)

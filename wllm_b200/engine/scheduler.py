@@ -54,6 +54,7 @@ Policy, with the reference's rule beside it:
 from __future__ import annotations
 
 import random
+from bisect import bisect_left
 
 from ..cache import OutOfPages
 from ..sampling.params import SamplingParams
@@ -118,21 +119,38 @@ class Scheduler:
         request.seed = request.sampling.seed if request.sampling.seed is not None else self._rng.getrandbits(63)
         self.waiting.append(request)
 
-    def _held_pages(self, request: Request | None = None, passing: bool = False) -> int:
+    def _own_pages(self, x: Prefix) -> int:
+        """Pages of a prefix beside the full pages of the one that it begins with."""
+        return self._pages(len(x.token_ids)) - (len(x.holder.prefix.token_ids) // self.cache.page_size if x.holder.prefix is not None else 0)
+
+    def _held(self) -> tuple:
+        """(pages of all prefixes, for those that were made for a few: the places in the queue at which they were added, sums of the pages of all in front of each)."""
+        total, orders, sums = 0, [], [0]
+        for x in self.prefixes:                  # in the order in which they were added
+            own = self._own_pages(x)
+            total += own
+            if x.auto:
+                orders.append(x.holder.order)
+                sums.append(sums[-1] + own)
+        return total, orders, sums
+
+    def _held_pages(self, request: Request | None = None, passing: bool = False, held: tuple | None = None) -> int:
         """Pages that prefixes hold, or will, when `request` has run so far that it is the only one left, and which it does not share: not the full pages of its own, nor what was made for a
-        few requests in front of it (they are live in front of it or over, unless it has passed them)."""
-        passing = passing or request is None or request.passed
-        total, mine, x = 0, [], request.prefix if request is not None else None
-        while x is not None:                     # its prefix, what that begins with, ...
-            mine.append(x)
+        few requests in front of it (they are live in front of it or over, unless it has passed them).  `held`: what `_held` says, if it was asked."""
+        total, orders, sums = held or self._held()
+        if request is None:
+            return total
+        skip = 0 if passing or request.passed else bisect_left(orders, request.order)
+        total -= sums[skip]
+        x = request.prefix
+        if x is not None:
+            total -= len(x.token_ids) // self.cache.page_size
+        while x is not None:                     # its prefix, what that begins with, ...: held as long as it runs
+            if skip and x.auto:
+                total += self._own_pages(x)
             x = x.holder.prefix
-        for x in self.prefixes:
-            if x.holder is request or (not passing and x.auto and x.holder.order < request.order and x not in mine):
-                continue
-            shared = len(x.holder.prefix.token_ids) // self.cache.page_size if x.holder.prefix is not None else 0
-            total += self._pages(len(x.token_ids)) - shared
-        if request is not None and request.prefix is not None:
-            total -= len(request.prefix.token_ids) // self.cache.page_size
+        if request.holds and request.order >= 0:
+            total -= sum(self._own_pages(x) for x in self.prefixes if x.holder is request)
         return total
 
     def prefix_refusal(self, num_tokens: int, prefix: Prefix | None = None, worst_tokens: int = 0) -> str | None:
@@ -328,7 +346,8 @@ class Scheduler:
 
     def largest_need(self) -> int:
         """Pages that the largest unfinished request may come to hold, beside what prefixes do."""
-        return max((self._pages(min(r.worst_case_tokens, self.max_model_len)) + self._held_pages(r) for r in self.waiting + self.live), default=self._held_pages())
+        held = self._held()
+        return max((self._pages(min(r.worst_case_tokens, self.max_model_len)) + self._held_pages(r, held=held) for r in self.waiting + self.live), default=held[0])
 
     def _finish(self) -> None:
         for r in [r for r in self.live if r.finished]:
